@@ -143,6 +143,95 @@ int kta_decode_gqa_bf16_noalloc(const void* Q, const void* Kc, const void* Vc,
                                 int64_t Hq, int64_t Hkv, int64_t D, int64_t cache_tokens,
                                 int64_t max_seqlen, float scale, void* stream);
 
+/* --- Paged KV cache ------------------------------------------------------------------------
+ * Caches Kc, Vc [num_blocks, block_size, Hkv, D] row-major; a request's tokens lie in the blocks
+ * that its row of the block table names, token p in slot table[p / block_size] * block_size +
+ * p % block_size. These entries have no counterpart in the reference, whose decode case reads a
+ * contiguous cache (perfmodel/testset/gen.py:493-590).
+ *
+ * kta_cache_slots: one step's bookkeeping on the device. For request b with context_lens[b]
+ * tokens in the cache and new_lens[b] more to come (int32 [B]), it takes the blocks they need
+ * beyond the ceil(context / block_size) held from the front of free_blocks (int32 [num_free]),
+ * requests in order, writes them into block_tables (int32 [B, max_blocks], row stride
+ * table_stride elements; other entries are not touched), and lists the new tokens request after
+ * request: slots (int64 [max_tokens]), positions (int32 [max_tokens]), offsets (int32 [B + 1],
+ * request b's rows are offsets[b] .. offsets[b + 1]) and used (int32 [1], blocks taken). Rows past
+ * the last token get slot -1 and position 0. Checked on the device, each recorded as
+ * KTA_ERR_DEVICE_BOUNDS: a request with a negative length or more tokens than its table's row
+ * holds is listed without new tokens; blocks past num_free are entered as -1, and their tokens'
+ * slots are -1; tokens past max_tokens are cut off (offsets end at max_tokens). B <= 2048,
+ * max_blocks * block_size < 2^31, max_tokens <= 2^30. The free list must not overlap the
+ * tables. */
+int kta_cache_slots(const void* context_lens, const void* new_lens, void* block_tables,
+                    const void* free_blocks, void* slots, void* positions, void* offsets, void* used,
+                    int64_t B, int64_t max_blocks, int64_t table_stride, int64_t num_free,
+                    int64_t block_size, int64_t max_tokens, void* stream);
+
+/* Rotary positions. Y = X with each pair (a, b) of a row's first `rot` dimensions turned by
+ * t = positions[n] * freqs[i]: scale * (a cos t - b sin t, b cos t + a sin t); pair i is
+ * (i, i + rot/2), or (2i, 2i + 1) with `interleaved`; dimensions from rot on are copied.
+ * `inverse` turns by -t: the gradient with respect to X of the same call. X, Y [tokens, heads, D]
+ * with token and head strides in elements (X's may be 0: one row for all); positions int32 or
+ * int64 (pos_bytes 4 or 8, any sign), freqs fp64 [rot / 2] finite radians per position. The angle
+ * is reduced exactly for any position. X and Y may be the same tensor, and must not overlap
+ * otherwise. D % 16 == 0, D <= 1024, rot % 16 == 0, strides multiples of 8, 16-byte aligned X, Y. */
+int kta_rope_f16(const void* X, const void* positions, int64_t pos_bytes, const void* freqs, void* Y,
+                 int64_t tokens, int64_t heads, int64_t D, int64_t rot, int64_t x_token,
+                 int64_t x_head, int64_t y_token, int64_t y_head, int interleaved, int inverse,
+                 float scale, void* stream);
+int kta_rope_bf16(const void* X, const void* positions, int64_t pos_bytes, const void* freqs, void* Y,
+                  int64_t tokens, int64_t heads, int64_t D, int64_t rot, int64_t x_token,
+                  int64_t x_head, int64_t y_token, int64_t y_head, int interleaved, int inverse,
+                  float scale, void* stream);
+
+/* The same for a step's Q [tokens, Hq, D] and K [tokens, Hkv, D] at once: Qo = rotated Q, and the
+ * rotated K and the V go to slots[n] (int64 [tokens]) of the caches Kc, Vc (num_slots =
+ * num_blocks * block_size rows of [Hkv, D]). A negative slot leaves the caches alone; one past
+ * num_slots does too and is recorded as KTA_ERR_DEVICE_BOUNDS; two tokens with one slot leave
+ * either's values there. `strides` points to eight host int64 values, token and head stride of Q,
+ * K, V and Qo in elements (slices of one fused tensor will do). Qo may be Q; the caches overlap
+ * no input. */
+int kta_rope_cache_f16(const void* Q, const void* K, const void* V, const void* positions,
+                       int64_t pos_bytes, const void* slots, const void* freqs, void* Qo, void* Kc,
+                       void* Vc, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t D, int64_t rot,
+                       const int64_t* strides, int64_t num_slots, int interleaved, float scale,
+                       void* stream);
+int kta_rope_cache_bf16(const void* Q, const void* K, const void* V, const void* positions,
+                        int64_t pos_bytes, const void* slots, const void* freqs, void* Qo, void* Kc,
+                        void* Vc, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t D, int64_t rot,
+                        const int64_t* strides, int64_t num_slots, int interleaved, float scale,
+                        void* stream);
+
+/* Attention of a tree of drafted tokens over the paged cache. Request b has context_lens[b]
+ * cached tokens and offsets[b + 1] - offsets[b] <= max_new <= 64 drafted ones, whose K and V
+ * already stand behind them in the cache; its rows of Q, O [tokens, Hq, D] and LSE [tokens, Hq]
+ * are offsets[b] .. offsets[b + 1] (int32 [B + 1]). Row i sees every cached token, and drafted
+ * token j iff bit j of tree[i] (int64 [tokens]) is set; without a tree (NULL) the drafted tokens
+ * are a chain, and one drafted token is a decode step. O = softmax(scale Q K^T) V over what a row
+ * sees, LSE = natural log of the sum; a row that sees nothing has O = 0 and LSE = -inf; values of
+ * tokens that a row does not see do not reach it, infinities and NaN included. Rows that belong to
+ * no request are left as they were. Q's token stride is q_token elements, its heads are D apart.
+ * block_tables int32 [B, max_blocks], row stride table_stride. Checked on the device, recorded as
+ * KTA_ERR_DEVICE_BOUNDS: a request whose offsets or lengths are out of range (more than max_new
+ * drafted tokens, more tokens than its table's row holds) gets O = 0 and LSE = -inf; a block id
+ * outside [0, num_blocks) reads as zeros. D = 64 or 128, Hq / Hkv <= 16, block_size a power of two
+ * from 8 to 256, B <= 65536, max_blocks * block_size <= 2^30, num_blocks * block_size * Hkv < 2^31.
+ * `workspace`: kta_tree_attn_workspace_bytes(...) bytes, 16-byte aligned, of any contents; calls
+ * that may run at the same time (two streams, two graphs) need one each. */
+size_t kta_tree_attn_workspace_bytes(int64_t max_new, int64_t Hq, int64_t Hkv, int64_t D);
+int kta_tree_attn_f16(const void* Q, const void* Kc, const void* Vc, const void* block_tables,
+                      const void* context_lens, const void* offsets, const void* tree, void* O,
+                      void* LSE, int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                      int64_t q_token, int64_t num_blocks, int64_t block_size, int64_t max_blocks,
+                      int64_t table_stride, int64_t max_new, float scale, void* workspace,
+                      size_t ws_bytes, void* stream);
+int kta_tree_attn_bf16(const void* Q, const void* Kc, const void* Vc, const void* block_tables,
+                       const void* context_lens, const void* offsets, const void* tree, void* O,
+                       void* LSE, int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                       int64_t q_token, int64_t num_blocks, int64_t block_size, int64_t max_blocks,
+                       int64_t table_stride, int64_t max_new, float scale, void* workspace,
+                       size_t ws_bytes, void* stream);
+
 /* GEMM with a 4-bit B dequantised in the main loop: C [M, N] f16 = A [M, K] f16 . B^T with
  * B[n, k] = decode(nibble k of Bq[n, :]) * Sc[n, k / group] rounded to f16; Bq [N, K/2] bytes,
  * two elements per byte, the lower nibble first; Sc [N, K/group] f16; fp32 accumulate.

@@ -1,0 +1,963 @@
+// Attention of a tree of drafted tokens over a paged KV cache, sm_100a.
+//
+//   For request b with c = ctx[b] tokens in the cache and t drafted ones behind them (rows
+//   offsets[b] .. offsets[b + 1] of Q, keys c .. c + t - 1 of the cache, t <= 64):
+//   row i sees key p iff p < c, or bit p - c of tree[i] is set (p - c < t);
+//   O = softmax(scale Q K^T over the seen keys) V,  LSE = log of the sum, natural.
+//
+// One drafted token is the decode step of a paged cache; a chain is the tree 1, 11, 111, ...
+//
+//   * A KV head's query rows of one request (tokens x heads of the group, up to 128 in a row
+//     tile) share its K and V, so they are the rows of one tcgen05 tile: S = Q K^T is 128 x 128
+//     per 128 keys however few of them are real. At 128 rows the tensor core needs ~1000 cycles
+//     for a tile of keys, the softmax ~1500 and the HBM stream ~2800 (64 KB at an SM's share), so
+//     the padding of few rows is free and one kernel serves from 1 to 128 rows at HBM speed.
+//   * Work is the list of 128-key tiles of every (request, KV head), in contiguous ranges of
+//     equal length, one range per CTA (or per `row_tiles` CTAs with a row tile each, which then
+//     read the same K and V at about the same time: the second reader finds them in L2). Ragged
+//     lengths balance to a tile; what a range cuts is joined by a second small kernel from fp32
+//     partials (O, maximum, sum) in the workspace: no counters to keep at zero between calls.
+//   * Six roles in 192 threads: warps 0-3 softmax (thread = query row = TMEM lane), warp 4 TMA
+//     producer, warp 5 TMEM owner and MMA issuer. K and V tiles share a ring of six slots in the
+//     order the tensor core takes them, K(0) K(1) V(0) K(2) V(1) ...: S of the next tile is
+//     computed while the softmax works, in the other of two S buffers.
+//   * Pages: a box of the tensor map is one page (up to 128 tokens) of one head, with the token
+//     index split as (8, page / 8): shared memory gets 8-token groups of both 64-wide halves of
+//     the head, [group][half][8 tokens][128 B], which for every page size is one uniform stride
+//     for the matrix descriptors and one TMA per page. Lane i of the producer loads page i.
+//   * The last tile of a request ends inside a page: K's leftover columns are masked by
+//     selection, and V's leftover rows are set to zero in shared memory, since 0 * NaN from a
+//     page's unwritten rows would reach every row through the matrix product. Likewise a drafted
+//     V row that is not finite is zeroed and handed to the rows that see it alone.
+//   * Out-of-range lengths, offsets and block ids become status KTA_ERR_DEVICE_BOUNDS: such a
+//     request's rows are zero (LSE -inf), such a block reads as zeros. Every wait is bounded.
+#include <algorithm>
+#include <cmath>
+
+#include "kta_common.cuh"
+#include "kta_host.h"
+
+namespace kta {
+namespace tree {
+
+constexpr int BM = 128;               // query rows of a row tile: TMEM lanes
+constexpr int BN = 128;               // keys of a tile
+constexpr int RING = 6;               // K and V tiles in flight
+constexpr int SOFTMAX_WARPS = 4;
+constexpr int PRODUCER_WARP = 4;
+constexpr int MMA_WARP = 5;
+constexpr int NUM_THREADS = 192;
+constexpr int MAX_DRAFT = 64;         // bits of a row of the tree
+constexpr int MAX_GROUP = 16;
+constexpr int MAX_BATCH = 1 << 16;
+constexpr int MAX_CTAS = 256;         // the workspace is sized for this many
+constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units: the maximum moves when it grew > 2^8
+constexpr uint32_t COL_O = 256;       // TMEM: S of buffer t at t * 128, O at 256
+
+enum : unsigned int {
+  SITE_PROD_SLOT = 0x901,
+  SITE_PROD_Q = 0x902,
+  SITE_MMA_Q = 0x903,
+  SITE_MMA_KV = 0x904,
+  SITE_MMA_P = 0x905,
+  SITE_MMA_OFREE = 0x906,
+  SITE_SM_S = 0x907,
+  SITE_SM_V = 0x908,
+  SITE_SM_PV = 0x909,
+  SITE_SM_O = 0x90A,
+  SITE_REQUEST = 0x911,  // lengths or offsets out of range
+  SITE_BLOCK = 0x912,    // a block id out of range
+};
+
+template <int D>
+struct Layout {
+  static constexpr int HALVES = D / 64;
+  static constexpr int GROUP = HALVES * 1024;      // 8 tokens: [half][8][128 B]
+  static constexpr int TILE = BN / 8 * GROUP;      // a K or V tile
+  static constexpr int Q_HALF = BM * 128;          // [128 rows][64 d]
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_RING = OFF_Q + HALVES * Q_HALF;
+  static constexpr int OFF_BAR = OFF_RING + RING * TILE;
+  // ring_full[R], ring_empty[R], q_full, q_empty, s_full[2], p_full[2], pv_done, o_done, o_free
+  static constexpr int NUM_BARS = 2 * RING + 9;
+  static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
+  // misc: tmem base, abort, the range's first request and pair start, non-finite drafts
+  static constexpr int TOTAL = OFF_MISC + 64;
+  static constexpr int ALLOC = TOTAL + 1024;
+  static_assert(ALLOC <= 232448, "shared memory budget of one sm_100 CTA");
+};
+
+// What the join kernel needs of a unit that starts in a CTA's range and ends in a later one.
+struct Desc {
+  int count;    // ranges that hold a part of it; 0: none
+  int slot;     // the first part's slot (the others are slot 0 of their CTA)
+  int row;      // first query token
+  int tokens;
+  int kvh;
+  int pad[3];
+};
+
+struct Params {
+  const int32_t* ctx;      // [B]
+  const int32_t* offsets;  // [B + 1]
+  const int64_t* tree;     // [rows] or nullptr: a chain
+  const int32_t* tables;   // [B, max_blocks]
+  void* out;               // [rows, Hq, D]
+  float* lse;              // [rows, Hq]
+  const void* v;           // the V cache, for drafted rows that are not finite
+  Desc* desc;              // [CTAs]
+  float2* part_ml;         // [2 CTAs][row_cap] (maximum, sum), log2 units
+  float4* part_o;          // [2 CTAs][D / 4][row_cap], not normalised
+  long long table_stride;
+  int batch, rows, hq, hkv, group, max_new, max_blocks, num_blocks;
+  int page_log2;           // tokens of a block
+  int box_log2;            // tokens of a TMA box: min(block, 128)
+  int tok_tile;            // drafted tokens of a row tile: 128 / group
+  int box_tokens;          // tokens of the Q box: min(tok_tile, max_new)
+  int row_tiles;           // CTAs that share a range
+  int row_cap;             // rows of a partial
+  float scale_log2;        // softmax scale * log2(e)
+  unsigned int* status;
+};
+
+__device__ __forceinline__ void tma_load_5d(const CUtensorMap* map, uint64_t* bar, void* dst, int32_t x,
+                                            int32_t y, int32_t z, int32_t w, int32_t v) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
+      : "memory");
+}
+
+struct Request {
+  int row, tokens, ctx, len;  // first row, drafted tokens, cached tokens, both
+  bool bad;
+};
+
+__device__ __forceinline__ Request request_of(const Params& p, int b) {
+  const int a = p.offsets[b], z = p.offsets[b + 1], c = p.ctx[b];
+  Request r;
+  const long long room = static_cast<long long>(p.max_blocks) << p.page_log2;
+  const long long t = static_cast<long long>(z) - a;
+  r.bad = a < 0 || t < 0 || z > p.rows || t > p.max_new || c < 0 || c + t > room;
+  r.row = a;
+  r.tokens = r.bad ? 0 : static_cast<int>(t);
+  r.ctx = c;
+  r.len = r.bad ? 0 : c + r.tokens;
+  return r;
+}
+
+// Tiles of keys of a request: none without a query row.
+__device__ __forceinline__ int tiles_of(const Request& r) {
+  return r.tokens > 0 ? (r.len + BN - 1) / BN : 0;
+}
+
+// The work list: tile i of KV head h of request b, b-major; range k of n is
+// [total k / n, total (k + 1) / n), and n <= total, so that none is empty.
+struct Ranges {
+  long long total;
+  int n;
+  __device__ __forceinline__ long long start(int k) const { return total * k / n; }
+  __device__ __forceinline__ int owner(long long t) const {
+    return static_cast<int>(((t + 1) * n - 1) / total);
+  }
+};
+
+// A range's walk over its segments: runs of tiles [i0, i1) of one (request, KV head).
+struct Walk {
+  Request rq;
+  int b, kvh, i0, i1, tiles;
+  long long t, end;
+
+  __device__ __forceinline__ void open(const Params& p, int b_first, long long b_start, long long from,
+                                       long long to) {
+    b = b_first;
+    t = from;
+    end = to;
+    rq = request_of(p, b);
+    tiles = tiles_of(rq);
+    const long long rel = from - b_start;
+    kvh = static_cast<int>(rel / tiles);
+    i0 = static_cast<int>(rel - static_cast<long long>(kvh) * tiles);
+    i1 = static_cast<int>(min(static_cast<long long>(tiles), i0 + (end - t)));
+  }
+  __device__ __forceinline__ bool more() const { return t < end; }
+  __device__ __forceinline__ void next(const Params& p) {
+    t += i1 - i0;
+    if (t >= end) return;
+    i0 = 0;
+    if (++kvh == p.hkv) {
+      kvh = 0;
+      do {  // tiles are left before `end`, so a request with some follows
+        rq = request_of(p, ++b);
+        tiles = tiles_of(rq);
+      } while (tiles == 0);
+    }
+    i1 = static_cast<int>(min(static_cast<long long>(tiles), end - t));
+  }
+  // Drafted tokens of row tile rt in the request: 0 where it has fewer.
+  __device__ __forceinline__ int tokens(const Params& p, int rt) const {
+    return max(0, min(rq.tokens - rt * p.tok_tile, p.tok_tile));
+  }
+};
+
+// Bits lo .. lo + 31 of a row's view of the keys, lo = first key of the word less ctx: cached
+// keys (negative) are all seen, drafted ones by the row's bits.
+__device__ __forceinline__ uint32_t view_word(uint64_t bits, int lo) {
+  if (lo <= -32) return 0xffffffffu;
+  if (lo < 0) return (0xffffffffu >> (32 + lo)) | static_cast<uint32_t>(bits << -lo);
+  return lo < 64 ? static_cast<uint32_t>(bits >> lo) : 0u;
+}
+
+// One S tile of one query row (this thread's TMEM lane): P = 2^(S sl - m) over the first 64
+// columns of S, the running maximum m (log2 units) and the row sum l. m moves only when the true
+// maximum grew by more than 2^8, so O is rescaled rarely; that waits for the PV before it.
+template <bool MASKED, bool BF16, int D>
+__device__ __forceinline__ bool softmax_step(uint32_t t_s, uint32_t t_o, const uint32_t (&view)[4],
+                                             float sl, float& m_used, float& lsum, uint64_t* pv_done,
+                                             uint32_t pv_parity, volatile int* abort,
+                                             unsigned int* status) {
+  uint32_t r[BN];
+#pragma unroll
+  for (int q = 0; q < BN / 32; ++q) {
+    tmem_ld_32x32b_x32(t_s + q * 32, *reinterpret_cast<uint32_t(*)[32]>(r + q * 32));
+  }
+  tmem_ld_wait();
+  reg_fence(r);
+  if (MASKED) {
+#pragma unroll
+    for (int c = 0; c < BN; ++c) {
+      if (!((view[c / 32] >> (c % 32)) & 1u)) r[c] = __float_as_uint(-INFINITY);
+    }
+  }
+  float mx[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) mx[i] = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < BN / 2; ++i) {
+    mx[i & 7] = max3(mx[i & 7], __uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+  }
+  const float rmax = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]),
+                          fmaxf(mx[6], mx[7])) * sl;
+  float factor = 1.f;
+  bool rescale = false;
+  if (rmax > m_used + RESCALE_THRESHOLD) {
+    factor = ex2(m_used - rmax);  // 0 where nothing was seen so far
+    rescale = m_used != -INFINITY;
+    m_used = rmax;
+  }
+  lsum *= factor;
+  if (__any_sync(0xffffffffu, rescale)) {
+    // The PV of the tile before (parity pv_parity). The one before that is complete, since this
+    // tile's S was issued behind it, so the barrier is at most one phase behind.
+    if (!mbar_wait(pv_done, pv_parity, abort, status, SITE_SM_PV)) return false;
+    tc_fence_after();
+    const float f = rescale ? factor : 1.f;
+#pragma unroll 1
+    for (int c = 0; c < D; c += 32) {
+      uint32_t o[32];
+      tmem_ld_32x32b_x32(t_o + c, o);
+      tmem_ld_wait();
+      reg_fence(o);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+      tmem_st_32x32b_x32(t_o + c, o);
+    }
+  }
+  // a row that has seen nothing keeps m = -inf: subtract 0 there, every exponential is 2^-inf
+  const float m = m_used == -INFINITY ? 0.f : m_used;
+  const uint64_t sl2 = f2(sl, sl);
+  const uint64_t neg2 = f2(-m, -m);
+  uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t pk[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int c = h * 64 + 2 * i;
+      const uint64_t x = fma2(f2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sl2, neg2);
+      float x0, x1;
+      f2_split(x, x0, x1);
+      const float e0 = ex2(x0), e1 = ex2(x1);
+      sum2[i & 3] = add2(sum2[i & 3], f2(e0, e1));
+      pk[i] = pack2<BF16>(e0, e1);
+    }
+    tmem_st_32x32b_x32(t_s + h * 32, pk);
+  }
+  tmem_st_wait();
+  const uint64_t s01 = add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3]));
+  float s0, s1;
+  f2_split(s01, s0, s1);
+  lsum += s0 + s1;
+  return true;
+}
+
+// 16-bit elements of a word whose exponent is all ones (infinities and NaN), as a mask of them.
+template <bool BF16>
+__device__ __forceinline__ uint32_t nonfinite(uint32_t w) {
+  constexpr uint32_t E = BF16 ? 0x7F80u : 0x7C00u;
+  return ((w & E) == E ? 0xffffu : 0u) | ((w >> 16 & E) == E ? 0xffff0000u : 0u);
+}
+
+// The V tile (shared memory, base `tile`) whose rows [first, valid) are drafted tokens: rows past
+// `valid` become zero, and so do drafted elements that are not finite, whose tokens are recorded
+// in bad[0..1] (bit row - first + bit0). The four softmax warps share the rows.
+template <bool BF16, int D>
+__device__ __forceinline__ void clean_v(uint8_t* tile, int first, int valid, int bit0, int tid,
+                                        unsigned int* bad) {
+  constexpr int CHUNKS = D / 8;  // 16-byte pieces of a row
+  first = max(first, 0);
+  for (int i = tid + first * CHUNKS; i < BN * CHUNKS; i += SOFTMAX_WARPS * 32) {
+    const int row = i / CHUNKS, ch = i % CHUNKS;
+    uint4* at = reinterpret_cast<uint4*>(tile + (row >> 3) * Layout<D>::GROUP + (ch >> 3) * 1024 +
+                                         (row & 7) * 128 + (ch & 7) * 16);
+    if (row >= valid) {
+      *at = make_uint4(0u, 0u, 0u, 0u);
+      continue;
+    }
+    const uint4 u = *at;
+    const uint4 n = make_uint4(nonfinite<BF16>(u.x), nonfinite<BF16>(u.y), nonfinite<BF16>(u.z),
+                               nonfinite<BF16>(u.w));
+    if ((n.x | n.y | n.z | n.w) != 0u) {
+      *at = make_uint4(u.x & ~n.x, u.y & ~n.y, u.z & ~n.z, u.w & ~n.w);
+      const int bit = row - first + bit0;
+      atomicOr(bad + (bit >> 5), 1u << (bit & 31));
+    }
+  }
+}
+
+template <bool BF16>
+__device__ __forceinline__ float load16(const void* base, long long i) {
+  if constexpr (BF16) {
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i]);
+  } else {
+    return __half2float(static_cast<const __half*>(base)[i]);
+  }
+}
+
+template <bool BF16, int D>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+    tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                const __grid_constant__ CUtensorMap tmV, const Params p) {
+  using L = Layout<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* ring_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
+  uint64_t* ring_empty = ring_full + RING;
+  uint64_t* q_full = ring_empty + RING;
+  uint64_t* q_empty = q_full + 1;    // the segment's last S has read Q
+  uint64_t* s_full = q_empty + 1;    // [buffer]
+  uint64_t* p_full = s_full + 2;     // [buffer]: P written, V cleaned
+  uint64_t* pv_done = p_full + 2;    // one phase for each PV
+  uint64_t* o_done = pv_done + 1;    // the segment's last PV
+  uint64_t* o_free = o_done + 1;     // the epilogue has read O
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
+  unsigned int* bad = reinterpret_cast<unsigned int*>(smem + L::OFF_MISC + 8);   // [2]
+  volatile int* first_b = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 16);
+  volatile long long* first_t = reinterpret_cast<volatile long long*>(smem + L::OFF_MISC + 24);
+  long long* warp_sum = reinterpret_cast<long long*>(smem + L::OFF_RING);        // before the ring is used
+
+  const int warp = warp_id();
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < RING; ++s) {
+      mbar_init(&ring_full[s], 1);
+      mbar_init(&ring_empty[s], 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], SOFTMAX_WARPS);
+    }
+    mbar_init(pv_done, 1);
+    mbar_init(o_done, 1);
+    mbar_init(o_free, SOFTMAX_WARPS);
+    *abort_flag = 0;
+    bad[0] = bad[1] = 0u;
+    fence_barrier_init();
+  }
+  if (warp == PRODUCER_WARP && lane == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == MMA_WARP) {
+    tmem_alloc(tmem_holder, 512);
+    tmem_relinquish();
+  }
+  pdl_wait();  // the previous grid's writes (this launch's inputs) are visible from here on
+  // after the wait: the join kernel may be scheduled now, and waits for this grid itself
+  pdl_launch_dependents();
+
+  // ---- tiles before each request: thread i sums a run of requests ----
+  const int per = (p.batch + NUM_THREADS - 1) / NUM_THREADS;
+  const int b0 = min(static_cast<int>(threadIdx.x) * per, p.batch), b1 = min(b0 + per, p.batch);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += static_cast<long long>(tiles_of(request_of(p, b))) * p.hkv;
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  long long before = incl - mine;
+  Ranges rg;
+  rg.total = 0;
+#pragma unroll
+  for (int w = 0; w < NUM_THREADS / 32; ++w) {
+    if (w < warp) before += warp_sum[w];
+    rg.total += warp_sum[w];
+  }
+  rg.n = static_cast<int>(min(static_cast<long long>(gridDim.x / p.row_tiles), rg.total));
+  const int range = blockIdx.x / p.row_tiles, rt = blockIdx.x % p.row_tiles;
+  const bool busy = range < rg.n;
+  const long long t_begin = busy ? rg.start(range) : 0, t_end = busy ? rg.start(range + 1) : 0;
+  if (busy && t_begin >= before && t_begin < before + mine) {
+    long long t = before;
+    for (int b = b0; b < b1; ++b) {
+      const long long k = static_cast<long long>(tiles_of(request_of(p, b))) * p.hkv;
+      if (t_begin < t + k) {
+        *first_b = b;
+        *first_t = t;
+        break;
+      }
+      t += k;
+    }
+  }
+  // requests that are out of range: their rows that exist become zero
+  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    if (!request_of(p, b).bad) continue;
+    if (threadIdx.x == 0) record_status(p.status, KTA_ERR_DEVICE_BOUNDS, SITE_REQUEST);
+    const long long a = max(p.offsets[b], 0), z = min(p.offsets[b + 1], p.rows);
+    const long long words = (z - a) * p.hq * (D / 2);
+    uint32_t* o = static_cast<uint32_t*>(p.out) + a * p.hq * (D / 2);
+    for (long long i = threadIdx.x; i < words; i += NUM_THREADS) o[i] = 0u;
+    for (long long i = threadIdx.x; i < (z - a) * p.hq; i += NUM_THREADS) p.lse[a * p.hq + i] = -INFINITY;
+  }
+  fence_proxy_async_smem();  // the scan's use of the ring's memory comes before its TMA writes
+  __syncthreads();
+  Walk w;
+  w.t = w.end = 0;
+  if (busy) w.open(p, *first_b, *first_t, t_begin, t_end);
+
+  if (warp == PRODUCER_WARP) {
+    // ------------------------------ TMA producer ------------------------------
+    uint32_t n = 0;  // loads into the ring so far
+    uint32_t qphase = 0;
+    bool ok = true;
+    const int box = 1 << p.box_log2;
+    const int pages = BN >> p.box_log2;              // boxes of a tile
+    const int split = p.page_log2 - p.box_log2;      // log2 of boxes in a block
+    const int group_box = box / 8;
+    // the index of the page's first (token, head) row, for this lane's page of tile i
+    auto page_of = [&](const Walk& s, int i) -> int {
+      const int box_index = i * pages + lane;
+      if (lane >= pages || (static_cast<long long>(box_index) << p.box_log2) >= s.rq.len) return 0;
+      const int id = p.tables[s.b * p.table_stride + (box_index >> split)];
+      if (id < 0 || id >= p.num_blocks) {
+        record_status(p.status, KTA_ERR_DEVICE_BOUNDS, SITE_BLOCK);
+        return p.num_blocks * p.hkv << p.page_log2;  // past the tensor: reads as zeros
+      }
+      return (id * p.hkv << p.page_log2) + s.kvh;
+    };
+    auto load = [&](const Walk& s, int i, int first, const CUtensorMap* map) -> bool {
+      const int st = static_cast<int>(n % RING);
+      if (!mbar_wait(&ring_empty[st], ((n / RING) & 1u) ^ 1u, abort_flag, p.status, SITE_PROD_SLOT)) {
+        return false;
+      }
+      ++n;
+      const int held = min(pages, (s.rq.len - i * BN + box - 1) >> p.box_log2);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&ring_full[st], static_cast<uint32_t>(held * group_box * L::GROUP));
+      }
+      __syncwarp();
+      if (lane < held) {
+        const int g = ((i * pages + lane) & ((1 << split) - 1)) * group_box;
+        tma_load_5d(map, &ring_full[st], smem + L::OFF_RING + st * L::TILE + lane * group_box * L::GROUP,
+                    0, 0, 0, g, first);
+      }
+      __syncwarp();
+      return true;
+    };
+    for (; w.more() && ok; w.next(p)) {
+      const int tokens = w.tokens(p, rt);
+      if (tokens == 0) continue;
+      int cur = page_of(w, w.i0);
+      int nxt = w.i0 + 1 < w.i1 ? page_of(w, w.i0 + 1) : 0;
+      if (!load(w, w.i0, cur, &tmK)) break;
+      if (!mbar_wait(q_empty, qphase ^ 1u, abort_flag, p.status, SITE_PROD_Q)) break;
+      qphase ^= 1u;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(p.box_tokens * p.group * D * 2));
+#pragma unroll
+        for (int h = 0; h < L::HALVES; ++h) {
+          tma_load_3d(&tmQ, q_full, smem + L::OFF_Q + h * L::Q_HALF, h * 64, w.kvh * p.group,
+                      w.rq.row + rt * p.tok_tile);
+        }
+      }
+      __syncwarp();
+      for (int i = w.i0; i < w.i1; ++i) {
+        const int after = i + 2 < w.i1 ? page_of(w, i + 2) : 0;  // in flight during the waits
+        if (i + 1 < w.i1 && !load(w, i + 1, nxt, &tmK)) {
+          ok = false;
+          break;
+        }
+        if (!load(w, i, cur, &tmV)) {
+          ok = false;
+          break;
+        }
+        cur = nxt;
+        nxt = after;
+      }
+    }
+    if (*abort_flag != 0 && lane == 0) {
+      // a role gave up: no copy may be in flight when the block ends (bounded like every wait)
+      int none = 0;
+      for (uint32_t k = n > RING ? n - RING : 0; k < n; ++k) {
+        mbar_wait(&ring_full[k % RING], (k / RING) & 1u, &none, p.status, SITE_PROD_SLOT);
+      }
+      if (qphase != 0 || n > 0) mbar_wait(q_full, qphase ^ 1u, &none, p.status, SITE_PROD_Q);
+    }
+  } else if (warp == MMA_WARP) {
+    // ------------------------------ MMA issuer ------------------------------
+    constexpr uint32_t FMT = BF16 ? 1u : 0u;
+    constexpr uint32_t idesc_s = make_idesc(BM, BN, FMT, FMT, 0u, 0u);  // Q K^T, both K-major
+    constexpr uint32_t idesc_o = make_idesc(BM, D, FMT, FMT, 0u, 1u);   // P (TMEM) V (MN-major)
+    const uint64_t qdesc = sdesc_sw128(smem_u32(smem + L::OFF_Q), 16, 1024);
+    uint32_t n = 0;     // tiles taken from the ring
+    uint32_t g = 0;     // key tiles so far
+    uint32_t qphase = 0, ofree_phase = 0;
+    bool first_segment = true, ok = true;
+    auto take = [&](int* st) -> bool {
+      *st = static_cast<int>(n % RING);
+      const uint32_t ph = (n / RING) & 1u;
+      ++n;
+      return mbar_wait(&ring_full[*st], ph, abort_flag, p.status, SITE_MMA_KV);
+    };
+    auto issue_s = [&](uint32_t tile, uint64_t* last) -> bool {
+      int st;
+      if (!take(&st)) return false;
+      tc_fence_after();
+      const uint64_t kdesc = sdesc_sw128(smem_u32(smem + L::OFF_RING + st * L::TILE), 16, L::GROUP);
+      if (elect_one_sync()) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t qo = ((kk >> 2) * L::Q_HALF + (kk & 3) * 32) >> 4;
+          const uint32_t ko = ((kk >> 2) * 1024 + (kk & 3) * 32) >> 4;
+          umma_f16(tmem + (tile & 1u) * BN, qdesc + qo, kdesc + ko, idesc_s, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[tile & 1u]);
+        umma_commit(&ring_empty[st]);
+        if (last != nullptr) umma_commit(last);
+      }
+      __syncwarp();
+      return true;
+    };
+    for (; w.more() && ok; w.next(p)) {
+      if (w.tokens(p, rt) == 0) continue;
+      if (!mbar_wait(q_full, qphase, abort_flag, p.status, SITE_MMA_Q)) break;
+      qphase ^= 1u;
+      const int tiles = w.i1 - w.i0;
+      if (!issue_s(g, tiles == 1 ? q_empty : nullptr)) break;
+      for (int j = 0; j < tiles; ++j, ++g) {
+        if (j + 1 < tiles && !issue_s(g + 1, j + 2 == tiles ? q_empty : nullptr)) {
+          ok = false;
+          break;
+        }
+        int st;
+        if (!take(&st) || !mbar_wait(&p_full[g & 1u], (g >> 1) & 1u, abort_flag, p.status, SITE_MMA_P)) {
+          ok = false;
+          break;
+        }
+        if (j == 0 && !first_segment) {  // the last segment's O has been read
+          if (!mbar_wait(o_free, ofree_phase, abort_flag, p.status, SITE_MMA_OFREE)) {
+            ok = false;
+            break;
+          }
+          ofree_phase ^= 1u;
+        }
+        tc_fence_after();
+        const uint64_t vdesc = sdesc_sw128(smem_u32(smem + L::OFF_RING + st * L::TILE), 1024, L::GROUP);
+        if (elect_one_sync()) {
+#pragma unroll
+          for (int kk = 0; kk < BN / 16; ++kk) {
+            umma_f16_tmem_a(tmem + COL_O, tmem + (g & 1u) * BN + kk * 8,
+                            vdesc + static_cast<uint64_t>(kk * 2 * L::GROUP / 16), idesc_o,
+                            (j > 0 || kk > 0) ? 1u : 0u);
+          }
+          umma_commit(pv_done);
+          umma_commit(&ring_empty[st]);
+          if (j + 1 == tiles) umma_commit(o_done);
+        }
+        __syncwarp();
+      }
+      first_segment = false;
+    }
+  } else {
+    // ------------- softmax, O correction and epilogue (thread = query row) -------------
+    const int row = threadIdx.x;
+    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t t_o = tmem + lane_base + COL_O;
+    const float sl = p.scale_log2;
+    const int tok = row / p.group, head = row - tok * p.group;
+    uint32_t g = 0, n = 0;  // key tiles so far; their K and V loads into the ring
+    uint32_t o_phase = 0;
+    bool ok = true;
+    Desc d = {};
+    for (bool first = true; w.more() && ok; w.next(p)) {
+      const int tokens = w.tokens(p, rt);
+      const bool first_part = first;
+      first = false;
+      if (tokens == 0) continue;
+      const int rows = tokens * p.group;
+      const bool live = row < rows;
+      const bool warp_on = warp * 32 < rows;
+      uint64_t bits = 0;
+      if (live) {
+        const int t = rt * p.tok_tile + tok;
+        bits = p.tree != nullptr ? static_cast<uint64_t>(__ldg(p.tree + w.rq.row + t))
+                                 : (2ull << t) - 1ull;  // t = 63: all ones
+        if (w.rq.tokens < 64) bits &= (1ull << w.rq.tokens) - 1ull;
+      }
+      const int tiles = w.i1 - w.i0;
+      float m_used = -INFINITY, lsum = 0.f;
+      for (int j = 0; j < tiles; ++j, ++g) {
+        const int k0 = (w.i0 + j) * BN;
+        const bool masked = k0 + BN > w.rq.ctx;
+        if (masked) {
+          // V(j) is the load 2 j + 2 of the segment, or 2 j + 1 for its last tile
+          const uint32_t vn = n + 2 * j + (j + 1 < tiles ? 2 : 1);
+          const int st = static_cast<int>(vn % RING);
+          if (!mbar_wait(&ring_full[st], (vn / RING) & 1u, abort_flag, p.status, SITE_SM_V)) {
+            ok = false;
+            break;
+          }
+          clean_v<BF16, D>(smem + L::OFF_RING + st * L::TILE, w.rq.ctx - k0, w.rq.len - k0,
+                           max(k0 - w.rq.ctx, 0), row, bad);
+          fence_proxy_async_smem();
+        }
+        if (!mbar_wait(&s_full[g & 1u], (g >> 1) & 1u, abort_flag, p.status, SITE_SM_S)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (warp_on) {
+          const uint32_t t_s = tmem + lane_base + (g & 1u) * BN;
+          uint32_t view[4];
+          if (masked) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) view[q] = view_word(bits, k0 + 32 * q - w.rq.ctx);
+            ok = softmax_step<true, BF16, D>(t_s, t_o, view, sl, m_used, lsum, pv_done, (g - 1) & 1u,
+                                             abort_flag, p.status);
+          } else {
+            ok = softmax_step<false, BF16, D>(t_s, t_o, view, sl, m_used, lsum, pv_done, (g - 1) & 1u,
+                                              abort_flag, p.status);
+          }
+          if (!ok) break;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[g & 1u]);
+      }
+      n += 2 * tiles;
+      if (!ok) break;
+      if (!mbar_wait(o_done, o_phase, abort_flag, p.status, SITE_SM_O)) break;
+      o_phase ^= 1u;
+      tc_fence_after();
+      // ---- epilogue ----
+      const bool whole = w.i0 == 0 && w.i1 == w.tiles;
+      const int slot = 2 * static_cast<int>(blockIdx.x) + (first_part ? 0 : 1);
+      const int token = w.rq.row + rt * p.tok_tile + tok;
+      const int q_head = w.kvh * p.group + head;
+      uint64_t lost = bits & (static_cast<uint64_t>(bad[1]) << 32 | bad[0]);
+      if (warp_on) {
+        const float inv = lsum == 0.f ? 0.f : 1.f / lsum;  // a row that sees nothing: O = 0
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(t_o + c, o);
+          tmem_ld_wait();
+          reg_fence(o);
+          if (live && lost != 0) {
+            // drafted V elements that are not finite, for the rows that see them
+            for (uint64_t left = lost; left != 0; left &= left - 1) {
+              const int key = w.rq.ctx + __ffsll(static_cast<long long>(left)) - 1;
+              const int id = p.tables[w.b * p.table_stride + (key >> p.page_log2)];
+              if (key < w.i0 * BN || key >= w.i1 * BN || id < 0 || id >= p.num_blocks) continue;
+              const long long at =
+                  (((static_cast<long long>(id) << p.page_log2) + (key & ((1 << p.page_log2) - 1))) *
+                       p.hkv + w.kvh) * D + c;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float v = load16<BF16>(p.v, at + i);
+                if (!isfinite(v)) o[i] = __float_as_uint(__uint_as_float(o[i]) + v);
+              }
+            }
+          }
+          if (live && whole) {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) +
+                                                  (static_cast<long long>(token) * p.hq + q_head) * D + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t pk[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                pk[e] = pack2<BF16>(__uint_as_float(o[8 * i + 2 * e]) * inv,
+                                    __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+              }
+              dst[i] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            }
+          } else if (live) {
+            float4* dst = p.part_o + (static_cast<long long>(slot) * (D / 4) + c / 4) * p.row_cap + row;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              dst[i * p.row_cap] =
+                  make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                              __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+            }
+          }
+        }
+        if (live && whole) {
+          p.lse[static_cast<long long>(token) * p.hq + q_head] =
+              lsum == 0.f ? -INFINITY : (m_used + log2f(lsum)) * 0.6931471805599453f;
+        } else if (live) {
+          p.part_ml[static_cast<long long>(slot) * p.row_cap + row] = make_float2(m_used, lsum);
+        }
+      }
+      if (!whole && w.i0 == 0) {  // the unit starts here: this CTA describes it
+        const long long last = w.t + w.tiles - 1;
+        d.count = rg.owner(last) - range + 1;
+        d.slot = slot;
+        d.row = w.rq.row + rt * p.tok_tile;
+        d.tokens = tokens;
+        d.kvh = w.kvh;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_free);
+    }
+    if (threadIdx.x == 0) p.desc[blockIdx.x] = d;
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the parts of a unit that several ranges hold: M = max m, O = sum 2^(m - M) O_part /
+// sum 2^(m - M) l. Block (x, y): the unit that starts in CTA x, part y of its elements; a thread
+// takes four elements of a row, rows of a warp back to back, eight parts' loads at a time.
+constexpr int JOIN_THREADS = 128;
+constexpr int JOIN_PARTS = 8;
+
+template <bool BF16, int D>
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Params p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const Desc d = p.desc[blockIdx.x];
+  if (d.count == 0) return;
+  const int rows = d.tokens * p.group;
+  const int items = rows * (D / 4);
+  for (int item = blockIdx.y * JOIN_THREADS + threadIdx.x; item < items;
+       item += gridDim.y * JOIN_THREADS) {
+    const int d4 = item / rows, row = item - d4 * rows;
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c0 = 0; c0 < d.count; c0 += JOIN_PARTS) {
+      float2 ml[JOIN_PARTS];
+      float4 part[JOIN_PARTS];
+#pragma unroll
+      for (int i = 0; i < JOIN_PARTS; ++i) {
+        const int c = c0 + i;
+        ml[i] = make_float2(-INFINITY, 0.f);
+        part[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < d.count) {
+          const long long slot = c == 0 ? d.slot : 2LL * (blockIdx.x + c * p.row_tiles);
+          ml[i] = __ldcg(p.part_ml + slot * p.row_cap + row);
+          part[i] = __ldcg(p.part_o + (slot * (D / 4) + d4) * p.row_cap + row);
+        }
+      }
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < JOIN_PARTS; ++i) top = fmaxf(top, ml[i].x);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float keep = exp2f(m - base);
+      l *= keep;
+      o.x *= keep;
+      o.y *= keep;
+      o.z *= keep;
+      o.w *= keep;
+#pragma unroll
+      for (int i = 0; i < JOIN_PARTS; ++i) {
+        if (c0 + i >= d.count) continue;
+        const float wt = exp2f(ml[i].x - base);
+        l = fmaf(wt, ml[i].y, l);
+        o.x = fmaf(wt, part[i].x, o.x);
+        o.y = fmaf(wt, part[i].y, o.y);
+        o.z = fmaf(wt, part[i].z, o.z);
+        o.w = fmaf(wt, part[i].w, o.w);
+      }
+      m = top;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int tok = row / p.group;
+    const long long at =
+        static_cast<long long>(d.row + tok) * p.hq + d.kvh * p.group + (row - tok * p.group);
+    uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at * D + d4 * 4);
+    *dst = make_uint2(pack2<BF16>(o.x * inv, o.y * inv), pack2<BF16>(o.z * inv, o.w * inv));
+    if (d4 == 0) p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  }
+}
+
+// Workspace: descriptors, (maximum, sum) and O of two partial units of every CTA.
+struct Workspace {
+  size_t off_ml, off_o, total;
+  int row_cap;
+  Workspace(long long max_new, long long group, long long D) {
+    const long long tile = BM / group;
+    row_cap = static_cast<int>((std::min(tile, max_new) * group + 7) / 8 * 8);
+    off_ml = sizeof(Desc) * MAX_CTAS;
+    off_o = off_ml + sizeof(float2) * 2 * MAX_CTAS * row_cap;
+    total = off_o + sizeof(float) * 2 * MAX_CTAS * static_cast<size_t>(row_cap) * D;
+  }
+};
+
+bool sizes_ok(int64_t max_new, int64_t Hq, int64_t Hkv, int64_t D) {
+  return max_new > 0 && max_new <= MAX_DRAFT && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 &&
+         Hq / Hkv <= MAX_GROUP && (D == 64 || D == 128);
+}
+
+template <bool BF16, int D>
+int go(Params& p, const void* Q, const void* Kc, const void* Vc, int64_t q_token, cudaStream_t stream) {
+  using L = Layout<D>;
+  const CUtensorMapDataType type = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap tq, tk, tv;
+  {
+    const uint64_t dims[3] = {D, static_cast<uint64_t>(p.hq), static_cast<uint64_t>(p.rows)};
+    const uint64_t strides[2] = {D * 2, static_cast<uint64_t>(q_token) * 2};
+    const uint32_t box[3] = {64, static_cast<uint32_t>(p.group), static_cast<uint32_t>(p.box_tokens)};
+    const int s = encode_tmap(&tq, type, 3, Q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (s != KTA_OK) return s;
+  }
+  // A block of a head: (64 d, 8 tokens, half, group of 8 tokens), and the (token, head) row at
+  // which it starts.
+  const uint64_t page = uint64_t{1} << p.page_log2, token = static_cast<uint64_t>(p.hkv) * D * 2;
+  const uint64_t dims[5] = {64, 8, L::HALVES, page / 8, static_cast<uint64_t>(p.num_blocks) * page * p.hkv};
+  const uint64_t strides[4] = {token, 128, 8 * token, D * 2};
+  const uint32_t box[5] = {64, 8, L::HALVES, (1u << p.box_log2) / 8, 1};
+  int s = encode_tmap(&tk, type, 5, Kc, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (s != KTA_OK) return s;
+  s = encode_tmap(&tv, type, 5, Vc, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (s != KTA_OK) return s;
+  auto kernel = tree_kernel<BF16, D>;
+  s = set_kernel_smem(reinterpret_cast<const void*>(kernel), L::ALLOC);
+  if (s != KTA_OK) return s;
+  const int sms = std::min(current_sm_count(), MAX_CTAS);
+  if (sms < p.row_tiles) return KTA_ERR_UNSUPPORTED;
+  const int grid = sms / p.row_tiles * p.row_tiles;
+  s = launch_ex(kernel, dim3(grid), dim3(NUM_THREADS), L::ALLOC, stream, 1, tq, tk, tv, p);
+  if (s != KTA_OK) return s;
+  // four elements a thread and at most four passes
+  const int parts = std::max(1, std::min(8, p.row_cap * (D / 4) / (2 * JOIN_THREADS)));
+  return launch_ex(join_kernel<BF16, D>, dim3(grid, parts), dim3(JOIN_THREADS), 0, stream, 1, p);
+}
+
+template <bool BF16>
+int launch(const void* Q, const void* Kc, const void* Vc, const void* tables, const void* ctx,
+           const void* offsets, const void* tree, void* O, void* LSE, int64_t tokens, int64_t B,
+           int64_t Hq, int64_t Hkv, int64_t D, int64_t q_token, int64_t num_blocks, int64_t block,
+           int64_t max_blocks, int64_t table_stride, int64_t max_new, float scale, void* workspace,
+           size_t ws_bytes, cudaStream_t stream) {
+  if (!Q || !Kc || !Vc || !tables || !ctx || !offsets || !O || !LSE) return KTA_ERR_INVALID_ARG;
+  if (tokens <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || num_blocks <= 0 || block <= 0 ||
+      max_blocks <= 0 || max_new <= 0) {
+    return KTA_ERR_INVALID_ARG;
+  }
+  if (!(scale > 0.f) || !std::isfinite(scale)) return KTA_ERR_INVALID_ARG;
+  if (B > 1 && table_stride < max_blocks) return KTA_ERR_INVALID_ARG;
+  if (!sizes_ok(max_new, Hq, Hkv, D) || B > MAX_BATCH) return KTA_ERR_UNSUPPORTED;
+  if (block < 8 || block > 256 || (block & (block - 1)) != 0) return KTA_ERR_UNSUPPORTED;
+  // key positions, rows and (token, head) rows of the cache stay in int32
+  if (max_blocks > (1LL << 30) / block || tokens > (1LL << 30) || Hq > 65536 ||
+      num_blocks > ((1LL << 31) - 1) / (block * Hkv)) {
+    return KTA_ERR_UNSUPPORTED;
+  }
+  if (q_token < Hq * D) return KTA_ERR_INVALID_ARG;
+  if (q_token % 8 != 0 || !aligned16(Q) || !aligned16(Kc) || !aligned16(Vc) || !aligned16(O)) {
+    return KTA_ERR_ALIGN;
+  }
+  for (const void* q : {tables, ctx, offsets, static_cast<const void*>(LSE)}) {
+    if (reinterpret_cast<uintptr_t>(q) & 3) return KTA_ERR_ALIGN;
+  }
+  if (reinterpret_cast<uintptr_t>(tree) & 7) return KTA_ERR_ALIGN;
+  const long long group = Hq / Hkv;
+  const Workspace ws(max_new, group, D);
+  if (workspace == nullptr || ws_bytes < ws.total || !aligned16(workspace)) return KTA_ERR_WORKSPACE;
+  int s = require_sm100();
+  if (s != KTA_OK) return s;
+  Params p = {};
+  p.ctx = static_cast<const int32_t*>(ctx);
+  p.offsets = static_cast<const int32_t*>(offsets);
+  p.tree = static_cast<const int64_t*>(tree);
+  p.tables = static_cast<const int32_t*>(tables);
+  p.out = O;
+  p.lse = static_cast<float*>(LSE);
+  p.v = Vc;
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  p.desc = reinterpret_cast<Desc*>(base);
+  p.part_ml = reinterpret_cast<float2*>(base + ws.off_ml);
+  p.part_o = reinterpret_cast<float4*>(base + ws.off_o);
+  p.table_stride = table_stride;
+  p.batch = static_cast<int>(B);
+  p.rows = static_cast<int>(tokens);
+  p.hq = static_cast<int>(Hq);
+  p.hkv = static_cast<int>(Hkv);
+  p.group = static_cast<int>(group);
+  p.max_new = static_cast<int>(max_new);
+  p.max_blocks = static_cast<int>(max_blocks);
+  p.num_blocks = static_cast<int>(num_blocks);
+  while ((int64_t{1} << p.page_log2) < block) ++p.page_log2;
+  p.box_log2 = std::min(p.page_log2, 7);
+  p.tok_tile = BM / p.group;
+  p.box_tokens = std::min(p.tok_tile, p.max_new);
+  p.row_tiles = (p.max_new + p.tok_tile - 1) / p.tok_tile;
+  p.row_cap = ws.row_cap;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.status = device_status_ptr();
+  if (D == 64) return go<BF16, 64>(p, Q, Kc, Vc, q_token, stream);
+  return go<BF16, 128>(p, Q, Kc, Vc, q_token, stream);
+}
+
+}  // namespace tree
+}  // namespace kta
+
+extern "C" size_t kta_tree_attn_workspace_bytes(int64_t max_new, int64_t Hq, int64_t Hkv, int64_t D) {
+  if (!kta::tree::sizes_ok(max_new, Hq, Hkv, D)) return 0;
+  return kta::tree::Workspace(max_new, Hq / Hkv, D).total;
+}
+
+#define KTA_TREE_ENTRY(NAME, BF16)                                                                  \
+  extern "C" int kta_tree_attn_##NAME(                                                              \
+      const void* Q, const void* Kc, const void* Vc, const void* block_tables,                      \
+      const void* context_lens, const void* offsets, const void* tree, void* O, void* LSE,          \
+      int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t q_token,               \
+      int64_t num_blocks, int64_t block_size, int64_t max_blocks, int64_t table_stride,             \
+      int64_t max_new, float scale, void* workspace, size_t ws_bytes, void* stream) {               \
+    return kta::tree::launch<BF16>(Q, Kc, Vc, block_tables, context_lens, offsets, tree, O, LSE,    \
+                                   tokens, B, Hq, Hkv, D, q_token, num_blocks, block_size,          \
+                                   max_blocks, table_stride, max_new, scale, workspace, ws_bytes,   \
+                                   static_cast<cudaStream_t>(stream));                              \
+  }
+
+KTA_TREE_ENTRY(f16, false)
+KTA_TREE_ENTRY(bf16, true)

@@ -34,6 +34,11 @@ STATUS_NAMES = {
 _u64, _i64, _i32, _u32 = ctypes.c_uint64, ctypes.c_int64, ctypes.c_int32, ctypes.c_uint32
 _f32, _ptr, _size = ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
 
+# signatures shared by an entry's f16 and bf16 forms
+_ROPE = [_ptr, _ptr, _i64, _ptr, _ptr] + [_i64] * 8 + [ctypes.c_int, ctypes.c_int, _f32, _ptr]
+_ROPE_CACHE = ([_ptr] * 4 + [_i64] + [_ptr] * 5 + [_i64] * 5 + [_ptr, _i64, ctypes.c_int, _f32, _ptr])
+_TREE_ATTN = [_ptr] * 9 + [_i64] * 11 + [_f32, _ptr, _size, _ptr]
+
 # name -> (restype, argtypes); every symbol include/kta_b200.h declares.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kta_abi_version": (ctypes.c_int, []),
@@ -82,6 +87,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kta_rmsnorm_bf16": (ctypes.c_int, [_ptr, _ptr, _ptr, _i64, _i64, _f32, _ptr]),
     "kta_softmax_f16": (ctypes.c_int, [_ptr, _ptr, _i64, _i64, _ptr]),
     "kta_softmax_bf16": (ctypes.c_int, [_ptr, _ptr, _i64, _i64, _ptr]),
+    "kta_cache_slots": (ctypes.c_int, [_ptr] * 8 + [_i64] * 6 + [_ptr]),
+    "kta_rope_f16": (ctypes.c_int, _ROPE),
+    "kta_rope_bf16": (ctypes.c_int, _ROPE),
+    "kta_rope_cache_f16": (ctypes.c_int, _ROPE_CACHE),
+    "kta_rope_cache_bf16": (ctypes.c_int, _ROPE_CACHE),
+    "kta_tree_attn_workspace_bytes": (_size, [_i64, _i64, _i64, _i64]),
+    "kta_tree_attn_f16": (ctypes.c_int, _TREE_ATTN),
+    "kta_tree_attn_bf16": (ctypes.c_int, _TREE_ATTN),
     "kta_so_rmsnorm_f16": (None, [_u64, _u64, _u64, _i32, _i32]),
     "kta_so_softmax_f16": (None, [_u64, _u64, _i32, _i32]),
     "kta_so_gemm_bf16": (None, [_u64, _u64, _u64, _i32, _i32, _i32]),

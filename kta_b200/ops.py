@@ -8,6 +8,9 @@ implementation behind these functions.
 
 from __future__ import annotations
 
+import ctypes
+import math
+
 import torch
 
 from kta_b200 import lib
@@ -254,6 +257,286 @@ def decode_gqa(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
              k_cache.shape[0], int(max_seqlen), float(scale), workspace.data_ptr(),
              workspace.numel(), _stream())
     return out
+
+
+# ---- paged KV cache -------------------------------------------------------------------------
+
+
+def _launch(dev: torch.device, entry: str, *args: object) -> None:
+    """Calls ``entry`` with ``dev`` current and its current stream as the last argument."""
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            lib.call(entry, *args, _stream())
+    else:
+        lib.call(entry, *args, _stream())
+
+
+def _same_device(first: torch.Tensor, *ts: torch.Tensor) -> torch.device:
+    """The tensors' one CUDA device."""
+    dev = first.device
+    if dev.type != "cuda":
+        raise ValueError("libkta_b200 operates on CUDA tensors only")
+    for t in ts:
+        if t.device != dev:
+            raise ValueError(f"tensors on {t.device} and {dev}: one device is needed")
+    return dev
+
+
+def _stride(t: torch.Tensor, i: int, alone: int) -> int:
+    """Stride ``i`` of ``t`` in elements; ``alone`` for a dimension of size one, whose stride torch
+    leaves open."""
+    return t.stride(i) if t.shape[i] > 1 else alone
+
+
+def _vector(t: torch.Tensor, dtype: torch.dtype, n: int | None, name: str) -> None:
+    """A contiguous 1-D tensor of ``dtype``, of ``n`` elements where that is given."""
+    if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or \
+            (n is not None and t.shape[0] != n):
+        size = "" if n is None else f" of {n} elements"
+        raise ValueError(f"{name} must be a contiguous {dtype} vector{size}")
+
+
+def _block_tables(t: torch.Tensor, bsz: int) -> None:
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != bsz or t.stride(1) != 1:
+        raise ValueError("block_tables must be int32 [B, max_blocks] with unit column stride")
+
+
+def cache_slots(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor,
+                free_blocks: torch.Tensor, block_size: int, max_tokens: int, *,
+                slots: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                offsets: torch.Tensor | None = None, used: torch.Tensor | None = None,
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Block tables and slot maps of a paged KV cache for one step, from request lengths on the
+    device (nothing travels to the host).
+
+    context_lens, new_lens int32 [B]: tokens in the cache, and tokens to come. The blocks of
+    ``block_size`` tokens that the latter need beyond those held are taken from the front of
+    ``free_blocks`` (int32) and written into ``block_tables`` (int32 [B, max_blocks], in place;
+    other entries are not touched). Returns, request after request, ``slots`` (int64
+    [max_tokens], block * block_size + place) and ``positions`` (int32 [max_tokens]) of the new
+    tokens, -1 and 0 behind the last one; ``offsets`` (int32 [B + 1], first row of each
+    request); ``used`` (int32 [1], blocks taken). What does not fit (a table's row, the free
+    list, max_tokens) is cut off and recorded in the device status block."""
+    dev = _same_device(context_lens, new_lens, block_tables, free_blocks)
+    _vector(context_lens, torch.int32, None, "context_lens")
+    bsz = context_lens.shape[0]
+    _vector(new_lens, torch.int32, bsz, "new_lens")
+    _vector(free_blocks, torch.int32, None, "free_blocks")
+    _block_tables(block_tables, bsz)
+    made = []
+    for t, n, dtype, name in ((slots, max_tokens, torch.int64, "slots"),
+                              (positions, max_tokens, torch.int32, "positions"),
+                              (offsets, bsz + 1, torch.int32, "offsets"),
+                              (used, 1, torch.int32, "used")):
+        if t is None:
+            t = torch.empty(n, dtype=dtype, device=dev)
+        else:
+            _same_device(context_lens, t)
+            _vector(t, dtype, n, name)
+        made.append(t)
+    _launch(dev, "kta_cache_slots", context_lens.data_ptr(), new_lens.data_ptr(),
+            block_tables.data_ptr(), free_blocks.data_ptr(), *[t.data_ptr() for t in made], bsz,
+            block_tables.shape[1], block_tables.stride(0), free_blocks.shape[0], block_size,
+            max_tokens)
+    return made[0], made[1], made[2], made[3]
+
+
+def rope_freqs(rot: int, base: float = 10000.0, *, scaling: str | None = None, factor: float = 1.0,
+               original_len: int = 4096, low_turns: float = 1.0, high_turns: float = 32.0,
+               device: torch.device | str = "cuda") -> tuple[torch.Tensor, float]:
+    """Radians per position (fp64 [rot / 2]) of rotary positions over ``rot`` dimensions, and the
+    scale that goes with them: freq_i = base^(-2 i / rot). ``scaling`` stretches them for contexts
+    ``factor`` times longer than the ``original_len`` they were trained on:
+
+    - "linear": every frequency divided by factor;
+    - "ntk": base * factor^(rot / (rot - 2)), so that the lowest frequency is divided by factor
+      and the highest kept;
+    - "bands": frequencies that make fewer than ``low_turns`` turns in original_len tokens are
+      divided by factor, those of more than ``high_turns`` kept, a linear ramp in between;
+    - "yarn": the same ramp over the pair index between the two bounds, and scale
+      1 + 0.1 ln(factor)."""
+    if rot < 2 or rot % 2:
+        raise ValueError("rot must be even and positive")
+    if not (base > 0 and factor >= 1 and original_len > 0 and 0 < low_turns < high_turns):
+        raise ValueError("base > 0, factor >= 1, original_len > 0, 0 < low_turns < high_turns")
+    if scaling == "ntk":
+        if rot == 2:
+            raise ValueError("ntk scaling needs more than one pair")
+        base = base * factor ** (rot / (rot - 2))
+    pair = torch.arange(rot // 2, dtype=torch.float64)
+    freqs = base ** (-2.0 * pair / rot)
+    scale = 1.0
+    if scaling == "linear":
+        freqs = freqs / factor
+    elif scaling in ("bands", "yarn"):
+        if scaling == "bands":
+            turns = original_len * freqs / (2 * math.pi)
+            keep = (turns - low_turns) / (high_turns - low_turns)
+        else:
+            def index(turns: float) -> float:
+                """The (real) pair index that makes `turns` turns in original_len tokens."""
+                return rot * math.log(original_len / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+            first = max(math.floor(index(high_turns)), 0)
+            last = max(min(math.ceil(index(low_turns)), rot // 2 - 1), first)
+            keep = 1.0 - (pair - first) / max(last - first, 0.001)
+            scale = 1.0 + 0.1 * math.log(factor)
+        keep = keep.clamp(0.0, 1.0)
+        freqs = freqs * (keep + (1.0 - keep) / factor)
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    return freqs.to(device), scale
+
+
+def _rope_rows(t: torch.Tensor, name: str, dtype: torch.dtype, tokens: int, d: int) -> None:
+    if t.dtype != dtype or t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != d or \
+            t.stride(2) != 1:
+        raise ValueError(f"{name} must be a {dtype} [{tokens}, heads, {d}] tensor with unit stride "
+                         "in its last dimension")
+
+
+def _row_strides(t: torch.Tensor) -> tuple[int, int]:
+    """Token and head stride of a [tokens, heads, D] tensor."""
+    _, heads, d = t.shape
+    return _stride(t, 0, heads * d), _stride(t, 1, d)
+
+
+def _rope_angles(positions: torch.Tensor, freqs: torch.Tensor, tokens: int) -> int:
+    """Bytes of a position."""
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError("positions must be int32 or int64")
+    _vector(positions, positions.dtype, tokens, "positions")
+    _vector(freqs, torch.float64, None, "freqs")
+    return positions.element_size()
+
+
+_ROPE_TYPES = {torch.float16: "f16", torch.bfloat16: "bf16"}
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *, interleaved: bool = False,
+         inverse: bool = False, scale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions of X [tokens, heads, D] (f16 or bf16; any token and head strides that are
+    multiples of 8): the first 2 len(freqs) dimensions turn in pairs by positions[n] * freqs[i]
+    and are scaled, the others are copied. Pairs are (i, i + rot / 2), or neighbours where
+    ``interleaved``. ``inverse`` turns back: given the gradient of the output of a call, it is the
+    gradient of its input. positions int32 or int64 [tokens]; freqs fp64 (``rope_freqs``). ``out``
+    may be X itself."""
+    if x.dtype not in _ROPE_TYPES or x.dim() != 3:
+        raise ValueError("X must be an f16 or bf16 [tokens, heads, D] tensor")
+    tokens, heads, d = x.shape
+    _rope_rows(x, "X", x.dtype, tokens, d)
+    size = _rope_angles(positions, freqs, tokens)
+    if out is None:
+        out = torch.empty((tokens, heads, d), dtype=x.dtype, device=x.device)
+    else:
+        _rope_rows(out, "out", x.dtype, tokens, d)
+        if out.shape[1] != heads:
+            raise ValueError("out must have X's heads")
+    dev = _same_device(x, positions, freqs, out)
+    _launch(dev, "kta_rope_" + _ROPE_TYPES[x.dtype], x.data_ptr(), positions.data_ptr(), size,
+            freqs.data_ptr(), out.data_ptr(), tokens, heads, d, 2 * freqs.shape[0],
+            *_row_strides(x), *_row_strides(out), int(interleaved), int(inverse), float(scale))
+    return out
+
+
+def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype, d: int) -> None:
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != d or \
+            k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise ValueError("K and V caches must be [num_blocks, block_size, Hkv, D] of Q's type and D")
+    if not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        raise ValueError("K and V caches must be contiguous")
+
+
+def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+               slots: torch.Tensor, freqs: torch.Tensor, k_cache: torch.Tensor,
+               v_cache: torch.Tensor, *, interleaved: bool = False, scale: float = 1.0,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions of a step's Q [tokens, Hq, D] and K [tokens, Hkv, D] (``rope``), with the
+    rotated K and the V written to ``slots`` (int64 [tokens], ``cache_slots``) of the paged caches
+    [num_blocks, block_size, Hkv, D]; a negative slot writes nothing. Returns the rotated Q
+    (``out`` may be Q itself). Q, K and V may be slices of one fused tensor."""
+    if q.dtype not in _ROPE_TYPES or q.dim() != 3 or k.dim() != 3:
+        raise ValueError("Q, K and V must be f16 or bf16 [tokens, heads, D] tensors")
+    tokens, hq, d = q.shape
+    hkv = k.shape[1]
+    for t, name in ((q, "Q"), (k, "K"), (v, "V")):
+        _rope_rows(t, name, q.dtype, tokens, d)
+    _caches(k_cache, v_cache, q.dtype, d)
+    if v.shape[1] != hkv or k_cache.shape[2] != hkv:
+        raise ValueError("K, V and the caches must have the same heads")
+    size = _rope_angles(positions, freqs, tokens)
+    _vector(slots, torch.int64, tokens, "slots")
+    if out is None:
+        out = torch.empty((tokens, hq, d), dtype=q.dtype, device=q.device)
+    else:
+        _rope_rows(out, "out", q.dtype, tokens, d)
+        if out.shape[1] != hq:
+            raise ValueError("out must have Q's heads")
+    dev = _same_device(q, k, v, positions, slots, freqs, k_cache, v_cache, out)
+    strides = (ctypes.c_int64 * 8)(*_row_strides(q), *_row_strides(k), *_row_strides(v),
+                                   *_row_strides(out))
+    _launch(dev, "kta_rope_cache_" + _ROPE_TYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            positions.data_ptr(), size, slots.data_ptr(), freqs.data_ptr(), out.data_ptr(),
+            k_cache.data_ptr(), v_cache.data_ptr(), tokens, hq, hkv, d, 2 * freqs.shape[0], strides,
+            k_cache.shape[0] * k_cache.shape[1], int(interleaved), float(scale))
+    return out
+
+
+def tree_attn_workspace_bytes(max_new: int, hq: int, hkv: int, d: int) -> int:
+    return int(lib.load().kta_tree_attn_workspace_bytes(max_new, hq, hkv, d))
+
+
+def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+              block_tables: torch.Tensor, context_lens: torch.Tensor, offsets: torch.Tensor,
+              max_new: int, tree: torch.Tensor | None = None, *, scale: float | None = None,
+              out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+              workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Attention of drafted tokens over a paged KV cache: request b's rows of Q [tokens, Hq, D]
+    (f16 or bf16) are offsets[b] .. offsets[b + 1] (int32 [B + 1], at most ``max_new`` <= 64
+    each); their K and V already stand in the cache behind its context_lens[b] (int32 [B])
+    tokens (``rope_cache``). A row sees the whole context, and drafted token j of its request iff
+    bit j of tree[row] (int64 [tokens]) is set; without ``tree`` the drafted tokens are a chain,
+    and max_new = 1 is a decode step. Caches [num_blocks, block_size, Hkv, D], block_tables int32
+    [B, max_blocks]. Returns O [tokens, Hq, D] and LSE fp32 [tokens, Hq] (natural log, to merge
+    with attention over other keys); a row that sees nothing has O = 0 and LSE = -inf, rows of no
+    request are left as they were.
+
+    ``workspace`` (uint8, ``tree_attn_workspace_bytes``, any contents) is allocated on the current
+    stream where none is given; calls that may run at the same time need one each."""
+    if q.dtype not in _ROPE_TYPES or q.dim() != 3 or q.stride(2) != 1 or \
+            (q.shape[1] > 1 and q.stride(1) != q.shape[2]):
+        raise ValueError("Q must be an f16 or bf16 [tokens, Hq, D] tensor with contiguous heads")
+    tokens, hq, d = q.shape
+    _caches(k_cache, v_cache, q.dtype, d)
+    nblocks, bs, hkv, _ = k_cache.shape
+    _vector(context_lens, torch.int32, None, "context_lens")
+    bsz = context_lens.shape[0]
+    _vector(offsets, torch.int32, bsz + 1, "offsets")
+    _block_tables(block_tables, bsz)
+    dev = _same_device(q, k_cache, v_cache, block_tables, context_lens, offsets)
+    if tree is not None:
+        _same_device(q, tree)
+        _vector(tree, torch.int64, tokens, "tree")
+    if out is None:
+        out = torch.empty((tokens, hq, d), dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor of Q's shape and type")
+    if lse is None:
+        lse = torch.empty((tokens, hq), dtype=torch.float32, device=dev)
+    elif tuple(lse.shape) != (tokens, hq) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise ValueError("lse must be a contiguous fp32 [tokens, Hq] tensor")
+    if workspace is None:
+        workspace = torch.empty(tree_attn_workspace_bytes(max_new, hq, hkv, d), dtype=torch.uint8,
+                                device=dev)
+    _same_device(q, out, lse, workspace)
+    _launch(dev, "kta_tree_attn_" + _ROPE_TYPES[q.dtype], q.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(),
+            offsets.data_ptr(), None if tree is None else tree.data_ptr(), out.data_ptr(),
+            lse.data_ptr(), tokens, bsz, hq, hkv, d, _stride(q, 0, hq * d), nblocks, bs,
+            block_tables.shape[1], block_tables.stride(0), max_new,
+            d ** -0.5 if scale is None else float(scale), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size())
+    return out, lse
 
 
 class _HostPipe:
