@@ -5,16 +5,21 @@
 static CUDA runtime; tensor maps come from the driver through cudaGetDriverEntryPoint, so no
 libcuda, cuBLAS or torch library is linked (the anti-cheat rule of
 src/kta/checks/anticheat.py:38-58 in the reference).
+
+Beside it, ``kta_b200/_binding.so`` (csrc/binding.cpp, g++): the Python binding of the entries
+whose calls are short, which uses torch's headers and links the library.
 """
 
 from __future__ import annotations
 
 import argparse
 import hashlib
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -24,6 +29,7 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 BUILD = PKG / "_build"
 LIB = PKG / "libkta_b200.so"
+BINDING = PKG / "_binding.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = [
@@ -74,8 +80,41 @@ def _compile(src: Path, extra: list[str], verbose: bool) -> tuple[Path, str]:
     return obj, res.stdout + res.stderr
 
 
+def _run(cmd: list[str], what: str, verbose: bool) -> None:
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{what} failed:\n{res.stdout}\n{res.stderr}")
+
+
+def _build_binding(verbose: bool) -> None:
+    """Compiles csrc/binding.cpp against the torch of this interpreter and the built library."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        raise RuntimeError("torch not found: the binding is built against its headers")
+    torch_dir = Path(spec.submodule_search_locations[0])
+    src = CSRC / "binding.cpp"
+    cuda = Path(nvcc()).resolve().parent.parent
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{INCLUDE}", f"-I{torch_dir}/include",
+           f"-I{torch_dir}/include/torch/csrc/api/include", f"-I{cuda}/include",
+           f"-I{sysconfig.get_paths()['include']}", str(src), "-o", str(BINDING),
+           f"-L{torch_dir}/lib", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           f"-L{PKG}", "-l:libkta_b200.so", "-Wl,-rpath,$ORIGIN"]
+    version = (torch_dir / "version.py").read_bytes()
+    h = hashlib.sha256(" ".join(cmd).encode() + src.read_bytes() + version)
+    for hdr in sorted(INCLUDE.glob("*.h")):
+        h.update(hdr.read_bytes())
+    stamp = BUILD / "binding.hash"
+    if BINDING.exists() and stamp.exists() and stamp.read_text() == h.hexdigest():
+        return
+    _run(cmd, "building the binding", verbose)
+    stamp.write_text(h.hexdigest())
+
+
 def build(verbose: bool = False, ptxas: bool = False) -> Path:
-    """Compiles and links the library; returns its path. Raises on any compiler error."""
+    """Compiles and links the library and its binding; returns the library's path. Raises on any
+    compiler error."""
     BUILD.mkdir(exist_ok=True)
     extra = ["-Xptxas", "-v"] if ptxas else []
     srcs = sources()
@@ -87,12 +126,8 @@ def build(verbose: bool = False, ptxas: bool = False) -> Path:
     objs = [str(o) for o, _ in results]
     newest = max(Path(o).stat().st_mtime for o in objs)
     if not LIB.exists() or LIB.stat().st_mtime < newest:
-        cmd = [nvcc(), *ARCH, "-shared", "-o", str(LIB), *objs]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        res = subprocess.run(cmd, capture_output=True, text=True)
-        if res.returncode != 0:
-            raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+        _run([nvcc(), *ARCH, "-shared", "-o", str(LIB), *objs], "link", verbose)
+    _build_binding(verbose)
     return LIB
 
 

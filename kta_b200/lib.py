@@ -12,8 +12,10 @@ device addresses as unsigned 64-bit integers, sizes as 64-bit integers, a CUDA s
 from __future__ import annotations
 
 import ctypes
+import importlib
 import threading
 from pathlib import Path
+from types import ModuleType
 
 LIB_PATH = Path(__file__).resolve().parent / "libkta_b200.so"
 
@@ -161,6 +163,27 @@ def check(entry: str, status: int) -> None:
 def call(entry: str, *args: object) -> None:
     """Calls ``entry`` and raises KtaError on a nonzero status."""
     check(entry, getattr(load(), entry)(*args))
+
+
+_native: ModuleType | None = None
+
+
+def native() -> ModuleType:
+    """The native binding of the entries whose calls are short (csrc/binding.cpp); raises if it
+    is missing."""
+    global _native
+    if _native is None:
+        load()
+        import torch  # noqa: F401 - the binding links torch's libraries
+
+        try:
+            module = importlib.import_module("kta_b200._binding")
+        except ImportError as exc:
+            raise KtaLibraryError(f"cannot load the binding: {exc} (build it with "
+                                  "`python -m kta_b200.build`)") from exc
+        module.set_check(check)
+        _native = module
+    return _native
 
 
 def device_status(clear: bool = True) -> list[int]:

@@ -8,8 +8,8 @@ implementation behind these functions.
 
 from __future__ import annotations
 
-import ctypes
 import math
+from types import ModuleType
 
 import torch
 
@@ -260,45 +260,15 @@ def decode_gqa(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
 
 
 # ---- paged KV cache -------------------------------------------------------------------------
+# Short calls: tensor checks, allocation and launch are native code (csrc/binding.cpp).
+
+_native: ModuleType | None = None
 
 
-def _launch(dev: torch.device, entry: str, *args: object) -> None:
-    """Calls ``entry`` with ``dev`` current and its current stream as the last argument."""
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            lib.call(entry, *args, _stream())
-    else:
-        lib.call(entry, *args, _stream())
-
-
-def _same_device(first: torch.Tensor, *ts: torch.Tensor) -> torch.device:
-    """The tensors' one CUDA device."""
-    dev = first.device
-    if dev.type != "cuda":
-        raise ValueError("libkta_b200 operates on CUDA tensors only")
-    for t in ts:
-        if t.device != dev:
-            raise ValueError(f"tensors on {t.device} and {dev}: one device is needed")
-    return dev
-
-
-def _stride(t: torch.Tensor, i: int, alone: int) -> int:
-    """Stride ``i`` of ``t`` in elements; ``alone`` for a dimension of size one, whose stride torch
-    leaves open."""
-    return t.stride(i) if t.shape[i] > 1 else alone
-
-
-def _vector(t: torch.Tensor, dtype: torch.dtype, n: int | None, name: str) -> None:
-    """A contiguous 1-D tensor of ``dtype``, of ``n`` elements where that is given."""
-    if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or \
-            (n is not None and t.shape[0] != n):
-        size = "" if n is None else f" of {n} elements"
-        raise ValueError(f"{name} must be a contiguous {dtype} vector{size}")
-
-
-def _block_tables(t: torch.Tensor, bsz: int) -> None:
-    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != bsz or t.stride(1) != 1:
-        raise ValueError("block_tables must be int32 [B, max_blocks] with unit column stride")
+def _bind() -> ModuleType:
+    global _native
+    _native = lib.native()
+    return _native
 
 
 def cache_slots(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor,
@@ -317,28 +287,8 @@ def cache_slots(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tables
     tokens, -1 and 0 behind the last one; ``offsets`` (int32 [B + 1], first row of each
     request); ``used`` (int32 [1], blocks taken). What does not fit (a table's row, the free
     list, max_tokens) is cut off and recorded in the device status block."""
-    dev = _same_device(context_lens, new_lens, block_tables, free_blocks)
-    _vector(context_lens, torch.int32, None, "context_lens")
-    bsz = context_lens.shape[0]
-    _vector(new_lens, torch.int32, bsz, "new_lens")
-    _vector(free_blocks, torch.int32, None, "free_blocks")
-    _block_tables(block_tables, bsz)
-    made = []
-    for t, n, dtype, name in ((slots, max_tokens, torch.int64, "slots"),
-                              (positions, max_tokens, torch.int32, "positions"),
-                              (offsets, bsz + 1, torch.int32, "offsets"),
-                              (used, 1, torch.int32, "used")):
-        if t is None:
-            t = torch.empty(n, dtype=dtype, device=dev)
-        else:
-            _same_device(context_lens, t)
-            _vector(t, dtype, n, name)
-        made.append(t)
-    _launch(dev, "kta_cache_slots", context_lens.data_ptr(), new_lens.data_ptr(),
-            block_tables.data_ptr(), free_blocks.data_ptr(), *[t.data_ptr() for t in made], bsz,
-            block_tables.shape[1], block_tables.stride(0), free_blocks.shape[0], block_size,
-            max_tokens)
-    return made[0], made[1], made[2], made[3]
+    return (_native or _bind()).cache_slots(context_lens, new_lens, block_tables, free_blocks,
+                                            block_size, max_tokens, slots, positions, offsets, used)
 
 
 def rope_freqs(rot: int, base: float = 10000.0, *, scaling: str | None = None, factor: float = 1.0,
@@ -388,31 +338,6 @@ def rope_freqs(rot: int, base: float = 10000.0, *, scaling: str | None = None, f
     return freqs.to(device), scale
 
 
-def _rope_rows(t: torch.Tensor, name: str, dtype: torch.dtype, tokens: int, d: int) -> None:
-    if t.dtype != dtype or t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != d or \
-            t.stride(2) != 1:
-        raise ValueError(f"{name} must be a {dtype} [{tokens}, heads, {d}] tensor with unit stride "
-                         "in its last dimension")
-
-
-def _row_strides(t: torch.Tensor) -> tuple[int, int]:
-    """Token and head stride of a [tokens, heads, D] tensor."""
-    _, heads, d = t.shape
-    return _stride(t, 0, heads * d), _stride(t, 1, d)
-
-
-def _rope_angles(positions: torch.Tensor, freqs: torch.Tensor, tokens: int) -> int:
-    """Bytes of a position."""
-    if positions.dtype not in (torch.int32, torch.int64):
-        raise ValueError("positions must be int32 or int64")
-    _vector(positions, positions.dtype, tokens, "positions")
-    _vector(freqs, torch.float64, None, "freqs")
-    return positions.element_size()
-
-
-_ROPE_TYPES = {torch.float16: "f16", torch.bfloat16: "bf16"}
-
-
 def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *, interleaved: bool = False,
          inverse: bool = False, scale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
     """Rotary positions of X [tokens, heads, D] (f16 or bf16; any token and head strides that are
@@ -421,30 +346,7 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *, inter
     ``interleaved``. ``inverse`` turns back: given the gradient of the output of a call, it is the
     gradient of its input. positions int32 or int64 [tokens]; freqs fp64 (``rope_freqs``). ``out``
     may be X itself."""
-    if x.dtype not in _ROPE_TYPES or x.dim() != 3:
-        raise ValueError("X must be an f16 or bf16 [tokens, heads, D] tensor")
-    tokens, heads, d = x.shape
-    _rope_rows(x, "X", x.dtype, tokens, d)
-    size = _rope_angles(positions, freqs, tokens)
-    if out is None:
-        out = torch.empty((tokens, heads, d), dtype=x.dtype, device=x.device)
-    else:
-        _rope_rows(out, "out", x.dtype, tokens, d)
-        if out.shape[1] != heads:
-            raise ValueError("out must have X's heads")
-    dev = _same_device(x, positions, freqs, out)
-    _launch(dev, "kta_rope_" + _ROPE_TYPES[x.dtype], x.data_ptr(), positions.data_ptr(), size,
-            freqs.data_ptr(), out.data_ptr(), tokens, heads, d, 2 * freqs.shape[0],
-            *_row_strides(x), *_row_strides(out), int(interleaved), int(inverse), float(scale))
-    return out
-
-
-def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype, d: int) -> None:
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != d or \
-            k_cache.dtype != dtype or v_cache.dtype != dtype:
-        raise ValueError("K and V caches must be [num_blocks, block_size, Hkv, D] of Q's type and D")
-    if not k_cache.is_contiguous() or not v_cache.is_contiguous():
-        raise ValueError("K and V caches must be contiguous")
+    return (_native or _bind()).rope(x, positions, freqs, interleaved, inverse, scale, out)
 
 
 def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
@@ -455,31 +357,8 @@ def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: tor
     rotated K and the V written to ``slots`` (int64 [tokens], ``cache_slots``) of the paged caches
     [num_blocks, block_size, Hkv, D]; a negative slot writes nothing. Returns the rotated Q
     (``out`` may be Q itself). Q, K and V may be slices of one fused tensor."""
-    if q.dtype not in _ROPE_TYPES or q.dim() != 3 or k.dim() != 3:
-        raise ValueError("Q, K and V must be f16 or bf16 [tokens, heads, D] tensors")
-    tokens, hq, d = q.shape
-    hkv = k.shape[1]
-    for t, name in ((q, "Q"), (k, "K"), (v, "V")):
-        _rope_rows(t, name, q.dtype, tokens, d)
-    _caches(k_cache, v_cache, q.dtype, d)
-    if v.shape[1] != hkv or k_cache.shape[2] != hkv:
-        raise ValueError("K, V and the caches must have the same heads")
-    size = _rope_angles(positions, freqs, tokens)
-    _vector(slots, torch.int64, tokens, "slots")
-    if out is None:
-        out = torch.empty((tokens, hq, d), dtype=q.dtype, device=q.device)
-    else:
-        _rope_rows(out, "out", q.dtype, tokens, d)
-        if out.shape[1] != hq:
-            raise ValueError("out must have Q's heads")
-    dev = _same_device(q, k, v, positions, slots, freqs, k_cache, v_cache, out)
-    strides = (ctypes.c_int64 * 8)(*_row_strides(q), *_row_strides(k), *_row_strides(v),
-                                   *_row_strides(out))
-    _launch(dev, "kta_rope_cache_" + _ROPE_TYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(),
-            positions.data_ptr(), size, slots.data_ptr(), freqs.data_ptr(), out.data_ptr(),
-            k_cache.data_ptr(), v_cache.data_ptr(), tokens, hq, hkv, d, 2 * freqs.shape[0], strides,
-            k_cache.shape[0] * k_cache.shape[1], int(interleaved), float(scale))
-    return out
+    return (_native or _bind()).rope_cache(q, k, v, positions, slots, freqs, k_cache, v_cache,
+                                           interleaved, scale, out)
 
 
 def tree_attn_workspace_bytes(max_new: int, hq: int, hkv: int, d: int) -> int:
@@ -503,40 +382,8 @@ def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
 
     ``workspace`` (uint8, ``tree_attn_workspace_bytes``, any contents) is allocated on the current
     stream where none is given; calls that may run at the same time need one each."""
-    if q.dtype not in _ROPE_TYPES or q.dim() != 3 or q.stride(2) != 1 or \
-            (q.shape[1] > 1 and q.stride(1) != q.shape[2]):
-        raise ValueError("Q must be an f16 or bf16 [tokens, Hq, D] tensor with contiguous heads")
-    tokens, hq, d = q.shape
-    _caches(k_cache, v_cache, q.dtype, d)
-    nblocks, bs, hkv, _ = k_cache.shape
-    _vector(context_lens, torch.int32, None, "context_lens")
-    bsz = context_lens.shape[0]
-    _vector(offsets, torch.int32, bsz + 1, "offsets")
-    _block_tables(block_tables, bsz)
-    dev = _same_device(q, k_cache, v_cache, block_tables, context_lens, offsets)
-    if tree is not None:
-        _same_device(q, tree)
-        _vector(tree, torch.int64, tokens, "tree")
-    if out is None:
-        out = torch.empty((tokens, hq, d), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-        raise ValueError("out must be a contiguous tensor of Q's shape and type")
-    if lse is None:
-        lse = torch.empty((tokens, hq), dtype=torch.float32, device=dev)
-    elif tuple(lse.shape) != (tokens, hq) or lse.dtype != torch.float32 or not lse.is_contiguous():
-        raise ValueError("lse must be a contiguous fp32 [tokens, Hq] tensor")
-    if workspace is None:
-        workspace = torch.empty(tree_attn_workspace_bytes(max_new, hq, hkv, d), dtype=torch.uint8,
-                                device=dev)
-    _same_device(q, out, lse, workspace)
-    _launch(dev, "kta_tree_attn_" + _ROPE_TYPES[q.dtype], q.data_ptr(), k_cache.data_ptr(),
-            v_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(),
-            offsets.data_ptr(), None if tree is None else tree.data_ptr(), out.data_ptr(),
-            lse.data_ptr(), tokens, bsz, hq, hkv, d, _stride(q, 0, hq * d), nblocks, bs,
-            block_tables.shape[1], block_tables.stride(0), max_new,
-            d ** -0.5 if scale is None else float(scale), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size())
-    return out, lse
+    return (_native or _bind()).tree_attn(q, k_cache, v_cache, block_tables, context_lens, offsets,
+                                          max_new, tree, scale, out, lse, workspace)
 
 
 class _HostPipe:
