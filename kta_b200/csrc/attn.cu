@@ -131,15 +131,6 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return done != 0;
 }
 
-template <int N>
-__device__ __forceinline__ void setmaxnreg_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void setmaxnreg_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 // 2^x0, 2^x1 on the FMA pipe for x <= 2^8 (the rescale threshold bounds x from above).
 // Cody-Waite: j = round(x) by the 1.5 * 2^23 shifter, f = x - j in [-1/2, 1/2], 2^f from a
 // degree-3 polynomial (minimax in relative error, fitted for this kernel: max 7.5e-5), and

@@ -50,6 +50,17 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 
 __device__ __forceinline__ bool elect_one_lane() { return (threadIdx.x & 31) == 0; }
 
+// Registers of a thread from here on, for the whole warpgroup: the sum over the CTA's warpgroups
+// stays within what it was launched with.
+template <int N>
+__device__ __forceinline__ void setmaxnreg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void setmaxnreg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // True on one lane of a converged warp (the same one each time).
 __device__ __forceinline__ bool elect_one_sync() {
   uint32_t pred = 0;

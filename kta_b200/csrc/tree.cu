@@ -43,16 +43,17 @@ namespace tree {
 constexpr int BM = 128;               // query rows of a row tile: TMEM lanes
 constexpr int BN = 128;               // keys of a tile
 constexpr int RING = 6;               // K and V tiles in flight
-constexpr int SOFTMAX_WARPS = 4;
-constexpr int PRODUCER_WARP = 4;
-constexpr int MMA_WARP = 5;
-constexpr int NUM_THREADS = 192;
+constexpr int HK = BN / 2;            // keys of a tile that a softmax warpgroup takes
+constexpr int SOFTMAX_WARPS = 8;      // two warpgroups
+constexpr int PRODUCER_WARP = 8;
+constexpr int MMA_WARP = 9;
+constexpr int NUM_THREADS = 320;
 constexpr int MAX_DRAFT = 64;         // bits of a row of the tree
 constexpr int MAX_GROUP = 16;
 constexpr int MAX_BATCH = 1 << 16;
 constexpr int MAX_CTAS = 256;         // the workspace is sized for this many
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units: the maximum moves when it grew > 2^8
-constexpr uint32_t COL_O = 256;       // TMEM: S of buffer t at t * 128, O at 256
+constexpr uint32_t COL_O = 256;       // TMEM: S buffer i at i * 128, O of warpgroup w at 256 + w * 128
 
 enum : unsigned int {
   SITE_PROD_SLOT = 0x901,
@@ -63,8 +64,10 @@ enum : unsigned int {
   SITE_MMA_OFREE = 0x906,
   SITE_SM_S = 0x907,
   SITE_SM_V = 0x908,
-  SITE_SM_PV = 0x909,
+  SITE_SM_ML = 0x909,
   SITE_SM_O = 0x90A,
+  SITE_SM_PV = 0x90B,
+  SITE_SMEM = 0x910,     // shared memory not aligned as declared
   SITE_REQUEST = 0x911,  // lengths or offsets out of range
   SITE_BLOCK = 0x912,    // a block id out of range
 };
@@ -77,24 +80,26 @@ struct Layout {
   static constexpr int Q_HALF = BM * 128;          // [128 rows][64 d]
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_RING = OFF_Q + HALVES * Q_HALF;
-  static constexpr int OFF_BAR = OFF_RING + RING * TILE;
-  // ring_full[R], ring_empty[R], q_full, q_empty, s_full[2], p_full[2], pv_done, o_done, o_free
-  static constexpr int NUM_BARS = 2 * RING + 9;
+  static constexpr int OFF_ML = OFF_RING + RING * TILE;  // [warpgroup][128 rows] (maximum, sum)
+  static constexpr int OFF_BAR = OFF_ML + 2 * BM * 8;
+  // ring_full[R], ring_empty[R], q_full, q_empty, s_full[2], p_full[2][2], pv_done[2], ml_full,
+  // o_done, o_free
+  static constexpr int NUM_BARS = 2 * RING + 13;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
-  // misc: tmem base, abort, the range's first request and pair start, non-finite drafts
+  // misc: tmem base, abort, non-finite drafts, the range's first request and its first tile
   static constexpr int TOTAL = OFF_MISC + 64;
-  static constexpr int ALLOC = TOTAL + 1024;
-  static_assert(ALLOC <= 232448, "shared memory budget of one sm_100 CTA");
+  static_assert(TOTAL <= 232448, "shared memory budget of one sm_100 CTA");
 };
 
 // What the join kernel needs of a unit that starts in a CTA's range and ends in a later one.
 struct Desc {
   int count;    // ranges that hold a part of it; 0: none
-  int slot;     // the first part's slot (the others are slot 0 of their CTA)
+  int slot;     // the first part's slot
+  int next;     // CTA of the second part; the others follow row_tiles apart, each in slot 0
   int row;      // first query token
   int tokens;
   int kvh;
-  int pad[3];
+  int pad[2];
 };
 
 struct Params {
@@ -163,41 +168,53 @@ struct Ranges {
   }
 };
 
-// A range's walk over its segments: runs of tiles [i0, i1) of one (request, KV head).
+// A range's walk over its segments: runs of count() tiles from i0 on of one (request, KV head).
+// Few fields, since the softmax warps keep it beside a row of S.
 struct Walk {
-  Request rq;
-  int b, kvh, i0, i1, tiles;
-  long long t, end;
+  int row, tokens, ctx;  // of the request
+  int b, kvh, i0;
+  int left;              // tiles of the range from here on
+  int turn;              // the CTA of the range's that takes the segment's first row tile
 
-  __device__ __forceinline__ void open(const Params& p, int b_first, long long b_start, long long from,
-                                       long long to) {
-    b = b_first;
-    t = from;
-    end = to;
-    rq = request_of(p, b);
-    tiles = tiles_of(rq);
-    const long long rel = from - b_start;
-    kvh = static_cast<int>(rel / tiles);
-    i0 = static_cast<int>(rel - static_cast<long long>(kvh) * tiles);
-    i1 = static_cast<int>(min(static_cast<long long>(tiles), i0 + (end - t)));
+  __device__ __forceinline__ void set(const Request& r) {
+    row = r.row;
+    tokens = r.tokens;
+    ctx = r.ctx;
   }
-  __device__ __forceinline__ bool more() const { return t < end; }
+  __device__ __forceinline__ void open(const Params& p, int b_first, long long rel, int count) {
+    b = b_first;
+    left = count;
+    turn = 0;
+    set(request_of(p, b));
+    kvh = static_cast<int>(rel / tiles());
+    i0 = static_cast<int>(rel - static_cast<long long>(kvh) * tiles());
+  }
+  __device__ __forceinline__ int len() const { return ctx + tokens; }
+  __device__ __forceinline__ int tiles() const { return (len() + BN - 1) / BN; }
+  __device__ __forceinline__ int count() const { return min(tiles() - i0, left); }
   __device__ __forceinline__ void next(const Params& p) {
-    t += i1 - i0;
-    if (t >= end) return;
+    left -= count();
+    if (left <= 0) return;
+    turn = (turn + (tokens + p.tok_tile - 1) / p.tok_tile) % p.row_tiles;
     i0 = 0;
     if (++kvh == p.hkv) {
       kvh = 0;
-      do {  // tiles are left before `end`, so a request with some follows
-        rq = request_of(p, ++b);
-        tiles = tiles_of(rq);
-      } while (tiles == 0);
+      Request r;
+      do {  // tiles are left in the range, so a request with some follows
+        r = request_of(p, ++b);
+      } while (tiles_of(r) == 0);
+      set(r);
     }
-    i1 = static_cast<int>(min(static_cast<long long>(tiles), end - t));
+  }
+  // The row tile of the request that falls to CTA `member` of the range's. Requests have between
+  // one and row_tiles of them: the CTAs take turns, so that each has its share over some segments.
+  __device__ __forceinline__ int row_tile(const Params& p, int member) const {
+    const int k = member - turn;
+    return k < 0 ? k + p.row_tiles : k;
   }
   // Drafted tokens of row tile rt in the request: 0 where it has fewer.
-  __device__ __forceinline__ int tokens(const Params& p, int rt) const {
-    return max(0, min(rq.tokens - rt * p.tok_tile, p.tok_tile));
+  __device__ __forceinline__ int rows(const Params& p, int rt) const {
+    return max(0, min(tokens - rt * p.tok_tile, p.tok_tile));
   }
 };
 
@@ -209,36 +226,36 @@ __device__ __forceinline__ uint32_t view_word(uint64_t bits, int lo) {
   return lo < 64 ? static_cast<uint32_t>(bits >> lo) : 0u;
 }
 
-// One S tile of one query row (this thread's TMEM lane): P = 2^(S sl - m) over the first 64
-// columns of S, the running maximum m (log2 units) and the row sum l. m moves only when the true
-// maximum grew by more than 2^8, so O is rescaled rarely; that waits for the PV before it.
+// Half an S tile of one query row (64 keys; this thread's TMEM lane): P = 2^(S sl - m) over the
+// first 32 columns, the running maximum m (log2 units) and the row sum l of this half. m moves only
+// when the true maximum grew by more than 2^8, so O is rescaled rarely; that waits for the PV
+// before. pv_done is at most one phase behind: S of this tile was issued behind the PV before that.
 template <bool MASKED, bool BF16, int D>
-__device__ __forceinline__ bool softmax_step(uint32_t t_s, uint32_t t_o, const uint32_t (&view)[4],
+__device__ __forceinline__ bool softmax_step(uint32_t t_s, uint32_t t_o, const uint32_t (&view)[2],
                                              float sl, float& m_used, float& lsum, uint64_t* pv_done,
                                              uint32_t pv_parity, volatile int* abort,
                                              unsigned int* status) {
-  uint32_t r[BN];
+  uint32_t r[HK];
 #pragma unroll
-  for (int q = 0; q < BN / 32; ++q) {
+  for (int q = 0; q < HK / 32; ++q) {
     tmem_ld_32x32b_x32(t_s + q * 32, *reinterpret_cast<uint32_t(*)[32]>(r + q * 32));
   }
   tmem_ld_wait();
   reg_fence(r);
   if (MASKED) {
 #pragma unroll
-    for (int c = 0; c < BN; ++c) {
+    for (int c = 0; c < HK; ++c) {
       if (!((view[c / 32] >> (c % 32)) & 1u)) r[c] = __float_as_uint(-INFINITY);
     }
   }
-  float mx[8];
+  float mx[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) mx[i] = -INFINITY;
+  for (int i = 0; i < 4; ++i) mx[i] = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < BN / 2; ++i) {
-    mx[i & 7] = max3(mx[i & 7], __uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+  for (int i = 0; i < HK / 2; ++i) {
+    mx[i & 3] = max3(mx[i & 3], __uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
   }
-  const float rmax = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]),
-                          fmaxf(mx[6], mx[7])) * sl;
+  const float rmax = max3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * sl;
   float factor = 1.f;
   bool rescale = false;
   if (rmax > m_used + RESCALE_THRESHOLD) {
@@ -248,20 +265,18 @@ __device__ __forceinline__ bool softmax_step(uint32_t t_s, uint32_t t_o, const u
   }
   lsum *= factor;
   if (__any_sync(0xffffffffu, rescale)) {
-    // The PV of the tile before (parity pv_parity). The one before that is complete, since this
-    // tile's S was issued behind it, so the barrier is at most one phase behind.
     if (!mbar_wait(pv_done, pv_parity, abort, status, SITE_SM_PV)) return false;
     tc_fence_after();
     const float f = rescale ? factor : 1.f;
 #pragma unroll 1
-    for (int c = 0; c < D; c += 32) {
-      uint32_t o[32];
-      tmem_ld_32x32b_x32(t_o + c, o);
+    for (int c = 0; c < D; c += 16) {
+      uint32_t o[16];
+      tmem_ld_32x32b_x16(t_o + c, o);
       tmem_ld_wait();
       reg_fence(o);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-      tmem_st_32x32b_x32(t_o + c, o);
+      for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+      tmem_st_32x32b_x16(t_o + c, o);
     }
   }
   // a row that has seen nothing keeps m = -inf: subtract 0 there, every exponential is 2^-inf
@@ -269,21 +284,17 @@ __device__ __forceinline__ bool softmax_step(uint32_t t_s, uint32_t t_o, const u
   const uint64_t sl2 = f2(sl, sl);
   const uint64_t neg2 = f2(-m, -m);
   uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
+  uint32_t pk[HK / 2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t pk[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const int c = h * 64 + 2 * i;
-      const uint64_t x = fma2(f2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sl2, neg2);
-      float x0, x1;
-      f2_split(x, x0, x1);
-      const float e0 = ex2(x0), e1 = ex2(x1);
-      sum2[i & 3] = add2(sum2[i & 3], f2(e0, e1));
-      pk[i] = pack2<BF16>(e0, e1);
-    }
-    tmem_st_32x32b_x32(t_s + h * 32, pk);
+  for (int i = 0; i < HK / 2; ++i) {
+    const uint64_t x = fma2(f2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), sl2, neg2);
+    float x0, x1;
+    f2_split(x, x0, x1);
+    const float e0 = ex2(x0), e1 = ex2(x1);
+    sum2[i & 3] = add2(sum2[i & 3], f2(e0, e1));
+    pk[i] = pack2<BF16>(e0, e1);
   }
+  tmem_st_32x32b_x32(t_s, pk);
   tmem_st_wait();
   const uint64_t s01 = add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3]));
   float s0, s1;
@@ -299,15 +310,14 @@ __device__ __forceinline__ uint32_t nonfinite(uint32_t w) {
   return ((w & E) == E ? 0xffffu : 0u) | ((w >> 16 & E) == E ? 0xffff0000u : 0u);
 }
 
-// The V tile (shared memory, base `tile`) whose rows [first, valid) are drafted tokens: rows past
-// `valid` become zero, and so do drafted elements that are not finite, whose tokens are recorded
-// in bad[0..1] (bit row - first + bit0). The four softmax warps share the rows.
+// Rows [from, from + 64) of a V tile (shared memory) of which [first, valid) are drafted tokens:
+// rows past `valid` become zero, and so do drafted elements that are not finite, whose tokens are
+// recorded in bad[0..1] (token = row + token0). By the 128 threads of a warpgroup.
 template <bool BF16, int D>
-__device__ __forceinline__ void clean_v(uint8_t* tile, int first, int valid, int bit0, int tid,
+__device__ __forceinline__ void clean_v(uint8_t* tile, int from, int first, int valid, int token0, int tid,
                                         unsigned int* bad) {
   constexpr int CHUNKS = D / 8;  // 16-byte pieces of a row
-  first = max(first, 0);
-  for (int i = tid + first * CHUNKS; i < BN * CHUNKS; i += SOFTMAX_WARPS * 32) {
+  for (int i = tid + max(first, from) * CHUNKS; i < (from + HK) * CHUNKS; i += BM) {
     const int row = i / CHUNKS, ch = i % CHUNKS;
     uint4* at = reinterpret_cast<uint4*>(tile + (row >> 3) * Layout<D>::GROUP + (ch >> 3) * 1024 +
                                          (row & 7) * 128 + (ch & 7) * 16);
@@ -320,8 +330,8 @@ __device__ __forceinline__ void clean_v(uint8_t* tile, int first, int valid, int
                                nonfinite<BF16>(u.w));
     if ((n.x | n.y | n.z | n.w) != 0u) {
       *at = make_uint4(u.x & ~n.x, u.y & ~n.y, u.z & ~n.z, u.w & ~n.w);
-      const int bit = row - first + bit0;
-      atomicOr(bad + (bit >> 5), 1u << (bit & 31));
+      const int token = row + token0;
+      atomicOr(bad + (token >> 5), 1u << (token & 31));
     }
   }
 }
@@ -340,23 +350,34 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const Params p) {
   using L = Layout<D>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  // Asked for at 1024 bytes (the 128-byte swizzle's period): there is no room to round up in.
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023u) != 0) {
+    pdl_wait();
+    if (threadIdx.x == 0) {
+      record_status(p.status, KTA_ERR_LAUNCH, SITE_SMEM);
+      p.desc[blockIdx.x] = Desc{};
+    }
+    return;
+  }
   uint64_t* ring_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* ring_empty = ring_full + RING;
   uint64_t* q_full = ring_empty + RING;
   uint64_t* q_empty = q_full + 1;    // the segment's last S has read Q
   uint64_t* s_full = q_empty + 1;    // [buffer]
-  uint64_t* p_full = s_full + 2;     // [buffer]: P written, V cleaned
-  uint64_t* pv_done = p_full + 2;    // one phase for each PV
-  uint64_t* o_done = pv_done + 1;    // the segment's last PV
-  uint64_t* o_free = o_done + 1;     // the epilogue has read O
+  uint64_t* p_full = s_full + 2;     // [buffer][warpgroup]: its half of P written, of V cleaned
+  uint64_t* pv_done = p_full + 4;    // [warpgroup]: one phase for each PV into its O
+  uint64_t* ml_full = pv_done + 2;   // both warpgroups' maxima and sums are in shared memory
+  uint64_t* o_done = ml_full + 1;    // the segment's last PV
+  uint64_t* o_free = o_done + 1;     // the epilogue has read both O
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   unsigned int* bad = reinterpret_cast<unsigned int*>(smem + L::OFF_MISC + 8);   // [2]
   volatile int* first_b = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 16);
   volatile long long* first_t = reinterpret_cast<volatile long long*>(smem + L::OFF_MISC + 24);
-  long long* warp_sum = reinterpret_cast<long long*>(smem + L::OFF_RING);        // before the ring is used
+  volatile long long* all_tiles = reinterpret_cast<volatile long long*>(smem + L::OFF_MISC + 32);
+  float2* ml = reinterpret_cast<float2*>(smem + L::OFF_ML);
+  long long* warp_sum = reinterpret_cast<long long*>(smem + L::OFF_RING);  // before the ring is used
 
   const int warp = warp_id();
   const int lane = threadIdx.x & 31;
@@ -369,9 +390,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], SOFTMAX_WARPS);
+      mbar_init(&p_full[2 * i], SOFTMAX_WARPS / 2);
+      mbar_init(&p_full[2 * i + 1], SOFTMAX_WARPS / 2);
+      mbar_init(&pv_done[i], 1);
     }
-    mbar_init(pv_done, 1);
+    mbar_init(ml_full, SOFTMAX_WARPS);
     mbar_init(o_done, 1);
     mbar_init(o_free, SOFTMAX_WARPS);
     *abort_flag = 0;
@@ -416,7 +439,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     rg.total += warp_sum[w];
   }
   rg.n = static_cast<int>(min(static_cast<long long>(gridDim.x / p.row_tiles), rg.total));
-  const int range = blockIdx.x / p.row_tiles, rt = blockIdx.x % p.row_tiles;
+  if (threadIdx.x == 0) *all_tiles = rg.total;
+  const int range = blockIdx.x / p.row_tiles, member = blockIdx.x % p.row_tiles;
   const bool busy = range < rg.n;
   const long long t_begin = busy ? rg.start(range) : 0, t_end = busy ? rg.start(range + 1) : 0;
   if (busy && t_begin >= before && t_begin < before + mine) {
@@ -444,8 +468,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   fence_proxy_async_smem();  // the scan's use of the ring's memory comes before its TMA writes
   __syncthreads();
   Walk w;
-  w.t = w.end = 0;
-  if (busy) w.open(p, *first_b, *first_t, t_begin, t_end);
+  w.left = 0;
+  if (busy) w.open(p, *first_b, t_begin - *first_t, static_cast<int>(t_end - t_begin));
 
   if (warp == PRODUCER_WARP) {
     // ------------------------------ TMA producer ------------------------------
@@ -459,7 +483,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // the index of the page's first (token, head) row, for this lane's page of tile i
     auto page_of = [&](const Walk& s, int i) -> int {
       const int box_index = i * pages + lane;
-      if (lane >= pages || (static_cast<long long>(box_index) << p.box_log2) >= s.rq.len) return 0;
+      if (lane >= pages || (static_cast<long long>(box_index) << p.box_log2) >= s.len()) return 0;
       const int id = p.tables[s.b * p.table_stride + (box_index >> split)];
       if (id < 0 || id >= p.num_blocks) {
         record_status(p.status, KTA_ERR_DEVICE_BOUNDS, SITE_BLOCK);
@@ -473,7 +497,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         return false;
       }
       ++n;
-      const int held = min(pages, (s.rq.len - i * BN + box - 1) >> p.box_log2);
+      const int held = min(pages, (s.len() - i * BN + box - 1) >> p.box_log2);
       if (lane == 0) {
         mbar_arrive_expect_tx(&ring_full[st], static_cast<uint32_t>(held * group_box * L::GROUP));
       }
@@ -486,11 +510,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       __syncwarp();
       return true;
     };
-    for (; w.more() && ok; w.next(p)) {
-      const int tokens = w.tokens(p, rt);
+    for (; w.left > 0 && ok; w.next(p)) {
+      const int rt = w.row_tile(p, member);
+      const int tokens = w.rows(p, rt);
       if (tokens == 0) continue;
       int cur = page_of(w, w.i0);
-      int nxt = w.i0 + 1 < w.i1 ? page_of(w, w.i0 + 1) : 0;
+      const int end = w.i0 + w.count();
+      int nxt = w.i0 + 1 < end ? page_of(w, w.i0 + 1) : 0;
       if (!load(w, w.i0, cur, &tmK)) break;
       if (!mbar_wait(q_empty, qphase ^ 1u, abort_flag, p.status, SITE_PROD_Q)) break;
       qphase ^= 1u;
@@ -499,13 +525,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
         for (int h = 0; h < L::HALVES; ++h) {
           tma_load_3d(&tmQ, q_full, smem + L::OFF_Q + h * L::Q_HALF, h * 64, w.kvh * p.group,
-                      w.rq.row + rt * p.tok_tile);
+                      w.row + rt * p.tok_tile);
         }
       }
       __syncwarp();
-      for (int i = w.i0; i < w.i1; ++i) {
-        const int after = i + 2 < w.i1 ? page_of(w, i + 2) : 0;  // in flight during the waits
-        if (i + 1 < w.i1 && !load(w, i + 1, nxt, &tmK)) {
+      for (int i = w.i0; i < end; ++i) {
+        const int after = i + 2 < end ? page_of(w, i + 2) : 0;  // in flight during the waits
+        if (i + 1 < end && !load(w, i + 1, nxt, &tmK)) {
           ok = false;
           break;
         }
@@ -532,8 +558,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     constexpr uint32_t idesc_o = make_idesc(BM, D, FMT, FMT, 0u, 1u);   // P (TMEM) V (MN-major)
     const uint64_t qdesc = sdesc_sw128(smem_u32(smem + L::OFF_Q), 16, 1024);
     uint32_t n = 0;     // tiles taken from the ring
-    uint32_t g = 0;     // key tiles so far
-    uint32_t qphase = 0, ofree_phase = 0;
+    uint32_t g = 0;     // tiles of keys so far: buffer g & 1, its phase (g >> 1) & 1
+    uint32_t q_phase = 0, o_phase = 0;
     bool first_segment = true, ok = true;
     auto take = [&](int* st) -> bool {
       *st = static_cast<int>(n % RING);
@@ -541,7 +567,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       ++n;
       return mbar_wait(&ring_full[*st], ph, abort_flag, p.status, SITE_MMA_KV);
     };
-    auto issue_s = [&](uint32_t tile, uint64_t* last) -> bool {
+    // S of tile t into buffer t & 1, which holds P of tile t - 2 until its PV has read it: that was
+    // issued before and ends before this begins.
+    auto issue_s = [&](uint32_t t, bool last) -> bool {
       int st;
       if (!take(&st)) return false;
       tc_fence_after();
@@ -551,86 +579,86 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t qo = ((kk >> 2) * L::Q_HALF + (kk & 3) * 32) >> 4;
           const uint32_t ko = ((kk >> 2) * 1024 + (kk & 3) * 32) >> 4;
-          umma_f16(tmem + (tile & 1u) * BN, qdesc + qo, kdesc + ko, idesc_s, kk > 0 ? 1u : 0u);
+          umma_f16(tmem + (t & 1u) * BN, qdesc + qo, kdesc + ko, idesc_s, kk > 0 ? 1u : 0u);
         }
-        umma_commit(&s_full[tile & 1u]);
+        umma_commit(&s_full[t & 1u]);
         umma_commit(&ring_empty[st]);
-        if (last != nullptr) umma_commit(last);
+        if (last) umma_commit(q_empty);
       }
       __syncwarp();
       return true;
     };
-    for (; w.more() && ok; w.next(p)) {
-      if (w.tokens(p, rt) == 0) continue;
-      if (!mbar_wait(q_full, qphase, abort_flag, p.status, SITE_MMA_Q)) break;
-      qphase ^= 1u;
-      const int tiles = w.i1 - w.i0;
-      if (!issue_s(g, tiles == 1 ? q_empty : nullptr)) break;
-      for (int j = 0; j < tiles; ++j, ++g) {
-        if (j + 1 < tiles && !issue_s(g + 1, j + 2 == tiles ? q_empty : nullptr)) {
-          ok = false;
-          break;
-        }
+    for (; w.left > 0 && ok; w.next(p)) {
+      if (w.rows(p, w.row_tile(p, member)) == 0) continue;
+      if (!mbar_wait(q_full, q_phase, abort_flag, p.status, SITE_MMA_Q)) break;
+      q_phase ^= 1u;
+      const int tiles = w.count();
+      if (!issue_s(g, tiles == 1)) break;
+      for (int j = 0; j < tiles && ok; ++j, ++g) {
         int st;
-        if (!take(&st) || !mbar_wait(&p_full[g & 1u], (g >> 1) & 1u, abort_flag, p.status, SITE_MMA_P)) {
-          ok = false;
-          break;
-        }
-        if (j == 0 && !first_segment) {  // the last segment's O has been read
-          if (!mbar_wait(o_free, ofree_phase, abort_flag, p.status, SITE_MMA_OFREE)) {
-            ok = false;
-            break;
-          }
-          ofree_phase ^= 1u;
-        }
-        tc_fence_after();
+        ok = (j + 1 == tiles || issue_s(g + 1, j + 2 == tiles)) && take(&st);
+        if (!ok) break;
         const uint64_t vdesc = sdesc_sw128(smem_u32(smem + L::OFF_RING + st * L::TILE), 1024, L::GROUP);
-        if (elect_one_sync()) {
 #pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk) {
-            umma_f16_tmem_a(tmem + COL_O, tmem + (g & 1u) * BN + kk * 8,
-                            vdesc + static_cast<uint64_t>(kk * 2 * L::GROUP / 16), idesc_o,
-                            (j > 0 || kk > 0) ? 1u : 0u);
+        for (int h = 0; h < 2; ++h) {  // the warpgroups' halves of the keys, into their own O
+          ok = mbar_wait(&p_full[2 * (g & 1u) + h], (g >> 1) & 1u, abort_flag, p.status, SITE_MMA_P);
+          if (!ok) break;
+          if (j == 0 && h == 0 && !first_segment) {  // the last segment's O has been read
+            ok = mbar_wait(o_free, o_phase, abort_flag, p.status, SITE_MMA_OFREE);
+            if (!ok) break;
+            o_phase ^= 1u;
           }
-          umma_commit(pv_done);
-          umma_commit(&ring_empty[st]);
-          if (j + 1 == tiles) umma_commit(o_done);
+          tc_fence_after();
+          if (elect_one_sync()) {
+#pragma unroll
+            for (int kk = 0; kk < HK / 16; ++kk) {
+              umma_f16_tmem_a(tmem + COL_O + h * BN, tmem + (g & 1u) * BN + h * HK + kk * 8,
+                              vdesc + static_cast<uint64_t>((h * HK / 16 + kk) * 2 * L::GROUP / 16),
+                              idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+            }
+            umma_commit(&pv_done[h]);
+            if (h == 1) umma_commit(&ring_empty[st]);
+            if (h == 1 && j + 1 == tiles) umma_commit(o_done);
+          }
+          __syncwarp();
         }
-        __syncwarp();
       }
       first_segment = false;
     }
   } else {
     // ------------- softmax, O correction and epilogue (thread = query row) -------------
-    const int row = threadIdx.x;
-    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
-    const uint32_t t_o = tmem + lane_base + COL_O;
+    const int wg = warp >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t t_s = tmem + lane_base + wg * HK;  // this half of S buffer 0
+    const uint32_t t_o = tmem + lane_base + COL_O;    // O of warpgroup 0; the other's is BN columns on
     const float sl = p.scale_log2;
-    const int tok = row / p.group, head = row - tok * p.group;
-    uint32_t g = 0, n = 0;  // key tiles so far; their K and V loads into the ring
+    uint32_t n = 0;  // loads into the ring of the segments so far
+    uint32_t g = 0;  // tiles of keys so far
     uint32_t o_phase = 0;
     bool ok = true;
-    Desc d = {};
-    for (bool first = true; w.more() && ok; w.next(p)) {
-      const int tokens = w.tokens(p, rt);
+    if (threadIdx.x == 0) p.desc[blockIdx.x] = Desc{};  // no unit to join so far
+    for (bool first = true; w.left > 0 && ok; w.next(p)) {
+      const int rt = w.row_tile(p, member);
+      const int tokens = w.rows(p, rt);
       const bool first_part = first;
       first = false;
       if (tokens == 0) continue;
       const int rows = tokens * p.group;
       const bool live = row < rows;
-      const bool warp_on = warp * 32 < rows;
+      const bool warp_on = quarter * 32 < rows;
       uint64_t bits = 0;
       if (live) {
-        const int t = rt * p.tok_tile + tok;
-        bits = p.tree != nullptr ? static_cast<uint64_t>(__ldg(p.tree + w.rq.row + t))
+        const int t = rt * p.tok_tile + row / p.group;
+        bits = p.tree != nullptr ? static_cast<uint64_t>(__ldg(p.tree + w.row + t))
                                  : (2ull << t) - 1ull;  // t = 63: all ones
-        if (w.rq.tokens < 64) bits &= (1ull << w.rq.tokens) - 1ull;
+        if (w.tokens < 64) bits &= (1ull << w.tokens) - 1ull;
       }
-      const int tiles = w.i1 - w.i0;
+      const int tiles = w.count();
       float m_used = -INFINITY, lsum = 0.f;
       for (int j = 0; j < tiles; ++j, ++g) {
         const int k0 = (w.i0 + j) * BN;
-        const bool masked = k0 + BN > w.rq.ctx;
+        const bool masked = k0 + BN > w.ctx;
         if (masked) {
           // V(j) is the load 2 j + 2 of the segment, or 2 j + 1 for its last tile
           const uint32_t vn = n + 2 * j + (j + 1 < tiles ? 2 : 1);
@@ -639,8 +667,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             ok = false;
             break;
           }
-          clean_v<BF16, D>(smem + L::OFF_RING + st * L::TILE, w.rq.ctx - k0, w.rq.len - k0,
-                           max(k0 - w.rq.ctx, 0), row, bad);
+          clean_v<BF16, D>(smem + L::OFF_RING + st * L::TILE, wg * HK, w.ctx - k0, w.len() - k0, k0 - w.ctx,
+                           row, bad);
           fence_proxy_async_smem();
         }
         if (!mbar_wait(&s_full[g & 1u], (g >> 1) & 1u, abort_flag, p.status, SITE_SM_S)) {
@@ -649,48 +677,69 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         tc_fence_after();
         if (warp_on) {
-          const uint32_t t_s = tmem + lane_base + (g & 1u) * BN;
-          uint32_t view[4];
+          const uint32_t at = t_s + (g & 1u) * BN;
+          uint32_t view[2];
           if (masked) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) view[q] = view_word(bits, k0 + 32 * q - w.rq.ctx);
-            ok = softmax_step<true, BF16, D>(t_s, t_o, view, sl, m_used, lsum, pv_done, (g - 1) & 1u,
-                                             abort_flag, p.status);
+            view[0] = view_word(bits, k0 + wg * HK - w.ctx);
+            view[1] = view_word(bits, k0 + wg * HK + 32 - w.ctx);
+            ok = softmax_step<true, BF16, D>(at, t_o + wg * BN, view, sl, m_used, lsum, &pv_done[wg],
+                                             (g - 1) & 1u, abort_flag, p.status);
           } else {
-            ok = softmax_step<false, BF16, D>(t_s, t_o, view, sl, m_used, lsum, pv_done, (g - 1) & 1u,
-                                              abort_flag, p.status);
+            ok = softmax_step<false, BF16, D>(at, t_o + wg * BN, view, sl, m_used, lsum, &pv_done[wg],
+                                              (g - 1) & 1u, abort_flag, p.status);
           }
           if (!ok) break;
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[g & 1u]);
+        if (lane == 0) mbar_arrive(&p_full[2 * (g & 1u) + wg]);
       }
       n += 2 * tiles;
       if (!ok) break;
+      // ---- epilogue: the two warpgroups' states become one, each for half of D ----
+      ml[wg * BM + row] = make_float2(m_used, lsum);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ml_full);
+      if (!mbar_wait(ml_full, o_phase, abort_flag, p.status, SITE_SM_ML)) break;
       if (!mbar_wait(o_done, o_phase, abort_flag, p.status, SITE_SM_O)) break;
       o_phase ^= 1u;
       tc_fence_after();
-      // ---- epilogue ----
-      const bool whole = w.i0 == 0 && w.i1 == w.tiles;
+      const bool whole = w.i0 == 0 && tiles == w.tiles();
       const int slot = 2 * static_cast<int>(blockIdx.x) + (first_part ? 0 : 1);
-      const int token = w.rq.row + rt * p.tok_tile + tok;
+      const int tok = row / p.group, head = row - tok * p.group;
+      const int token = w.row + rt * p.tok_tile + tok;
       const int q_head = w.kvh * p.group + head;
-      uint64_t lost = bits & (static_cast<uint64_t>(bad[1]) << 32 | bad[0]);
+      const uint64_t lost = bits & (static_cast<uint64_t>(bad[1]) << 32 | bad[0]);
       if (warp_on) {
-        const float inv = lsum == 0.f ? 0.f : 1.f / lsum;  // a row that sees nothing: O = 0
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
+        const float2 a = ml[row], b = ml[BM + row];
+        const float m = fmaxf(a.x, b.x);
+        const float base = m == -INFINITY ? 0.f : m;
+        float wa = ex2(a.x - base), wb = ex2(b.x - base);
+        const float l = fmaf(wa, a.y, wb * b.y);
+        if (whole) {  // a row that sees nothing: O = 0
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          wa *= inv;
+          wb *= inv;
+        }
+#pragma unroll 1
+        for (int c = wg * (D / 2); c < (wg + 1) * (D / 2); c += 32) {
+          uint32_t o[32], o1[32];
           tmem_ld_32x32b_x32(t_o + c, o);
+          tmem_ld_32x32b_x32(t_o + BN + c, o1);
           tmem_ld_wait();
           reg_fence(o);
+          reg_fence(o1);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            o[i] = __float_as_uint(fmaf(__uint_as_float(o[i]), wa, __uint_as_float(o1[i]) * wb));
+          }
           if (live && lost != 0) {
             // drafted V elements that are not finite, for the rows that see them
             for (uint64_t left = lost; left != 0; left &= left - 1) {
-              const int key = w.rq.ctx + __ffsll(static_cast<long long>(left)) - 1;
+              const int key = w.ctx + __ffsll(static_cast<long long>(left)) - 1;
+              if (key < w.i0 * BN || key >= (w.i0 + tiles) * BN) continue;
               const int id = p.tables[w.b * p.table_stride + (key >> p.page_log2)];
-              if (key < w.i0 * BN || key >= w.i1 * BN || id < 0 || id >= p.num_blocks) continue;
+              if (id < 0 || id >= p.num_blocks) continue;
               const long long at =
                   (((static_cast<long long>(id) << p.page_log2) + (key & ((1 << p.page_log2) - 1))) *
                        p.hkv + w.kvh) * D + c;
@@ -709,8 +758,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               uint32_t pk[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                pk[e] = pack2<BF16>(__uint_as_float(o[8 * i + 2 * e]) * inv,
-                                    __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+                pk[e] = pack2<BF16>(__uint_as_float(o[8 * i + 2 * e]), __uint_as_float(o[8 * i + 2 * e + 1]));
               }
               dst[i] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
             }
@@ -724,26 +772,31 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             }
           }
         }
-        if (live && whole) {
+        if (wg == 0 && live && whole) {
           p.lse[static_cast<long long>(token) * p.hq + q_head] =
-              lsum == 0.f ? -INFINITY : (m_used + log2f(lsum)) * 0.6931471805599453f;
-        } else if (live) {
-          p.part_ml[static_cast<long long>(slot) * p.row_cap + row] = make_float2(m_used, lsum);
+              l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        } else if (wg == 0 && live) {
+          p.part_ml[static_cast<long long>(slot) * p.row_cap + row] = make_float2(m, l);
         }
       }
-      if (!whole && w.i0 == 0) {  // the unit starts here: this CTA describes it
-        const long long last = w.t + w.tiles - 1;
-        d.count = rg.owner(last) - range + 1;
+      if (threadIdx.x == 0 && !whole && w.i0 == 0) {  // the unit starts here: this CTA describes it
+        Ranges r;
+        r.total = *all_tiles;
+        r.n = static_cast<int>(min(static_cast<long long>(gridDim.x / p.row_tiles), r.total));
+        const long long last = r.start(range + 1) - w.left + w.tiles() - 1;
+        Desc d = {};
+        d.count = r.owner(last) - range + 1;
         d.slot = slot;
-        d.row = w.rq.row + rt * p.tok_tile;
+        d.next = (range + 1) * p.row_tiles + rt;  // a range's first segment is row tile = member
+        d.row = w.row + rt * p.tok_tile;
         d.tokens = tokens;
         d.kvh = w.kvh;
+        p.desc[blockIdx.x] = d;
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free);
     }
-    if (threadIdx.x == 0) p.desc[blockIdx.x] = d;
   }
 
   tc_fence_before();
@@ -782,7 +835,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Params p) {
         ml[i] = make_float2(-INFINITY, 0.f);
         part[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (c < d.count) {
-          const long long slot = c == 0 ? d.slot : 2LL * (blockIdx.x + c * p.row_tiles);
+          const long long slot = c == 0 ? d.slot : 2LL * (d.next + (c - 1) * p.row_tiles);
           ml[i] = __ldcg(p.part_ml + slot * p.row_cap + row);
           part[i] = __ldcg(p.part_o + (slot * (D / 4) + d4) * p.row_cap + row);
         }
@@ -860,12 +913,12 @@ int go(Params& p, const void* Q, const void* Kc, const void* Vc, int64_t q_token
   s = encode_tmap(&tv, type, 5, Vc, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   if (s != KTA_OK) return s;
   auto kernel = tree_kernel<BF16, D>;
-  s = set_kernel_smem(reinterpret_cast<const void*>(kernel), L::ALLOC);
+  s = set_kernel_smem(reinterpret_cast<const void*>(kernel), L::TOTAL);
   if (s != KTA_OK) return s;
   const int sms = std::min(current_sm_count(), MAX_CTAS);
   if (sms < p.row_tiles) return KTA_ERR_UNSUPPORTED;
   const int grid = sms / p.row_tiles * p.row_tiles;
-  s = launch_ex(kernel, dim3(grid), dim3(NUM_THREADS), L::ALLOC, stream, 1, tq, tk, tv, p);
+  s = launch_ex(kernel, dim3(grid), dim3(NUM_THREADS), L::TOTAL, stream, 1, tq, tk, tv, p);
   if (s != KTA_OK) return s;
   // four elements a thread and at most four passes
   const int parts = std::max(1, std::min(8, p.row_cap * (D / 4) / (2 * JOIN_THREADS)));
