@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(THREADS) slots_kernel(const Params p) {
           id[i] = p.tables[b * p.table_stride + j];
         } else {
           const long long k = static_cast<long long>(blk0[b]) + (j - held);
-          if (k < p.pool_size) id[i] = __ldg(p.pool + k);
+          if (k < p.pool_size) id[i] = p.pool[k];
         }
       }
     }
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(THREADS) slots_kernel(const Params p) {
   for (long long k = blockIdx.x * THREADS + threadIdx.x; k < total_blks; k += step) {
     const int b = owner_of(blk0, p.batch, static_cast<int>(k));
     const long long j = blocks_of(held_tokens[b], p.block) + (k - blk0[b]);
-    p.tables[b * p.table_stride + j] = k < p.pool_size ? __ldg(p.pool + k) : -1;
+    p.tables[b * p.table_stride + j] = k < p.pool_size ? p.pool[k] : -1;
   }
 }
 

@@ -42,12 +42,14 @@ namespace tree {
 
 constexpr int BM = 128;               // query rows of a row tile: TMEM lanes
 constexpr int BN = 128;               // keys of a tile
-constexpr int RING = 6;               // K and V tiles in flight
+constexpr int RING = 3;               // K tiles in flight, and V tiles
 constexpr int HK = BN / 2;            // keys of a tile that a softmax warpgroup takes
 constexpr int SOFTMAX_WARPS = 8;      // two warpgroups
-constexpr int PRODUCER_WARP = 8;
-constexpr int MMA_WARP = 9;
-constexpr int NUM_THREADS = 320;
+constexpr int MMA_WARP = 8;
+constexpr int K_WARP = 9;             // TMA producers
+constexpr int V_WARP = 10;
+constexpr int Q_WARP = 11;
+constexpr int NUM_THREADS = 384;
 constexpr int MAX_DRAFT = 64;         // bits of a row of the tree
 constexpr int MAX_GROUP = 16;
 constexpr int MAX_BATCH = 1 << 16;
@@ -56,10 +58,11 @@ constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units: the maximum moves when
 constexpr uint32_t COL_O = 256;       // TMEM: S buffer i at i * 128, O of warpgroup w at 256 + w * 128
 
 enum : unsigned int {
-  SITE_PROD_SLOT = 0x901,
+  SITE_PROD_KV = 0x901,
   SITE_PROD_Q = 0x902,
   SITE_MMA_Q = 0x903,
-  SITE_MMA_KV = 0x904,
+  SITE_MMA_K = 0x904,
+  SITE_MMA_V = 0x90C,
   SITE_MMA_P = 0x905,
   SITE_MMA_OFREE = 0x906,
   SITE_SM_S = 0x907,
@@ -79,14 +82,15 @@ struct Layout {
   static constexpr int TILE = BN / 8 * GROUP;      // a K or V tile
   static constexpr int Q_HALF = BM * 128;          // [128 rows][64 d]
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_RING = OFF_Q + HALVES * Q_HALF;
-  static constexpr int OFF_ML = OFF_RING + RING * TILE;  // [warpgroup][128 rows] (maximum, sum)
+  static constexpr int OFF_K = OFF_Q + HALVES * Q_HALF;
+  static constexpr int OFF_V = OFF_K + RING * TILE;
+  static constexpr int OFF_ML = OFF_V + RING * TILE;  // [warpgroup][128 rows] (maximum, sum)
   static constexpr int OFF_BAR = OFF_ML + 2 * BM * 8;
-  // ring_full[R], ring_empty[R], q_full, q_empty, s_full[2], p_full[2][2], pv_done[2], ml_full,
-  // o_done, o_free
-  static constexpr int NUM_BARS = 2 * RING + 13;
+  // k_full[R], k_empty[R], v_full[R], v_empty[R], q_full[2], q_empty[2], s_full[2], p_full[2][2],
+  // pv_done[2], ml_full, o_done, o_free
+  static constexpr int NUM_BARS = 4 * RING + 15;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
-  // misc: tmem base, abort, non-finite drafts, the range's first request and its first tile
+  // misc: tmem base, abort, non-finite drafts, the range's first segment and end
   static constexpr int TOTAL = OFF_MISC + 64;
   static_assert(TOTAL <= 232448, "shared memory budget of one sm_100 CTA");
 };
@@ -120,6 +124,7 @@ struct Params {
   int tok_tile;            // drafted tokens of a row tile: 128 / group
   int box_tokens;          // tokens of the Q box: min(tok_tile, max_new)
   int row_tiles;           // CTAs that share a range
+  int q_bufs, q_shift;     // Q tiles in shared memory, bytes from one to the next
   int row_cap;             // rows of a partial
   float scale_log2;        // softmax scale * log2(e)
   unsigned int* status;
@@ -157,14 +162,25 @@ __device__ __forceinline__ int tiles_of(const Request& r) {
   return r.tokens > 0 ? (r.len + BN - 1) / BN : 0;
 }
 
-// The work list: tile i of KV head h of request b, b-major; range k of n is
-// [total k / n, total (k + 1) / n), and n <= total, so that none is empty.
+// Row tiles of a request.
+__device__ __forceinline__ int row_tiles_of(const Params& p, int tokens) {
+  return (tokens + p.tok_tile - 1) / p.tok_tile;
+}
+
+// The work list: tile i of KV head h of request b, b-major, each counted once for every row tile
+// of its request (the CTAs of a range share those). Range k of n is [total k / n, total (k + 1) / n)
+// rounded down to whole tiles; n <= total / row_tiles, so that none is empty.
 struct Ranges {
-  long long total;
-  int n;
-  __device__ __forceinline__ long long start(int k) const { return total * k / n; }
-  __device__ __forceinline__ int owner(long long t) const {
-    return static_cast<int>(((t + 1) * n - 1) / total);
+  int total, n;
+  __device__ __forceinline__ Ranges(const Params& p, int total_) : total(total_) {
+    n = total == 0 ? 0 : max(1, min(static_cast<int>(gridDim.x) / p.row_tiles, total / p.row_tiles));
+  }
+  __device__ __forceinline__ int start(int k) const {
+    return static_cast<int>(static_cast<long long>(total) * k / n);
+  }
+  // the range of the last tile before position `end`, the end of a unit
+  __device__ __forceinline__ int owner_before(int end) const {
+    return static_cast<int>((static_cast<long long>(end) * n - 1) / total);
   }
 };
 
@@ -173,7 +189,7 @@ struct Ranges {
 struct Walk {
   int row, tokens, ctx;  // of the request
   int b, kvh, i0;
-  int left;              // tiles of the range from here on
+  int left;              // of the range from here on, in the work list's count
   int turn;              // the CTA of the range's that takes the segment's first row tile
 
   __device__ __forceinline__ void set(const Request& r) {
@@ -181,21 +197,16 @@ struct Walk {
     tokens = r.tokens;
     ctx = r.ctx;
   }
-  __device__ __forceinline__ void open(const Params& p, int b_first, long long rel, int count) {
-    b = b_first;
-    left = count;
-    turn = 0;
-    set(request_of(p, b));
-    kvh = static_cast<int>(rel / tiles());
-    i0 = static_cast<int>(rel - static_cast<long long>(kvh) * tiles());
-  }
   __device__ __forceinline__ int len() const { return ctx + tokens; }
   __device__ __forceinline__ int tiles() const { return (len() + BN - 1) / BN; }
-  __device__ __forceinline__ int count() const { return min(tiles() - i0, left); }
+  __device__ __forceinline__ int count(const Params& p) const {
+    return min(tiles() - i0, left / row_tiles_of(p, tokens));
+  }
   __device__ __forceinline__ void next(const Params& p) {
-    left -= count();
+    const int k = row_tiles_of(p, tokens);
+    left -= count(p) * k;
     if (left <= 0) return;
-    turn = (turn + (tokens + p.tok_tile - 1) / p.tok_tile) % p.row_tiles;
+    turn = (turn + k) % p.row_tiles;
     i0 = 0;
     if (++kvh == p.hkv) {
       kvh = 0;
@@ -215,6 +226,10 @@ struct Walk {
   // Drafted tokens of row tile rt in the request: 0 where it has fewer.
   __device__ __forceinline__ int rows(const Params& p, int rt) const {
     return max(0, min(tokens - rt * p.tok_tile, p.tok_tile));
+  }
+  // To the next segment, this one included, in which CTA `member` has rows.
+  __device__ __forceinline__ void settle(const Params& p, int member) {
+    while (left > 0 && rows(p, row_tile(p, member)) == 0) next(p);
   }
 };
 
@@ -360,11 +375,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     }
     return;
   }
-  uint64_t* ring_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
-  uint64_t* ring_empty = ring_full + RING;
-  uint64_t* q_full = ring_empty + RING;
-  uint64_t* q_empty = q_full + 1;    // the segment's last S has read Q
-  uint64_t* s_full = q_empty + 1;    // [buffer]
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
+  uint64_t* k_empty = k_full + RING;
+  uint64_t* v_full = k_empty + RING;
+  uint64_t* v_empty = v_full + RING;
+  uint64_t* q_full = v_empty + RING;  // [Q buffer]
+  uint64_t* q_empty = q_full + 2;     // [Q buffer]: the segment's last S has read Q
+  uint64_t* s_full = q_empty + 2;    // [S buffer]
   uint64_t* p_full = s_full + 2;     // [buffer][warpgroup]: its half of P written, of V cleaned
   uint64_t* pv_done = p_full + 4;    // [warpgroup]: one phase for each PV into its O
   uint64_t* ml_full = pv_done + 2;   // both warpgroups' maxima and sums are in shared memory
@@ -373,22 +390,24 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   unsigned int* bad = reinterpret_cast<unsigned int*>(smem + L::OFF_MISC + 8);   // [2]
-  volatile int* first_b = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 16);
-  volatile long long* first_t = reinterpret_cast<volatile long long*>(smem + L::OFF_MISC + 24);
-  volatile long long* all_tiles = reinterpret_cast<volatile long long*>(smem + L::OFF_MISC + 32);
+  // the range's first segment (request, KV head, tile), its place in the work list, the range's end,
+  // and the list's total
+  volatile int* plan = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 16);  // [6]
   float2* ml = reinterpret_cast<float2*>(smem + L::OFF_ML);
-  long long* warp_sum = reinterpret_cast<long long*>(smem + L::OFF_RING);  // before the ring is used
+  int* warp_sum = reinterpret_cast<int*>(smem + L::OFF_K);  // before the ring is used
 
   const int warp = warp_id();
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < RING; ++s) {
-      mbar_init(&ring_full[s], 1);
-      mbar_init(&ring_empty[s], 1);
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
     }
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[2 * i], SOFTMAX_WARPS / 2);
       mbar_init(&p_full[2 * i + 1], SOFTMAX_WARPS / 2);
@@ -401,7 +420,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     bad[0] = bad[1] = 0u;
     fence_barrier_init();
   }
-  if (warp == PRODUCER_WARP && lane == 0) {
+  if (warp == K_WARP && lane == 0) {
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
@@ -414,15 +433,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   // after the wait: the join kernel may be scheduled now, and waits for this grid itself
   pdl_launch_dependents();
 
-  // ---- tiles before each request: thread i sums a run of requests ----
+  // ---- the work list: thread i sums a run of requests ----
   const int per = (p.batch + NUM_THREADS - 1) / NUM_THREADS;
   const int b0 = min(static_cast<int>(threadIdx.x) * per, p.batch), b1 = min(b0 + per, p.batch);
-  long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += static_cast<long long>(tiles_of(request_of(p, b))) * p.hkv;
-  long long incl = mine;
+  auto work_of = [&](const Request& r) { return tiles_of(r) * p.hkv * row_tiles_of(p, r.tokens); };
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) mine += work_of(request_of(p, b));
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
   if (lane == 31) warp_sum[warp] = incl;
@@ -430,29 +450,43 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
-  long long before = incl - mine;
-  Ranges rg;
-  rg.total = 0;
+  int before = incl - mine, total = 0;
 #pragma unroll
   for (int w = 0; w < NUM_THREADS / 32; ++w) {
     if (w < warp) before += warp_sum[w];
-    rg.total += warp_sum[w];
+    total += warp_sum[w];
   }
-  rg.n = static_cast<int>(min(static_cast<long long>(gridDim.x / p.row_tiles), rg.total));
-  if (threadIdx.x == 0) *all_tiles = rg.total;
+  const Ranges rg(p, total);
   const int range = blockIdx.x / p.row_tiles, member = blockIdx.x % p.row_tiles;
   const bool busy = range < rg.n;
-  const long long t_begin = busy ? rg.start(range) : 0, t_end = busy ? rg.start(range + 1) : 0;
-  if (busy && t_begin >= before && t_begin < before + mine) {
-    long long t = before;
-    for (int b = b0; b < b1; ++b) {
-      const long long k = static_cast<long long>(tiles_of(request_of(p, b))) * p.hkv;
-      if (t_begin < t + k) {
-        *first_b = b;
-        *first_t = t;
+  if (busy) {
+    // the range's two ends, by the threads whose requests they fall into
+    const int from = rg.start(range), to = rg.start(range + 1);
+    for (int e = 0; e < 2; ++e) {
+      const int at = e == 0 ? from : to;
+      if (at < before || at >= before + mine) continue;
+      int t = before;
+      for (int b = b0; b < b1; ++b) {
+        const Request r = request_of(p, b);
+        const int n = work_of(r);
+        if (at >= t + n) {
+          t += n;
+          continue;
+        }
+        const int k = row_tiles_of(p, r.tokens), pair = tiles_of(r) * k;
+        const int kvh = (at - t) / pair, off = at - t - kvh * pair;
+        if (e == 0) {
+          plan[0] = b;
+          plan[1] = kvh;
+          plan[2] = off / k;
+        }
+        plan[3 + e] = at - off % k;
         break;
       }
-      t += k;
+    }
+    if (threadIdx.x == 0) {
+      if (to == total) plan[4] = total;
+      plan[5] = total;
     }
   }
   // requests that are out of range: their rows that exist become zero
@@ -469,111 +503,117 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   __syncthreads();
   Walk w;
   w.left = 0;
-  if (busy) w.open(p, *first_b, t_begin - *first_t, static_cast<int>(t_end - t_begin));
+  if (busy) {
+    w.b = plan[0];
+    w.kvh = plan[1];
+    w.i0 = plan[2];
+    w.left = plan[4] - plan[3];
+    w.turn = 0;
+    w.set(request_of(p, w.b));
+    w.settle(p, member);
+  }
 
-  if (warp == PRODUCER_WARP) {
-    // ------------------------------ TMA producer ------------------------------
-    uint32_t n = 0;  // loads into the ring so far
-    uint32_t qphase = 0;
-    bool ok = true;
+  if (warp == K_WARP || warp == V_WARP) {
+    // ------------------------------ K and V producers ------------------------------
+    const bool is_k = warp == K_WARP;
+    uint64_t* full = is_k ? k_full : v_full;
+    uint64_t* empty = is_k ? k_empty : v_empty;
+    uint8_t* ring = smem + (is_k ? L::OFF_K : L::OFF_V);
+    const CUtensorMap* map = is_k ? &tmK : &tmV;
     const int box = 1 << p.box_log2;
-    const int pages = BN >> p.box_log2;              // boxes of a tile
-    const int split = p.page_log2 - p.box_log2;      // log2 of boxes in a block
+    const int pages = BN >> p.box_log2;          // boxes of a tile: lane i loads box i
+    const int split = p.page_log2 - p.box_log2;  // log2 of boxes in a block
     const int group_box = box / 8;
-    // the index of the page's first (token, head) row, for this lane's page of tile i
-    auto page_of = [&](const Walk& s, int i) -> int {
-      const int box_index = i * pages + lane;
-      if (lane >= pages || (static_cast<long long>(box_index) << p.box_log2) >= s.len()) return 0;
-      const int id = p.tables[s.b * p.table_stride + (box_index >> split)];
-      if (id < 0 || id >= p.num_blocks) {
-        record_status(p.status, KTA_ERR_DEVICE_BOUNDS, SITE_BLOCK);
-        return p.num_blocks * p.hkv << p.page_log2;  // past the tensor: reads as zeros
-      }
-      return (id * p.hkv << p.page_log2) + s.kvh;
+    uint32_t n = 0;  // tiles so far
+    bool ok = true;
+    // this lane's block of tile i; only used a tile or two later, so that it stays in flight
+    auto block_of = [&](int i) -> int {
+      const int at = i * pages + lane;
+      if (lane >= pages || at << p.box_log2 >= w.len()) return 0;
+      return p.tables[w.b * p.table_stride + (at >> split)];
     };
-    auto load = [&](const Walk& s, int i, int first, const CUtensorMap* map) -> bool {
-      const int st = static_cast<int>(n % RING);
-      if (!mbar_wait(&ring_empty[st], ((n / RING) & 1u) ^ 1u, abort_flag, p.status, SITE_PROD_SLOT)) {
-        return false;
-      }
-      ++n;
-      const int held = min(pages, (s.len() - i * BN + box - 1) >> p.box_log2);
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&ring_full[st], static_cast<uint32_t>(held * group_box * L::GROUP));
-      }
-      __syncwarp();
-      if (lane < held) {
-        const int g = ((i * pages + lane) & ((1 << split) - 1)) * group_box;
-        tma_load_5d(map, &ring_full[st], smem + L::OFF_RING + st * L::TILE + lane * group_box * L::GROUP,
-                    0, 0, 0, g, first);
-      }
-      __syncwarp();
-      return true;
-    };
-    for (; w.left > 0 && ok; w.next(p)) {
-      const int rt = w.row_tile(p, member);
-      const int tokens = w.rows(p, rt);
-      if (tokens == 0) continue;
-      int cur = page_of(w, w.i0);
-      const int end = w.i0 + w.count();
-      int nxt = w.i0 + 1 < end ? page_of(w, w.i0 + 1) : 0;
-      if (!load(w, w.i0, cur, &tmK)) break;
-      if (!mbar_wait(q_empty, qphase ^ 1u, abort_flag, p.status, SITE_PROD_Q)) break;
-      qphase ^= 1u;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(p.box_tokens * p.group * D * 2));
-#pragma unroll
-        for (int h = 0; h < L::HALVES; ++h) {
-          tma_load_3d(&tmQ, q_full, smem + L::OFF_Q + h * L::Q_HALF, h * 64, w.kvh * p.group,
-                      w.row + rt * p.tok_tile);
-        }
-      }
-      __syncwarp();
-      for (int i = w.i0; i < end; ++i) {
-        const int after = i + 2 < end ? page_of(w, i + 2) : 0;  // in flight during the waits
-        if (i + 1 < end && !load(w, i + 1, nxt, &tmK)) {
+    for (; w.left > 0 && ok; w.next(p), w.settle(p, member)) {
+      const int end = w.i0 + w.count(p);
+      int id = block_of(w.i0), id1 = w.i0 + 1 < end ? block_of(w.i0 + 1) : 0;
+      for (int i = w.i0; i < end; ++i, ++n) {
+        const int id2 = i + 2 < end ? block_of(i + 2) : 0;
+        const int st = static_cast<int>(n % RING);
+        if (!mbar_wait(&empty[st], ((n / RING) & 1u) ^ 1u, abort_flag, p.status, SITE_PROD_KV)) {
           ok = false;
           break;
         }
-        if (!load(w, i, cur, &tmV)) {
-          ok = false;
-          break;
+        const int held = min(pages, (w.len() - i * BN + box - 1) >> p.box_log2);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(held * group_box * L::GROUP));
         }
-        cur = nxt;
-        nxt = after;
+        __syncwarp();
+        if (lane < held) {
+          // the block's first (token, head) row; past the tensor, which reads as zeros, for no block
+          int first = p.num_blocks * p.hkv << p.page_log2;
+          if (id >= 0 && id < p.num_blocks) {
+            first = (id * p.hkv << p.page_log2) + w.kvh;
+          } else {
+            record_status(p.status, KTA_ERR_DEVICE_BOUNDS, SITE_BLOCK);
+          }
+          tma_load_5d(map, &full[st], ring + st * L::TILE + lane * group_box * L::GROUP, 0, 0, 0,
+                      ((i * pages + lane) & ((1 << split) - 1)) * group_box, first);
+        }
+        __syncwarp();
+        id = id1;
+        id1 = id2;
       }
     }
     if (*abort_flag != 0 && lane == 0) {
       // a role gave up: no copy may be in flight when the block ends (bounded like every wait)
       int none = 0;
       for (uint32_t k = n > RING ? n - RING : 0; k < n; ++k) {
-        mbar_wait(&ring_full[k % RING], (k / RING) & 1u, &none, p.status, SITE_PROD_SLOT);
+        mbar_wait(&full[k % RING], (k / RING) & 1u, &none, p.status, SITE_PROD_KV);
       }
-      if (qphase != 0 || n > 0) mbar_wait(q_full, qphase ^ 1u, &none, p.status, SITE_PROD_Q);
     }
+  } else if (warp == Q_WARP) {
+    // ------------------------------ Q producer ------------------------------
+    if (lane == 0) {
+      uint32_t n = 0;  // segments so far: buffer n % q_bufs
+      for (; w.left > 0; w.next(p), w.settle(p, member), ++n) {
+        const uint32_t buf = n % p.q_bufs, phase = (n / p.q_bufs) & 1u;
+        if (!mbar_wait(&q_empty[buf], phase ^ 1u, abort_flag, p.status, SITE_PROD_Q)) break;
+        mbar_arrive_expect_tx(&q_full[buf], static_cast<uint32_t>(p.box_tokens * p.group * D * 2));
+#pragma unroll
+        for (int h = 0; h < L::HALVES; ++h) {
+          tma_load_3d(&tmQ, &q_full[buf], smem + L::OFF_Q + h * L::Q_HALF + buf * p.q_shift, h * 64,
+                      w.kvh * p.group, w.row + w.row_tile(p, member) * p.tok_tile);
+        }
+      }
+      if (*abort_flag != 0) {
+        int none = 0;
+        for (uint32_t k = n > static_cast<uint32_t>(p.q_bufs) ? n - p.q_bufs : 0; k < n; ++k) {
+          mbar_wait(&q_full[k % p.q_bufs], (k / p.q_bufs) & 1u, &none, p.status, SITE_PROD_Q);
+        }
+      }
+    }
+    __syncwarp();
   } else if (warp == MMA_WARP) {
     // ------------------------------ MMA issuer ------------------------------
     constexpr uint32_t FMT = BF16 ? 1u : 0u;
     constexpr uint32_t idesc_s = make_idesc(BM, BN, FMT, FMT, 0u, 0u);  // Q K^T, both K-major
     constexpr uint32_t idesc_o = make_idesc(BM, D, FMT, FMT, 0u, 1u);   // P (TMEM) V (MN-major)
-    const uint64_t qdesc = sdesc_sw128(smem_u32(smem + L::OFF_Q), 16, 1024);
-    uint32_t n = 0;     // tiles taken from the ring
-    uint32_t g = 0;     // tiles of keys so far: buffer g & 1, its phase (g >> 1) & 1
-    uint32_t q_phase = 0, o_phase = 0;
-    bool first_segment = true, ok = true;
-    auto take = [&](int* st) -> bool {
-      *st = static_cast<int>(n % RING);
-      const uint32_t ph = (n / RING) & 1u;
-      ++n;
-      return mbar_wait(&ring_full[*st], ph, abort_flag, p.status, SITE_MMA_KV);
-    };
+    // w and j run one tile ahead of the PVs, into the next segment: its first S is ready when the
+    // softmax warps come from this one's epilogue.
+    int j = 0, tiles = w.left > 0 ? w.count(p) : 0;
+    uint32_t segment = 0, o_phase = 0;
+    bool first_segment = true;
     // S of tile t into buffer t & 1, which holds P of tile t - 2 until its PV has read it: that was
     // issued before and ends before this begins.
-    auto issue_s = [&](uint32_t t, bool last) -> bool {
-      int st;
-      if (!take(&st)) return false;
+    auto issue_s = [&](uint32_t t) -> bool {
+      const uint32_t buf = segment % p.q_bufs;
+      if (j == 0 && !mbar_wait(&q_full[buf], (segment / p.q_bufs) & 1u, abort_flag, p.status, SITE_MMA_Q)) {
+        return false;
+      }
+      const int st = static_cast<int>(t % RING);
+      if (!mbar_wait(&k_full[st], (t / RING) & 1u, abort_flag, p.status, SITE_MMA_K)) return false;
       tc_fence_after();
-      const uint64_t kdesc = sdesc_sw128(smem_u32(smem + L::OFF_RING + st * L::TILE), 16, L::GROUP);
+      const uint64_t qdesc = sdesc_sw128(smem_u32(smem + L::OFF_Q + buf * p.q_shift), 16, 1024);
+      const uint64_t kdesc = sdesc_sw128(smem_u32(smem + L::OFF_K + st * L::TILE), 16, L::GROUP);
       if (elect_one_sync()) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -582,48 +622,55 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           umma_f16(tmem + (t & 1u) * BN, qdesc + qo, kdesc + ko, idesc_s, kk > 0 ? 1u : 0u);
         }
         umma_commit(&s_full[t & 1u]);
-        umma_commit(&ring_empty[st]);
-        if (last) umma_commit(q_empty);
+        umma_commit(&k_empty[st]);
+        if (j + 1 == tiles) umma_commit(&q_empty[buf]);
       }
       __syncwarp();
       return true;
     };
-    for (; w.left > 0 && ok; w.next(p)) {
-      if (w.rows(p, w.row_tile(p, member)) == 0) continue;
-      if (!mbar_wait(q_full, q_phase, abort_flag, p.status, SITE_MMA_Q)) break;
-      q_phase ^= 1u;
-      const int tiles = w.count();
-      if (!issue_s(g, tiles == 1)) break;
-      for (int j = 0; j < tiles && ok; ++j, ++g) {
-        int st;
-        ok = (j + 1 == tiles || issue_s(g + 1, j + 2 == tiles)) && take(&st);
-        if (!ok) break;
-        const uint64_t vdesc = sdesc_sw128(smem_u32(smem + L::OFF_RING + st * L::TILE), 1024, L::GROUP);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {  // the warpgroups' halves of the keys, into their own O
-          ok = mbar_wait(&p_full[2 * (g & 1u) + h], (g >> 1) & 1u, abort_flag, p.status, SITE_MMA_P);
-          if (!ok) break;
-          if (j == 0 && h == 0 && !first_segment) {  // the last segment's O has been read
-            ok = mbar_wait(o_free, o_phase, abort_flag, p.status, SITE_MMA_OFREE);
-            if (!ok) break;
-            o_phase ^= 1u;
-          }
-          tc_fence_after();
-          if (elect_one_sync()) {
-#pragma unroll
-            for (int kk = 0; kk < HK / 16; ++kk) {
-              umma_f16_tmem_a(tmem + COL_O + h * BN, tmem + (g & 1u) * BN + h * HK + kk * 8,
-                              vdesc + static_cast<uint64_t>((h * HK / 16 + kk) * 2 * L::GROUP / 16),
-                              idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
-            }
-            umma_commit(&pv_done[h]);
-            if (h == 1) umma_commit(&ring_empty[st]);
-            if (h == 1 && j + 1 == tiles) umma_commit(o_done);
-          }
-          __syncwarp();
-        }
+    bool more = w.left > 0;
+    if (more && !issue_s(0)) more = false;
+    for (uint32_t g = 0; more; ++g) {  // tile g: S buffer g & 1, its phase (g >> 1) & 1
+      const bool first = j == 0, last = j + 1 == tiles;
+      if (last) {
+        w.next(p);
+        w.settle(p, member);
+        j = 0;
+        tiles = w.left > 0 ? w.count(p) : 0;
+        ++segment;
+      } else {
+        ++j;
       }
-      first_segment = false;
+      more = w.left > 0;
+      if (more && !issue_s(g + 1)) break;
+      const int st = static_cast<int>(g % RING);
+      if (!mbar_wait(&v_full[st], (g / RING) & 1u, abort_flag, p.status, SITE_MMA_V)) break;
+      const uint64_t vdesc = sdesc_sw128(smem_u32(smem + L::OFF_V + st * L::TILE), 1024, L::GROUP);
+      bool ok = true;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // the warpgroups' halves of the keys, into their own O
+        ok = ok && mbar_wait(&p_full[2 * (g & 1u) + h], (g >> 1) & 1u, abort_flag, p.status, SITE_MMA_P);
+        if (first && h == 0 && !first_segment) {  // the last segment's O has been read
+          ok = ok && mbar_wait(o_free, o_phase, abort_flag, p.status, SITE_MMA_OFREE);
+          o_phase ^= 1u;
+        }
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one_sync()) {
+#pragma unroll
+          for (int kk = 0; kk < HK / 16; ++kk) {
+            umma_f16_tmem_a(tmem + COL_O + h * BN, tmem + (g & 1u) * BN + h * HK + kk * 8,
+                            vdesc + static_cast<uint64_t>((h * HK / 16 + kk) * 2 * L::GROUP / 16),
+                            idesc_o, (!first || kk > 0) ? 1u : 0u);
+          }
+          umma_commit(&pv_done[h]);
+          if (h == 1) umma_commit(&v_empty[st]);
+          if (h == 1 && last) umma_commit(o_done);
+        }
+        __syncwarp();
+      }
+      if (!ok) break;
+      if (last) first_segment = false;
     }
   } else {
     // ------------- softmax, O correction and epilogue (thread = query row) -------------
@@ -633,41 +680,35 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const uint32_t t_s = tmem + lane_base + wg * HK;  // this half of S buffer 0
     const uint32_t t_o = tmem + lane_base + COL_O;    // O of warpgroup 0; the other's is BN columns on
     const float sl = p.scale_log2;
-    uint32_t n = 0;  // loads into the ring of the segments so far
     uint32_t g = 0;  // tiles of keys so far
     uint32_t o_phase = 0;
     bool ok = true;
     if (threadIdx.x == 0) p.desc[blockIdx.x] = Desc{};  // no unit to join so far
-    for (bool first = true; w.left > 0 && ok; w.next(p)) {
+    for (bool first_part = true; w.left > 0 && ok; w.next(p), w.settle(p, member), first_part = false) {
       const int rt = w.row_tile(p, member);
       const int tokens = w.rows(p, rt);
-      const bool first_part = first;
-      first = false;
-      if (tokens == 0) continue;
       const int rows = tokens * p.group;
       const bool live = row < rows;
       const bool warp_on = quarter * 32 < rows;
       uint64_t bits = 0;
       if (live) {
         const int t = rt * p.tok_tile + row / p.group;
-        bits = p.tree != nullptr ? static_cast<uint64_t>(__ldg(p.tree + w.row + t))
+        bits = p.tree != nullptr ? static_cast<uint64_t>(p.tree[w.row + t])
                                  : (2ull << t) - 1ull;  // t = 63: all ones
         if (w.tokens < 64) bits &= (1ull << w.tokens) - 1ull;
       }
-      const int tiles = w.count();
+      const int tiles = w.count(p);
       float m_used = -INFINITY, lsum = 0.f;
       for (int j = 0; j < tiles; ++j, ++g) {
         const int k0 = (w.i0 + j) * BN;
         const bool masked = k0 + BN > w.ctx;
         if (masked) {
-          // V(j) is the load 2 j + 2 of the segment, or 2 j + 1 for its last tile
-          const uint32_t vn = n + 2 * j + (j + 1 < tiles ? 2 : 1);
-          const int st = static_cast<int>(vn % RING);
-          if (!mbar_wait(&ring_full[st], (vn / RING) & 1u, abort_flag, p.status, SITE_SM_V)) {
+          const int st = static_cast<int>(g % RING);
+          if (!mbar_wait(&v_full[st], (g / RING) & 1u, abort_flag, p.status, SITE_SM_V)) {
             ok = false;
             break;
           }
-          clean_v<BF16, D>(smem + L::OFF_RING + st * L::TILE, wg * HK, w.ctx - k0, w.len() - k0, k0 - w.ctx,
+          clean_v<BF16, D>(smem + L::OFF_V + st * L::TILE, wg * HK, w.ctx - k0, w.len() - k0, k0 - w.ctx,
                            row, bad);
           fence_proxy_async_smem();
         }
@@ -694,7 +735,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * (g & 1u) + wg]);
       }
-      n += 2 * tiles;
       if (!ok) break;
       // ---- epilogue: the two warpgroups' states become one, each for half of D ----
       ml[wg * BM + row] = make_float2(m_used, lsum);
@@ -780,12 +820,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
       }
       if (threadIdx.x == 0 && !whole && w.i0 == 0) {  // the unit starts here: this CTA describes it
-        Ranges r;
-        r.total = *all_tiles;
-        r.n = static_cast<int>(min(static_cast<long long>(gridDim.x / p.row_tiles), r.total));
-        const long long last = r.start(range + 1) - w.left + w.tiles() - 1;
+        const Ranges r(p, plan[5]);
+        const int end = plan[4] - w.left + w.tiles() * row_tiles_of(p, w.tokens);  // of the unit
         Desc d = {};
-        d.count = r.owner(last) - range + 1;
+        d.count = r.owner_before(end) - range + 1;
         d.slot = slot;
         d.next = (range + 1) * p.row_tiles + rt;  // a range's first segment is row tile = member
         d.row = w.row + rt * p.tok_tile;
@@ -945,6 +983,11 @@ int launch(const void* Q, const void* Kc, const void* Vc, const void* tables, co
       num_blocks > ((1LL << 31) - 1) / (block * Hkv)) {
     return KTA_ERR_UNSUPPORTED;
   }
+  // and so does the work list: every request's tiles of keys, for each KV head and row tile
+  const long long row_tiles = (max_new + BM / (Hq / Hkv) - 1) / (BM / (Hq / Hkv));
+  if (B * Hkv * row_tiles * ((max_blocks * block + BN - 1) / BN) > (1LL << 31) - 1) {
+    return KTA_ERR_UNSUPPORTED;
+  }
   if (q_token < Hq * D) return KTA_ERR_INVALID_ARG;
   if (q_token % 8 != 0 || !aligned16(Q) || !aligned16(Kc) || !aligned16(Vc) || !aligned16(O)) {
     return KTA_ERR_ALIGN;
@@ -983,7 +1026,11 @@ int launch(const void* Q, const void* Kc, const void* Vc, const void* tables, co
   p.box_log2 = std::min(p.page_log2, 7);
   p.tok_tile = BM / p.group;
   p.box_tokens = std::min(p.tok_tile, p.max_new);
-  p.row_tiles = (p.max_new + p.tok_tile - 1) / p.tok_tile;
+  p.row_tiles = static_cast<int>(row_tiles);
+  // two Q tiles where they fit (64 rows): the next segment's Q then comes while this one runs
+  const int q_rows = (p.box_tokens * p.group + 7) / 8 * 8;
+  p.q_bufs = q_rows <= BM / 2 ? 2 : 1;
+  p.q_shift = BM / 2 * 128;
   p.row_cap = ws.row_cap;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = device_status_ptr();
