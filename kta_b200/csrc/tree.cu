@@ -34,46 +34,15 @@
 #include <algorithm>
 #include <cmath>
 
-#include "kta_common.cuh"
-#include "kta_host.h"
+#include "tree_common.cuh"
 
 namespace kta {
 namespace tree {
 
-constexpr int BM = 128;               // query rows of a row tile: TMEM lanes
-constexpr int BN = 128;               // keys of a tile
 constexpr int RING = 3;               // K tiles in flight, and V tiles
 constexpr int HK = BN / 2;            // keys of a tile that a softmax warpgroup takes
 constexpr int SOFTMAX_WARPS = 8;      // two warpgroups
-constexpr int MMA_WARP = 8;
-constexpr int K_WARP = 9;             // TMA producers
-constexpr int V_WARP = 10;
-constexpr int Q_WARP = 11;
-constexpr int NUM_THREADS = 384;
-constexpr int MAX_DRAFT = 64;         // bits of a row of the tree
-constexpr int MAX_GROUP = 16;
-constexpr int MAX_BATCH = 1 << 16;
-constexpr int MAX_CTAS = 256;         // the workspace is sized for this many
-constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units: the maximum moves when it grew > 2^8
 constexpr uint32_t COL_O = 256;       // TMEM: S buffer i at i * 128, O of warpgroup w at 256 + w * 128
-
-enum : unsigned int {
-  SITE_PROD_KV = 0x901,
-  SITE_PROD_Q = 0x902,
-  SITE_MMA_Q = 0x903,
-  SITE_MMA_K = 0x904,
-  SITE_MMA_V = 0x90C,
-  SITE_MMA_P = 0x905,
-  SITE_MMA_OFREE = 0x906,
-  SITE_SM_S = 0x907,
-  SITE_SM_V = 0x908,
-  SITE_SM_ML = 0x909,
-  SITE_SM_O = 0x90A,
-  SITE_SM_PV = 0x90B,
-  SITE_SMEM = 0x910,     // shared memory not aligned as declared
-  SITE_REQUEST = 0x911,  // lengths or offsets out of range
-  SITE_BLOCK = 0x912,    // a block id out of range
-};
 
 template <int D>
 struct Layout {
@@ -86,160 +55,14 @@ struct Layout {
   static constexpr int OFF_V = OFF_K + RING * TILE;
   static constexpr int OFF_ML = OFF_V + RING * TILE;  // [warpgroup][128 rows] (maximum, sum)
   static constexpr int OFF_BAR = OFF_ML + 2 * BM * 8;
-  // k_full[R], k_empty[R], v_full[R], v_empty[R], q_full[2], q_empty[2], s_full[2], p_full[2][2],
+  // k_full[R], k_empty[R], v_full[R], v_empty[R], q_full, q_empty, s_full[2], p_full[2][2],
   // pv_done[2], ml_full, o_done, o_free
-  static constexpr int NUM_BARS = 4 * RING + 15;
+  static constexpr int NUM_BARS = 4 * RING + 13;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
   // misc: tmem base, abort, non-finite drafts, the range's first segment and end
   static constexpr int TOTAL = OFF_MISC + 64;
   static_assert(TOTAL <= 232448, "shared memory budget of one sm_100 CTA");
 };
-
-// What the join kernel needs of a unit that starts in a CTA's range and ends in a later one.
-struct Desc {
-  int count;    // ranges that hold a part of it; 0: none
-  int slot;     // the first part's slot
-  int next;     // CTA of the second part; the others follow row_tiles apart, each in slot 0
-  int row;      // first query token
-  int tokens;
-  int kvh;
-  int pad[2];
-};
-
-struct Params {
-  const int32_t* ctx;      // [B]
-  const int32_t* offsets;  // [B + 1]
-  const int64_t* tree;     // [rows] or nullptr: a chain
-  const int32_t* tables;   // [B, max_blocks]
-  void* out;               // [rows, Hq, D]
-  float* lse;              // [rows, Hq]
-  const void* v;           // the V cache, for drafted rows that are not finite
-  Desc* desc;              // [CTAs]
-  float2* part_ml;         // [2 CTAs][row_cap] (maximum, sum), log2 units
-  float4* part_o;          // [2 CTAs][D / 4][row_cap], not normalised
-  long long table_stride;
-  int batch, rows, hq, hkv, group, max_new, max_blocks, num_blocks;
-  int page_log2;           // tokens of a block
-  int box_log2;            // tokens of a TMA box: min(block, 128)
-  int tok_tile;            // drafted tokens of a row tile: 128 / group
-  int box_tokens;          // tokens of the Q box: min(tok_tile, max_new)
-  int row_tiles;           // CTAs that share a range
-  int q_bufs, q_shift;     // Q tiles in shared memory, bytes from one to the next
-  int row_cap;             // rows of a partial
-  float scale_log2;        // softmax scale * log2(e)
-  unsigned int* status;
-};
-
-__device__ __forceinline__ void tma_load_5d(const CUtensorMap* map, uint64_t* bar, void* dst, int32_t x,
-                                            int32_t y, int32_t z, int32_t w, int32_t v) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
-      : "memory");
-}
-
-struct Request {
-  int row, tokens, ctx, len;  // first row, drafted tokens, cached tokens, both
-  bool bad;
-};
-
-__device__ __forceinline__ Request request_of(const Params& p, int b) {
-  const int a = p.offsets[b], z = p.offsets[b + 1], c = p.ctx[b];
-  Request r;
-  const long long room = static_cast<long long>(p.max_blocks) << p.page_log2;
-  const long long t = static_cast<long long>(z) - a;
-  r.bad = a < 0 || t < 0 || z > p.rows || t > p.max_new || c < 0 || c + t > room;
-  r.row = a;
-  r.tokens = r.bad ? 0 : static_cast<int>(t);
-  r.ctx = c;
-  r.len = r.bad ? 0 : c + r.tokens;
-  return r;
-}
-
-// Tiles of keys of a request: none without a query row.
-__device__ __forceinline__ int tiles_of(const Request& r) {
-  return r.tokens > 0 ? (r.len + BN - 1) / BN : 0;
-}
-
-// Row tiles of a request.
-__device__ __forceinline__ int row_tiles_of(const Params& p, int tokens) {
-  return (tokens + p.tok_tile - 1) / p.tok_tile;
-}
-
-// The work list: tile i of KV head h of request b, b-major, each counted once for every row tile
-// of its request (the CTAs of a range share those). Range k of n is [total k / n, total (k + 1) / n)
-// rounded down to whole tiles; n <= total / row_tiles, so that none is empty.
-struct Ranges {
-  int total, n;
-  __device__ __forceinline__ Ranges(const Params& p, int total_) : total(total_) {
-    n = total == 0 ? 0 : max(1, min(static_cast<int>(gridDim.x) / p.row_tiles, total / p.row_tiles));
-  }
-  __device__ __forceinline__ int start(int k) const {
-    return static_cast<int>(static_cast<long long>(total) * k / n);
-  }
-  // the range of the last tile before position `end`, the end of a unit
-  __device__ __forceinline__ int owner_before(int end) const {
-    return static_cast<int>((static_cast<long long>(end) * n - 1) / total);
-  }
-};
-
-// A range's walk over its segments: runs of count() tiles from i0 on of one (request, KV head).
-// Few fields, since the softmax warps keep it beside a row of S.
-struct Walk {
-  int row, tokens, ctx;  // of the request
-  int b, kvh, i0;
-  int left;              // of the range from here on, in the work list's count
-  int turn;              // the CTA of the range's that takes the segment's first row tile
-
-  __device__ __forceinline__ void set(const Request& r) {
-    row = r.row;
-    tokens = r.tokens;
-    ctx = r.ctx;
-  }
-  __device__ __forceinline__ int len() const { return ctx + tokens; }
-  __device__ __forceinline__ int tiles() const { return (len() + BN - 1) / BN; }
-  __device__ __forceinline__ int count(const Params& p) const {
-    return min(tiles() - i0, left / row_tiles_of(p, tokens));
-  }
-  __device__ __forceinline__ void next(const Params& p) {
-    const int k = row_tiles_of(p, tokens);
-    left -= count(p) * k;
-    if (left <= 0) return;
-    turn = (turn + k) % p.row_tiles;
-    i0 = 0;
-    if (++kvh == p.hkv) {
-      kvh = 0;
-      Request r;
-      do {  // tiles are left in the range, so a request with some follows
-        r = request_of(p, ++b);
-      } while (tiles_of(r) == 0);
-      set(r);
-    }
-  }
-  // The row tile of the request that falls to CTA `member` of the range's. Requests have between
-  // one and row_tiles of them: the CTAs take turns, so that each has its share over some segments.
-  __device__ __forceinline__ int row_tile(const Params& p, int member) const {
-    const int k = member - turn;
-    return k < 0 ? k + p.row_tiles : k;
-  }
-  // Drafted tokens of row tile rt in the request: 0 where it has fewer.
-  __device__ __forceinline__ int rows(const Params& p, int rt) const {
-    return max(0, min(tokens - rt * p.tok_tile, p.tok_tile));
-  }
-  // To the next segment, this one included, in which CTA `member` has rows.
-  __device__ __forceinline__ void settle(const Params& p, int member) {
-    while (left > 0 && rows(p, row_tile(p, member)) == 0) next(p);
-  }
-};
-
-// Bits lo .. lo + 31 of a row's view of the keys, lo = first key of the word less ctx: cached
-// keys (negative) are all seen, drafted ones by the row's bits.
-__device__ __forceinline__ uint32_t view_word(uint64_t bits, int lo) {
-  if (lo <= -32) return 0xffffffffu;
-  if (lo < 0) return (0xffffffffu >> (32 + lo)) | static_cast<uint32_t>(bits << -lo);
-  return lo < 64 ? static_cast<uint32_t>(bits >> lo) : 0u;
-}
 
 // Half an S tile of one query row (64 keys; this thread's TMEM lane): P = 2^(S sl - m) over the
 // first 32 columns, the running maximum m (log2 units) and the row sum l of this half. m moves only
@@ -318,51 +141,9 @@ __device__ __forceinline__ bool softmax_step(uint32_t t_s, uint32_t t_o, const u
   return true;
 }
 
-// 16-bit elements of a word whose exponent is all ones (infinities and NaN), as a mask of them.
-template <bool BF16>
-__device__ __forceinline__ uint32_t nonfinite(uint32_t w) {
-  constexpr uint32_t E = BF16 ? 0x7F80u : 0x7C00u;
-  return ((w & E) == E ? 0xffffu : 0u) | ((w >> 16 & E) == E ? 0xffff0000u : 0u);
-}
-
-// Rows [from, from + 64) of a V tile (shared memory) of which [first, valid) are drafted tokens:
-// rows past `valid` become zero, and so do drafted elements that are not finite, whose tokens are
-// recorded in bad[0..1] (token = row + token0). By the 128 threads of a warpgroup.
-template <bool BF16, int D>
-__device__ __forceinline__ void clean_v(uint8_t* tile, int from, int first, int valid, int token0, int tid,
-                                        unsigned int* bad) {
-  constexpr int CHUNKS = D / 8;  // 16-byte pieces of a row
-  for (int i = tid + max(first, from) * CHUNKS; i < (from + HK) * CHUNKS; i += BM) {
-    const int row = i / CHUNKS, ch = i % CHUNKS;
-    uint4* at = reinterpret_cast<uint4*>(tile + (row >> 3) * Layout<D>::GROUP + (ch >> 3) * 1024 +
-                                         (row & 7) * 128 + (ch & 7) * 16);
-    if (row >= valid) {
-      *at = make_uint4(0u, 0u, 0u, 0u);
-      continue;
-    }
-    const uint4 u = *at;
-    const uint4 n = make_uint4(nonfinite<BF16>(u.x), nonfinite<BF16>(u.y), nonfinite<BF16>(u.z),
-                               nonfinite<BF16>(u.w));
-    if ((n.x | n.y | n.z | n.w) != 0u) {
-      *at = make_uint4(u.x & ~n.x, u.y & ~n.y, u.z & ~n.z, u.w & ~n.w);
-      const int token = row + token0;
-      atomicOr(bad + (token >> 5), 1u << (token & 31));
-    }
-  }
-}
-
-template <bool BF16>
-__device__ __forceinline__ float load16(const void* base, long long i) {
-  if constexpr (BF16) {
-    return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i]);
-  } else {
-    return __half2float(static_cast<const __half*>(base)[i]);
-  }
-}
-
 template <bool BF16, int D>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
-    tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+    wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const Params p) {
   using L = Layout<D>;
   // Asked for at 1024 bytes (the 128-byte swizzle's period): there is no room to round up in.
@@ -379,9 +160,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   uint64_t* k_empty = k_full + RING;
   uint64_t* v_full = k_empty + RING;
   uint64_t* v_empty = v_full + RING;
-  uint64_t* q_full = v_empty + RING;  // [Q buffer]
-  uint64_t* q_empty = q_full + 2;     // [Q buffer]: the segment's last S has read Q
-  uint64_t* s_full = q_empty + 2;    // [S buffer]
+  uint64_t* q_full = v_empty + RING;
+  uint64_t* q_empty = q_full + 1;    // the segment's last S has read Q
+  uint64_t* s_full = q_empty + 1;    // [S buffer]
   uint64_t* p_full = s_full + 2;     // [buffer][warpgroup]: its half of P written, of V cleaned
   uint64_t* pv_done = p_full + 4;    // [warpgroup]: one phase for each PV into its O
   uint64_t* ml_full = pv_done + 2;   // both warpgroups' maxima and sums are in shared memory
@@ -394,7 +175,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   // and the list's total
   volatile int* plan = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 16);  // [6]
   float2* ml = reinterpret_cast<float2*>(smem + L::OFF_ML);
-  int* warp_sum = reinterpret_cast<int*>(smem + L::OFF_K);  // before the ring is used
+  int* warp_sum = reinterpret_cast<int*>(smem + L::OFF_ML);  // before the first segment ends
 
   const int warp = warp_id();
   const int lane = threadIdx.x & 31;
@@ -406,13 +187,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       mbar_init(&v_empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[2 * i], SOFTMAX_WARPS / 2);
       mbar_init(&p_full[2 * i + 1], SOFTMAX_WARPS / 2);
       mbar_init(&pv_done[i], 1);
     }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     mbar_init(ml_full, SOFTMAX_WARPS);
     mbar_init(o_done, 1);
     mbar_init(o_free, SOFTMAX_WARPS);
@@ -433,165 +214,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   // after the wait: the join kernel may be scheduled now, and waits for this grid itself
   pdl_launch_dependents();
 
-  // ---- the work list: thread i sums a run of requests ----
-  const int per = (p.batch + NUM_THREADS - 1) / NUM_THREADS;
-  const int b0 = min(static_cast<int>(threadIdx.x) * per, p.batch), b1 = min(b0 + per, p.batch);
-  auto work_of = [&](const Request& r) { return tiles_of(r) * p.hkv * row_tiles_of(p, r.tokens); };
-  int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += work_of(request_of(p, b));
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) warp_sum[warp] = incl;
+  const int member = blockIdx.x % p.row_tiles;
   tc_fence_before();
-  __syncthreads();
+  Walk w = plan_range<D>(p, member, plan, warp_sum);
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
-  int before = incl - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < NUM_THREADS / 32; ++w) {
-    if (w < warp) before += warp_sum[w];
-    total += warp_sum[w];
-  }
-  const Ranges rg(p, total);
-  const int range = blockIdx.x / p.row_tiles, member = blockIdx.x % p.row_tiles;
-  const bool busy = range < rg.n;
-  if (busy) {
-    // the range's two ends, by the threads whose requests they fall into
-    const int from = rg.start(range), to = rg.start(range + 1);
-    for (int e = 0; e < 2; ++e) {
-      const int at = e == 0 ? from : to;
-      if (at < before || at >= before + mine) continue;
-      int t = before;
-      for (int b = b0; b < b1; ++b) {
-        const Request r = request_of(p, b);
-        const int n = work_of(r);
-        if (at >= t + n) {
-          t += n;
-          continue;
-        }
-        const int k = row_tiles_of(p, r.tokens), pair = tiles_of(r) * k;
-        const int kvh = (at - t) / pair, off = at - t - kvh * pair;
-        if (e == 0) {
-          plan[0] = b;
-          plan[1] = kvh;
-          plan[2] = off / k;
-        }
-        plan[3 + e] = at - off % k;
-        break;
-      }
-    }
-    if (threadIdx.x == 0) {
-      if (to == total) plan[4] = total;
-      plan[5] = total;
-    }
-  }
-  // requests that are out of range: their rows that exist become zero
-  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-    if (!request_of(p, b).bad) continue;
-    if (threadIdx.x == 0) record_status(p.status, KTA_ERR_DEVICE_BOUNDS, SITE_REQUEST);
-    const long long a = max(p.offsets[b], 0), z = min(p.offsets[b + 1], p.rows);
-    const long long words = (z - a) * p.hq * (D / 2);
-    uint32_t* o = static_cast<uint32_t*>(p.out) + a * p.hq * (D / 2);
-    for (long long i = threadIdx.x; i < words; i += NUM_THREADS) o[i] = 0u;
-    for (long long i = threadIdx.x; i < (z - a) * p.hq; i += NUM_THREADS) p.lse[a * p.hq + i] = -INFINITY;
-  }
-  fence_proxy_async_smem();  // the scan's use of the ring's memory comes before its TMA writes
-  __syncthreads();
-  Walk w;
-  w.left = 0;
-  if (busy) {
-    w.b = plan[0];
-    w.kvh = plan[1];
-    w.i0 = plan[2];
-    w.left = plan[4] - plan[3];
-    w.turn = 0;
-    w.set(request_of(p, w.b));
-    w.settle(p, member);
-  }
 
-  if (warp == K_WARP || warp == V_WARP) {
-    // ------------------------------ K and V producers ------------------------------
-    const bool is_k = warp == K_WARP;
-    uint64_t* full = is_k ? k_full : v_full;
-    uint64_t* empty = is_k ? k_empty : v_empty;
-    uint8_t* ring = smem + (is_k ? L::OFF_K : L::OFF_V);
-    const CUtensorMap* map = is_k ? &tmK : &tmV;
-    const int box = 1 << p.box_log2;
-    const int pages = BN >> p.box_log2;          // boxes of a tile: lane i loads box i
-    const int split = p.page_log2 - p.box_log2;  // log2 of boxes in a block
-    const int group_box = box / 8;
-    uint32_t n = 0;  // tiles so far
-    bool ok = true;
-    // this lane's block of tile i; only used a tile or two later, so that it stays in flight
-    auto block_of = [&](int i) -> int {
-      const int at = i * pages + lane;
-      if (lane >= pages || at << p.box_log2 >= w.len()) return 0;
-      return p.tables[w.b * p.table_stride + (at >> split)];
-    };
-    for (; w.left > 0 && ok; w.next(p), w.settle(p, member)) {
-      const int end = w.i0 + w.count(p);
-      int id = block_of(w.i0), id1 = w.i0 + 1 < end ? block_of(w.i0 + 1) : 0;
-      for (int i = w.i0; i < end; ++i, ++n) {
-        const int id2 = i + 2 < end ? block_of(i + 2) : 0;
-        const int st = static_cast<int>(n % RING);
-        if (!mbar_wait(&empty[st], ((n / RING) & 1u) ^ 1u, abort_flag, p.status, SITE_PROD_KV)) {
-          ok = false;
-          break;
-        }
-        const int held = min(pages, (w.len() - i * BN + box - 1) >> p.box_log2);
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(held * group_box * L::GROUP));
-        }
-        __syncwarp();
-        if (lane < held) {
-          // the block's first (token, head) row; past the tensor, which reads as zeros, for no block
-          int first = p.num_blocks * p.hkv << p.page_log2;
-          if (id >= 0 && id < p.num_blocks) {
-            first = (id * p.hkv << p.page_log2) + w.kvh;
-          } else {
-            record_status(p.status, KTA_ERR_DEVICE_BOUNDS, SITE_BLOCK);
-          }
-          tma_load_5d(map, &full[st], ring + st * L::TILE + lane * group_box * L::GROUP, 0, 0, 0,
-                      ((i * pages + lane) & ((1 << split) - 1)) * group_box, first);
-        }
-        __syncwarp();
-        id = id1;
-        id1 = id2;
-      }
-    }
-    if (*abort_flag != 0 && lane == 0) {
-      // a role gave up: no copy may be in flight when the block ends (bounded like every wait)
-      int none = 0;
-      for (uint32_t k = n > RING ? n - RING : 0; k < n; ++k) {
-        mbar_wait(&full[k % RING], (k / RING) & 1u, &none, p.status, SITE_PROD_KV);
-      }
-    }
+  if (warp == K_WARP) {
+    produce_kv<D, RING>(p, w, member, &tmK, smem + L::OFF_K, k_full, k_empty, abort_flag);
+  } else if (warp == V_WARP) {
+    produce_kv<D, RING>(p, w, member, &tmV, smem + L::OFF_V, v_full, v_empty, abort_flag);
   } else if (warp == Q_WARP) {
-    // ------------------------------ Q producer ------------------------------
-    if (lane == 0) {
-      uint32_t n = 0;  // segments so far: buffer n % q_bufs
-      for (; w.left > 0; w.next(p), w.settle(p, member), ++n) {
-        const uint32_t buf = n % p.q_bufs, phase = (n / p.q_bufs) & 1u;
-        if (!mbar_wait(&q_empty[buf], phase ^ 1u, abort_flag, p.status, SITE_PROD_Q)) break;
-        mbar_arrive_expect_tx(&q_full[buf], static_cast<uint32_t>(p.box_tokens * p.group * D * 2));
-#pragma unroll
-        for (int h = 0; h < L::HALVES; ++h) {
-          tma_load_3d(&tmQ, &q_full[buf], smem + L::OFF_Q + h * L::Q_HALF + buf * p.q_shift, h * 64,
-                      w.kvh * p.group, w.row + w.row_tile(p, member) * p.tok_tile);
-        }
-      }
-      if (*abort_flag != 0) {
-        int none = 0;
-        for (uint32_t k = n > static_cast<uint32_t>(p.q_bufs) ? n - p.q_bufs : 0; k < n; ++k) {
-          mbar_wait(&q_full[k % p.q_bufs], (k / p.q_bufs) & 1u, &none, p.status, SITE_PROD_Q);
-        }
-      }
-    }
-    __syncwarp();
+    produce_q<D, 1>(p, w, member, &tmQ, smem + L::OFF_Q, 0, L::Q_HALF, q_full, q_empty, abort_flag);
   } else if (warp == MMA_WARP) {
     // ------------------------------ MMA issuer ------------------------------
     constexpr uint32_t FMT = BF16 ? 1u : 0u;
@@ -599,20 +233,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     constexpr uint32_t idesc_o = make_idesc(BM, D, FMT, FMT, 0u, 1u);   // P (TMEM) V (MN-major)
     // w and j run one tile ahead of the PVs, into the next segment: its first S is ready when the
     // softmax warps come from this one's epilogue.
+    const uint64_t qdesc = sdesc_sw128(smem_u32(smem + L::OFF_Q), 16, 1024);
     int j = 0, tiles = w.left > 0 ? w.count(p) : 0;
     uint32_t segment = 0, o_phase = 0;
     bool first_segment = true;
     // S of tile t into buffer t & 1, which holds P of tile t - 2 until its PV has read it: that was
     // issued before and ends before this begins.
     auto issue_s = [&](uint32_t t) -> bool {
-      const uint32_t buf = segment % p.q_bufs;
-      if (j == 0 && !mbar_wait(&q_full[buf], (segment / p.q_bufs) & 1u, abort_flag, p.status, SITE_MMA_Q)) {
-        return false;
-      }
+      if (j == 0 && !mbar_wait(q_full, segment & 1u, abort_flag, p.status, SITE_MMA_Q)) return false;
       const int st = static_cast<int>(t % RING);
       if (!mbar_wait(&k_full[st], (t / RING) & 1u, abort_flag, p.status, SITE_MMA_K)) return false;
       tc_fence_after();
-      const uint64_t qdesc = sdesc_sw128(smem_u32(smem + L::OFF_Q + buf * p.q_shift), 16, 1024);
       const uint64_t kdesc = sdesc_sw128(smem_u32(smem + L::OFF_K + st * L::TILE), 16, L::GROUP);
       if (elect_one_sync()) {
 #pragma unroll
@@ -623,7 +254,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         umma_commit(&s_full[t & 1u]);
         umma_commit(&k_empty[st]);
-        if (j + 1 == tiles) umma_commit(&q_empty[buf]);
+        if (j + 1 == tiles) umma_commit(q_empty);
       }
       __syncwarp();
       return true;
@@ -691,12 +322,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const bool live = row < rows;
       const bool warp_on = quarter * 32 < rows;
       uint64_t bits = 0;
-      if (live) {
-        const int t = rt * p.tok_tile + row / p.group;
-        bits = p.tree != nullptr ? static_cast<uint64_t>(p.tree[w.row + t])
-                                 : (2ull << t) - 1ull;  // t = 63: all ones
-        if (w.tokens < 64) bits &= (1ull << w.tokens) - 1ull;
-      }
+      if (live) bits = bits_of(p, w.row, rt * p.tok_tile + row / p.group, w.tokens);
       const int tiles = w.count(p);
       float m_used = -INFINITY, lsum = 0.f;
       for (int j = 0; j < tiles; ++j, ++g) {
@@ -708,7 +334,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             ok = false;
             break;
           }
-          clean_v<BF16, D>(smem + L::OFF_V + st * L::TILE, wg * HK, w.ctx - k0, w.len() - k0, k0 - w.ctx,
+          clean_v<BF16, D>(smem + L::OFF_V + st * L::TILE, wg * HK, HK, w.ctx - k0, w.len() - k0, k0 - w.ctx,
                            row, bad);
           fence_proxy_async_smem();
         }
@@ -803,12 +429,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               dst[i] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
             }
           } else if (live) {
-            float4* dst = p.part_o + (static_cast<long long>(slot) * (D / 4) + c / 4) * p.row_cap + row;
+            float4* dst = reinterpret_cast<float4*>(
+                p.part_o + (static_cast<long long>(slot) * p.row_cap + row) * D + c);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              dst[i * p.row_cap] =
-                  make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                              __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+              dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                   __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
             }
           }
         }
@@ -820,16 +446,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
       }
       if (threadIdx.x == 0 && !whole && w.i0 == 0) {  // the unit starts here: this CTA describes it
-        const Ranges r(p, plan[5]);
-        const int end = plan[4] - w.left + w.tiles() * row_tiles_of(p, w.tokens);  // of the unit
-        Desc d = {};
-        d.count = r.owner_before(end) - range + 1;
-        d.slot = slot;
-        d.next = (range + 1) * p.row_tiles + rt;  // a range's first segment is row tile = member
-        d.row = w.row + rt * p.tok_tile;
-        d.tokens = tokens;
-        d.kvh = w.kvh;
-        p.desc[blockIdx.x] = d;
+        p.desc[blockIdx.x] = describe(p, w, rt, tokens, slot, plan);
       }
       tc_fence_before();
       __syncwarp();
@@ -847,7 +464,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 
 // Joins the parts of a unit that several ranges hold: M = max m, O = sum 2^(m - M) O_part /
 // sum 2^(m - M) l. Block (x, y): the unit that starts in CTA x, part y of its elements; a thread
-// takes four elements of a row, rows of a warp back to back, eight parts' loads at a time.
+// takes four elements of a row, a warp the row's 128 back to back, eight parts' loads at a time.
 constexpr int JOIN_THREADS = 128;
 constexpr int JOIN_PARTS = 8;
 
@@ -861,7 +478,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Params p) {
   const int items = rows * (D / 4);
   for (int item = blockIdx.y * JOIN_THREADS + threadIdx.x; item < items;
        item += gridDim.y * JOIN_THREADS) {
-    const int d4 = item / rows, row = item - d4 * rows;
+    const int row = item / (D / 4), d4 = item % (D / 4);
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c0 = 0; c0 < d.count; c0 += JOIN_PARTS) {
@@ -875,7 +492,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Params p) {
         if (c < d.count) {
           const long long slot = c == 0 ? d.slot : 2LL * (d.next + (c - 1) * p.row_tiles);
           ml[i] = __ldcg(p.part_ml + slot * p.row_cap + row);
-          part[i] = __ldcg(p.part_o + (slot * (D / 4) + d4) * p.row_cap + row);
+          part[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (slot * p.row_cap + row) * D) + d4);
         }
       }
       float top = m;
@@ -950,13 +567,18 @@ int go(Params& p, const void* Q, const void* Kc, const void* Vc, int64_t q_token
   if (s != KTA_OK) return s;
   s = encode_tmap(&tv, type, 5, Vc, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   if (s != KTA_OK) return s;
-  auto kernel = tree_kernel<BF16, D>;
-  s = set_kernel_smem(reinterpret_cast<const void*>(kernel), L::TOTAL);
-  if (s != KTA_OK) return s;
   const int sms = std::min(current_sm_count(), MAX_CTAS);
   if (sms < p.row_tiles) return KTA_ERR_UNSUPPORTED;
   const int grid = sms / p.row_tiles * p.row_tiles;
-  s = launch_ex(kernel, dim3(grid), dim3(NUM_THREADS), L::TOTAL, stream, 1, tq, tk, tv, p);
+  // One tcgen05 tile has 128 rows in wide_kernel however few are real, and up to 64 in the other.
+  if (p.box_tokens * p.group <= NARROW_ROWS) {
+    s = launch_narrow<BF16, D>(p, tq, tk, tv, grid, stream);
+  } else {
+    auto kernel = wide_kernel<BF16, D>;
+    s = set_kernel_smem(reinterpret_cast<const void*>(kernel), L::TOTAL);
+    if (s != KTA_OK) return s;
+    s = launch_ex(kernel, dim3(grid), dim3(NUM_THREADS), L::TOTAL, stream, 1, tq, tk, tv, p);
+  }
   if (s != KTA_OK) return s;
   // four elements a thread and at most four passes
   const int parts = std::max(1, std::min(8, p.row_cap * (D / 4) / (2 * JOIN_THREADS)));
@@ -1012,7 +634,7 @@ int launch(const void* Q, const void* Kc, const void* Vc, const void* tables, co
   uint8_t* base = static_cast<uint8_t*>(workspace);
   p.desc = reinterpret_cast<Desc*>(base);
   p.part_ml = reinterpret_cast<float2*>(base + ws.off_ml);
-  p.part_o = reinterpret_cast<float4*>(base + ws.off_o);
+  p.part_o = reinterpret_cast<float*>(base + ws.off_o);
   p.table_stride = table_stride;
   p.batch = static_cast<int>(B);
   p.rows = static_cast<int>(tokens);
@@ -1027,10 +649,6 @@ int launch(const void* Q, const void* Kc, const void* Vc, const void* tables, co
   p.tok_tile = BM / p.group;
   p.box_tokens = std::min(p.tok_tile, p.max_new);
   p.row_tiles = static_cast<int>(row_tiles);
-  // two Q tiles where they fit (64 rows): the next segment's Q then comes while this one runs
-  const int q_rows = (p.box_tokens * p.group + 7) / 8 * 8;
-  p.q_bufs = q_rows <= BM / 2 ? 2 : 1;
-  p.q_shift = BM / 2 * 128;
   p.row_cap = ws.row_cap;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = device_status_ptr();
