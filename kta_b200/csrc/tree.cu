@@ -172,8 +172,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   unsigned int* bad = reinterpret_cast<unsigned int*>(smem + L::OFF_MISC + 8);   // [2]
   // the range's first segment (request, KV head, tile), its place in the work list, the range's end,
-  // and the list's total
-  volatile int* plan = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 16);  // [6]
+  // the list's total, and the first request's rows, tokens and context
+  volatile int* plan = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 16);  // [9]
   float2* ml = reinterpret_cast<float2*>(smem + L::OFF_ML);
   int* warp_sum = reinterpret_cast<int*>(smem + L::OFF_ML);  // before the first segment ends
 

@@ -238,7 +238,7 @@ __device__ __forceinline__ uint64_t bits_of(const Params& p, int row, int t, int
 }
 
 // The start of every CTA, after griddepcontrol.wait and with the barriers initialised: finds its
-// range's first segment and end, by all threads. plan[0..5] and warp_sum[12] are shared memory;
+// range's first segment and end, by all threads. plan[0..8] and warp_sum[12] are shared memory;
 // rejected requests' rows are zeroed on the way. Synchronises the CTA twice.
 template <int D>
 __device__ __forceinline__ Walk plan_range(const Params& p, int member, volatile int* plan, int* warp_sum) {
@@ -246,8 +246,16 @@ __device__ __forceinline__ Walk plan_range(const Params& p, int member, volatile
   const int per = (p.batch + NUM_THREADS - 1) / NUM_THREADS;  // requests of a thread
   const int b0 = min(static_cast<int>(threadIdx.x) * per, p.batch), b1 = min(b0 + per, p.batch);
   auto work_of = [&](const Request& r) { return tiles_of(r) * p.hkv * row_tiles_of(p, r.tokens); };
+  // a thread's first request is kept: with up to 384 of them nothing is loaded twice
+  Request mine_first = {};
   int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += work_of(request_of(p, b));
+  bool bad = false;
+  for (int b = b0; b < b1; ++b) {
+    const Request r = request_of(p, b);
+    if (b == b0) mine_first = r;
+    mine += work_of(r);
+    bad |= r.bad;
+  }
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -273,7 +281,7 @@ __device__ __forceinline__ Walk plan_range(const Params& p, int member, volatile
       if (at < before || at >= before + mine) continue;
       int t = before;
       for (int b = b0; b < b1; ++b) {
-        const Request r = request_of(p, b);
+        const Request r = b == b0 ? mine_first : request_of(p, b);
         const int n = work_of(r);
         if (at >= t + n) {
           t += n;
@@ -285,6 +293,9 @@ __device__ __forceinline__ Walk plan_range(const Params& p, int member, volatile
           plan[0] = b;
           plan[1] = kvh;
           plan[2] = off / k;
+          plan[6] = r.row;
+          plan[7] = r.tokens;
+          plan[8] = r.ctx;
         }
         plan[3 + e] = at - off % k;
         break;
@@ -295,17 +306,18 @@ __device__ __forceinline__ Walk plan_range(const Params& p, int member, volatile
       plan[5] = total;
     }
   }
-  // requests that are out of range: their rows that exist become zero
-  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-    if (!request_of(p, b).bad) continue;
-    if (threadIdx.x == 0) record_status(p.status, KTA_ERR_DEVICE_BOUNDS, SITE_REQUEST);
-    const long long a = max(p.offsets[b], 0), z = min(p.offsets[b + 1], p.rows);
-    const long long words = (z - a) * p.hq * (D / 2);
-    uint32_t* o = static_cast<uint32_t*>(p.out) + a * p.hq * (D / 2);
-    for (long long i = threadIdx.x; i < words; i += NUM_THREADS) o[i] = 0u;
-    for (long long i = threadIdx.x; i < (z - a) * p.hq; i += NUM_THREADS) p.lse[a * p.hq + i] = -INFINITY;
+  if (__syncthreads_or(bad ? 1 : 0)) {
+    // requests that are out of range: their rows that exist become zero
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+      if (!request_of(p, b).bad) continue;
+      if (threadIdx.x == 0) record_status(p.status, KTA_ERR_DEVICE_BOUNDS, SITE_REQUEST);
+      const long long a = max(p.offsets[b], 0), z = min(p.offsets[b + 1], p.rows);
+      const long long words = (z - a) * p.hq * (D / 2);
+      uint32_t* o = static_cast<uint32_t*>(p.out) + a * p.hq * (D / 2);
+      for (long long i = threadIdx.x; i < words; i += NUM_THREADS) o[i] = 0u;
+      for (long long i = threadIdx.x; i < (z - a) * p.hq; i += NUM_THREADS) p.lse[a * p.hq + i] = -INFINITY;
+    }
   }
-  __syncthreads();
   Walk w;
   w.left = 0;
   if (busy) {
@@ -314,7 +326,9 @@ __device__ __forceinline__ Walk plan_range(const Params& p, int member, volatile
     w.i0 = plan[2];
     w.left = plan[4] - plan[3];
     w.turn = 0;
-    w.set(request_of(p, w.b));
+    w.row = plan[6];
+    w.tokens = plan[7];
+    w.ctx = plan[8];
     w.settle(p, member);
   }
   return w;

@@ -56,13 +56,14 @@ struct Narrow {
   static constexpr int OFF_P = OFF_Q + Q_BUFS * Q_BUF;
   static constexpr int OFF_ML = OFF_P + 2 * P_BUF;                   // [warp][N] (maximum, sum)
   static constexpr int OFF_FACTOR = OFF_ML + SOFTMAX_WARPS * N * 8;  // [buffer][warp][N]
-  static constexpr int OFF_BAR = OFF_FACTOR + 2 * SOFTMAX_WARPS * N * 4;
+  static constexpr int OFF_WEIGHT = OFF_FACTOR + 2 * SOFTMAX_WARPS * N * 4;  // [N][warp]
+  static constexpr int OFF_BAR = OFF_WEIGHT + SOFTMAX_WARPS * N * 4;
   // k_full, k_empty, v_full, v_empty, q_full, q_empty, s_full[2], p_full[2], p_empty[2], pv_done,
   // corrected, ml_full, ml_empty, o_full, o_free
   static constexpr int NUM_BARS = 2 * K_RING + 2 * V_RING + 2 * Q_BUFS + 12;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
-  // misc: tmem base, abort, non-finite drafts [2], plan [6], correction requests [2][4]
-  static constexpr int TOTAL = OFF_MISC + 80;
+  // misc: tmem base, abort, non-finite drafts [2], plan [9], correction requests [2][4]
+  static constexpr int TOTAL = OFF_MISC + 96;
   static_assert(TOTAL <= 232448, "shared memory budget of one sm_100 CTA");
   // TMEM: S^T of buffer i at i N, O^T of warp w at (2 + w) N
   static constexpr uint32_t COL_O = 2 * N;
@@ -140,15 +141,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   uint64_t* pv_done = p_empty + 2;            // one phase for each PV
   uint64_t* corrected = pv_done + 1;          // the scaling that a tile asked for is done
   uint64_t* ml_full = corrected + 1;          // the segment's maxima and sums are written
-  uint64_t* ml_empty = ml_full + 1;           // ... and read
+  uint64_t* ml_empty = ml_full + 1;           // ... and read, and the weights made of them
   uint64_t* o_full = ml_empty + 1;            // the segment's last PV
   uint64_t* o_free = o_full + 1;              // the epilogue has read O
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   unsigned int* bad = reinterpret_cast<unsigned int*>(smem + L::OFF_MISC + 8);    // [2]
-  volatile int* plan = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 16);  // [6]
-  volatile int* ask = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 40);   // [buffer][warp]
+  volatile int* plan = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 16);  // [9]
+  volatile int* ask = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 56);   // [buffer][warp]
   float2* ml = reinterpret_cast<float2*>(smem + L::OFF_ML);
+  float4* weights = reinterpret_cast<float4*>(smem + L::OFF_WEIGHT);  // [N] of the four warps
   volatile float* factors = reinterpret_cast<volatile float*>(smem + L::OFF_FACTOR);
 
   const int warp = warp_id();
@@ -309,6 +311,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     bool ok = true;
     for (; w.left > 0 && ok; w.next(p), w.settle(p, 0), ++segment) {
       const int tiles = w.count(p);
+      // lane r (and r + 32): what row r sees, for the tiles that hold drafted tokens
+      constexpr int PER = (N + 31) / 32;
+      uint64_t bits[PER];
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        const int r = lane + 32 * u;
+        bits[u] = r < w.tokens * p.group && (w.i0 + tiles) * BN > w.ctx
+                      ? bits_of(p, w.row, r / p.group, w.tokens)
+                      : 0ull;
+      }
       float m[C8][2];
       uint64_t sum[C8];
 #pragma unroll
@@ -341,42 +353,42 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         reg_fence(s[0]);
         reg_fence(s[1]);
         if (masked) {
-          const int rows = w.tokens * p.group;
           const int key = k0 - w.ctx + warp * 32 + (lane >> 2);  // of the first, drafted from 0 on
 #pragma unroll
           for (int c = 0; c < C8; ++c) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int r = 8 * c + col0 + e;
-              const uint64_t bits = r < rows ? bits_of(p, w.row, r / p.group, w.tokens) : 0ull;
+              const uint64_t view = __shfl_sync(0xffffffffu, bits[c / 4], (8 * c + col0 + e) & 31);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int k = key + 8 * i;
-                const bool sees = k < 0 || (k < 64 && ((bits >> k) & 1ull) != 0);
+                const bool sees = k < 0 || (k < 64 && ((view >> k) & 1ull) != 0);
                 if (!sees) s[i >> 1][4 * c + 2 * (i & 1) + e] = __float_as_uint(-INFINITY);
               }
             }
           }
         }
-        uint64_t x[C8][4];  // s sl - m, pairs of columns of four keys
-        float top = -INFINITY;
-        auto shift = [&]() {
-          top = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < C8; ++c) {
-            const uint64_t neg = f2(-m[c][0], -m[c][1]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              x[c][i] = fma2(f2(__uint_as_float(s[i >> 1][4 * c + 2 * (i & 1)]),
-                                __uint_as_float(s[i >> 1][4 * c + 2 * (i & 1) + 1])),
-                             sl2, neg);
-              float x0, x1;
-              f2_split(x[c][i], x0, x1);
-              top = max3(top, x0, x1);
-            }
-          }
+        // s sl - m of the thread's i-th key, columns 8 c + col0 and its neighbour
+        auto shifted = [&](int c, int i) -> uint64_t {
+          return fma2(f2(__uint_as_float(s[i >> 1][4 * c + 2 * (i & 1)]),
+                         __uint_as_float(s[i >> 1][4 * c + 2 * (i & 1) + 1])),
+                      sl2, f2(-m[c][0], -m[c][1]));
         };
-        shift();
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < C8; ++c) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float x0, x1;
+            f2_split(shifted(c, i), x0, x1);
+            top = max3(top, x0, x1);
+          }
+        }
+        // the buffer of P and of the factors: the PV two tiles ago has read the one, warps 4-7 the other
+        if (!mbar_wait(&p_empty[buf], ((g >> 1) & 1u) ^ 1u, abort_flag, p.status, SITE_N_SM_P)) {
+          ok = false;
+          break;
+        }
         int scale_o = 0;
         if (__any_sync(0xffffffffu, top > RESCALE_THRESHOLD)) {
           // some column's maximum moves: take the columns' maxima over the warp's 32 keys
@@ -409,12 +421,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             sum[c] = f2(s0 * f[0], s1 * f[1]);
           }
           scale_o = __any_sync(0xffffffffu, scale) ? 1 : 0;
-          shift();
-        }
-        // P's buffer: the PV two tiles ago has read it, and warps 4-7 what it asked for
-        if (!mbar_wait(&p_empty[buf], ((g >> 1) & 1u) ^ 1u, abort_flag, p.status, SITE_N_SM_P)) {
-          ok = false;
-          break;
         }
 #pragma unroll
         for (int c = 0; c < C8; ++c) {
@@ -422,7 +428,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float x0, x1;
-            f2_split(x[c][i], x0, x1);
+            f2_split(shifted(c, i), x0, x1);
             const float e0 = ex2(x0), e1 = ex2(x1);
             sum[c] = add2(sum[c], f2(e0, e1));
             pk[i] = pack2<BF16>(e0, e1);
@@ -511,92 +517,93 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const bool whole = w.i0 == 0 && tiles == w.tiles();
       const int rows = w.tokens * p.group;
       const int slot = 2 * static_cast<int>(blockIdx.x) + (first_part ? 0 : 1);
-      // lane r (and r + 32): row r's four states, their weights and the joined maximum and sum
-      constexpr int PER = (N + 31) / 32;
-      float wt[PER][SOFTMAX_WARPS];
-      uint64_t lost[PER];
+      // Lane r (and r + 32): the weights of row r's four states. The four warps write the same
+      // values; none gets to the next segment's while another reads these (ml_empty).
 #pragma unroll
-      for (int u = 0; u < PER; ++u) {
+      for (int u = 0; u < (N + 31) / 32; ++u) {
         const int r = lane + 32 * u;
-        float mm[SOFTMAX_WARPS], ll[SOFTMAX_WARPS];
+        if (r >= N) continue;
+        float wt[SOFTMAX_WARPS];
         float top = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int h = 0; h < SOFTMAX_WARPS; ++h) {
-          const float2 v = r < N ? ml[h * N + r] : make_float2(-INFINITY, 0.f);
-          mm[h] = v.x;
-          ll[h] = v.y;
-          top = fmaxf(top, v.x);
-        }
+        for (int h = 0; h < SOFTMAX_WARPS; ++h) top = fmaxf(top, ml[h * N + r].x);
         const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int h = 0; h < SOFTMAX_WARPS; ++h) {
-          wt[u][h] = ex2(mm[h] - base);
-          l = fmaf(wt[u][h], ll[h], l);
+          const float2 v = ml[h * N + r];
+          wt[h] = ex2(v.x - base);
+          l = fmaf(wt[h], v.y, l);
         }
-        lost[u] = 0;
-        if (r < rows) {
-          const int tok = r / p.group;
-          lost[u] = static_cast<uint64_t>(bad[1]) << 32 | bad[0];
-          if (lost[u] != 0) lost[u] &= bits_of(p, w.row, tok, w.tokens);
-          if (quarter == 0) {
-            if (whole) {
-              p.lse[static_cast<long long>(w.row + tok) * p.hq + w.kvh * p.group + (r - tok * p.group)] =
-                  l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
-            } else {
-              p.part_ml[static_cast<long long>(slot) * p.row_cap + r] = make_float2(top, l);
-            }
+        if (r < rows && quarter == 0) {
+          if (whole) {
+            const int tok = r / p.group;
+            p.lse[static_cast<long long>(w.row + tok) * p.hq + w.kvh * p.group + (r - tok * p.group)] =
+                l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+          } else {
+            p.part_ml[static_cast<long long>(slot) * p.row_cap + r] = make_float2(top, l);
           }
         }
-        if (whole) {  // a row that sees nothing: O = 0
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-          for (int h = 0; h < SOFTMAX_WARPS; ++h) wt[u][h] *= inv;
-        }
+        // a row that sees nothing: O = 0; a partial stays as it is, for the join to divide
+        const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        weights[r] = make_float4(wt[0] * inv, wt[1] * inv, wt[2] * inv, wt[3] * inv);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(ml_empty);
       if (!mbar_wait(o_full, segment & 1u, abort_flag, p.status, SITE_N_OUT_O)) break;
       tc_fence_after();
       uint16_t* out = static_cast<uint16_t*>(p.out) +
                       (static_cast<long long>(w.row) * p.hq + w.kvh * p.group) * D + d;
       float* part = p.part_o + static_cast<long long>(slot) * p.row_cap * D + d;
+      const int gap = (p.hq - p.group) * D;  // from a token's last head to the next token's first
+      long long at = 0;
+      int head = 0;
+#pragma unroll 1
+      for (int c = 0; c < rows; c += 8) {
+        uint32_t o[SOFTMAX_WARPS][8];
 #pragma unroll
-      for (int c = 0; c < N; c += 16) {
-        if (c >= rows) break;
-        uint32_t o[SOFTMAX_WARPS][16];
-#pragma unroll
-        for (int h = 0; h < SOFTMAX_WARPS; ++h) tmem_ld_32x32b_x16(t_o + h * N + c, o[h]);
+        for (int h = 0; h < SOFTMAX_WARPS; ++h) tmem_ld_32x32b_x8(t_o + h * N + c, o[h]);
         tmem_ld_wait();
 #pragma unroll
         for (int h = 0; h < SOFTMAX_WARPS; ++h) reg_fence(o[h]);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int r = c + i;
-          float v = 0.f;
-#pragma unroll
-          for (int h = 0; h < SOFTMAX_WARPS; ++h) {
-            v = fmaf(__uint_as_float(o[h][i]), __shfl_sync(0xffffffffu, wt[c / 32][h], r & 31), v);
-          }
-          uint64_t left = __shfl_sync(0xffffffffu, lost[c / 32], r & 31);
-          if (r < rows && d < D) {
-            // drafted V elements that are not finite, for the rows that see them
-            for (; left != 0; left &= left - 1) {
-              const int key = w.ctx + __ffsll(static_cast<long long>(left)) - 1;
-              if (key < w.i0 * BN || key >= (w.i0 + tiles) * BN) continue;
-              const int id = p.tables[w.b * p.table_stride + (key >> p.page_log2)];
-              if (id < 0 || id >= p.num_blocks) continue;
-              const float bad_v = load16<BF16>(
-                  p.v, (((static_cast<long long>(id) << p.page_log2) + (key & ((1 << p.page_log2) - 1))) *
-                            p.hkv + w.kvh) * D + d);
-              if (!isfinite(bad_v)) v += bad_v;
-            }
+        for (int i = 0; i < 8; ++i) {
+          const float4 wt = weights[c + i];
+          float v = __uint_as_float(o[0][i]) * wt.x;
+          v = fmaf(__uint_as_float(o[1][i]), wt.y, v);
+          v = fmaf(__uint_as_float(o[2][i]), wt.z, v);
+          v = fmaf(__uint_as_float(o[3][i]), wt.w, v);
+          if (c + i < rows && d < D) {
             if (whole) {
-              const int tok = r / p.group;
-              const uint32_t pair = pack2<BF16>(v, 0.f);
-              out[(static_cast<long long>(tok) * p.hq + (r - tok * p.group)) * D] =
-                  static_cast<uint16_t>(pair & 0xffffu);
+              out[at] = static_cast<uint16_t>(pack2<BF16>(v, 0.f) & 0xffffu);
             } else {
-              part[static_cast<long long>(r) * D] = v;
+              part[(c + i) * D] = v;
+            }
+          }
+          at += D;
+          if (++head == p.group) {
+            head = 0;
+            at += gap;
+          }
+        }
+      }
+      if ((bad[0] | bad[1]) != 0u && d < D) {
+        // drafted V elements that are not finite, for the rows that see them
+        const uint64_t marked = static_cast<uint64_t>(bad[1]) << 32 | bad[0];
+        for (int r = 0; r < rows; ++r) {
+          const int tok = r / p.group;
+          for (uint64_t left = marked & bits_of(p, w.row, tok, w.tokens); left != 0; left &= left - 1) {
+            const int key = w.ctx + __ffsll(static_cast<long long>(left)) - 1;
+            if (key < w.i0 * BN || key >= (w.i0 + tiles) * BN) continue;
+            const int id = p.tables[w.b * p.table_stride + (key >> p.page_log2)];
+            if (id < 0 || id >= p.num_blocks) continue;
+            const float v = load16<BF16>(
+                p.v, (((static_cast<long long>(id) << p.page_log2) + (key & ((1 << p.page_log2) - 1))) *
+                          p.hkv + w.kvh) * D + d);
+            if (isfinite(v)) continue;
+            if (whole) {
+              uint16_t* o = out + (static_cast<long long>(tok) * p.hq + (r - tok * p.group)) * D;
+              *o = static_cast<uint16_t>(pack2<BF16>(load16<BF16>(o, 0) + v, 0.f) & 0xffffu);
+            } else {
+              part[r * D] += v;
             }
           }
         }
@@ -606,7 +613,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(o_free);
+      if (lane == 0) {
+        mbar_arrive(ml_empty);
+        mbar_arrive(o_free);
+      }
     }
   }
 
