@@ -3,6 +3,8 @@
 // of V tiles that end inside a page. The operator is described in tree.cu.
 #pragma once
 
+#include <cstddef>
+
 #include "kta_common.cuh"
 #include "kta_host.h"
 
@@ -18,8 +20,10 @@ constexpr int V_WARP = 10;
 constexpr int Q_WARP = 11;
 constexpr int MAX_DRAFT = 64;         // bits of a row of the tree
 constexpr int MAX_GROUP = 16;
-constexpr int MAX_BATCH = 1 << 16;
-constexpr int MAX_CTAS = 256;         // the workspace is sized for this many
+constexpr int MAX_BATCH = 2048;       // the decode entries' limit
+constexpr int MAX_CTAS = 160;         // the workspace is sized for this many
+constexpr int ROUNDS = 4;             // ranges of a CTA, about
+constexpr int MAX_ITEMS = ROUNDS * MAX_CTAS;
 constexpr int NARROW_ROWS = 64;       // up to so many rows of a request: tree_narrow.cu
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units: the maximum moves when it grew > 2^8
 
@@ -39,17 +43,29 @@ enum : unsigned int {
   SITE_SMEM = 0x910,     // shared memory not aligned as declared
   SITE_REQUEST = 0x911,  // lengths or offsets out of range
   SITE_BLOCK = 0x912,    // a block id out of range
+  SITE_NEXT = 0x913,     // the next range's entry
+  SITE_NEXT_FREE = 0x914,
+  SITE_JOIN = 0x915,     // the warps that join a unit, among themselves
 };
 
-// What the join kernel needs of a unit that starts in a CTA's range and ends in a later one.
-struct Desc {
-  int count;    // ranges that hold a part of it; 0: none
-  int slot;     // the first part's slot
-  int next;     // CTA of the second part; the others follow row_tiles apart, each in slot 0
-  int row;      // first query token
-  int tokens;
-  int kvh;
-  int pad[2];
+// The work list is the 128-key tiles of every (request, KV head), cut into ranges (plan_kernel).
+// An item is a range for one of its row_tiles members.
+struct Range {
+  int b, kvh, i0;        // the first tile
+  int left;              // its length in the work list's count, 0: no more ranges
+  int row, tokens, ctx;  // of request b
+  int home;              // i0 > 0: the range in which the first tile's unit starts
+  int span;              // ranges that hold a part of the unit that starts here and ends later; 0: none
+  int id, member;        // filled in where the item is taken
+  int pad;
+};
+constexpr int RANGE_WORDS = sizeof(Range) / 4;
+
+// Ranges stand in the order of the list, `cuts` of a share one after the other. Items are taken in
+// the order (cut, share, member).
+struct Plan {
+  int shares, cuts;
+  unsigned int next;  // items taken beyond the first gridDim.x
 };
 
 struct Params {
@@ -60,16 +76,18 @@ struct Params {
   void* out;               // [rows, Hq, D]
   float* lse;              // [rows, Hq]
   const void* v;           // the V cache, for drafted rows that are not finite
-  Desc* desc;              // [CTAs]
-  float2* part_ml;         // [2 CTAs][row_cap] (maximum, sum), log2 units
-  float* part_o;           // [2 CTAs][row_cap][D], not normalised
+  Plan* plan;
+  Range* ranges;           // [MAX_ITEMS]
+  unsigned int* arrived;   // [MAX_ITEMS] parts of the unit that starts in a range, for a row tile
+  float2* part_ml;         // [2 MAX_ITEMS][row_cap] (maximum, sum), log2 units
+  float* part_o;           // [2 MAX_ITEMS][row_cap][D], not normalised
   long long table_stride;
   int batch, rows, hq, hkv, group, max_new, max_blocks, num_blocks;
   int page_log2;           // tokens of a block
   int box_log2;            // tokens of a TMA box: min(block, 128)
   int tok_tile;            // drafted tokens of a row tile: 128 / group
   int box_tokens;          // tokens of the Q box: min(tok_tile, max_new)
-  int row_tiles;           // CTAs that share a range
+  int row_tiles;           // members of a range, a row tile each
   int row_cap;             // rows of a partial
   float scale_log2;        // softmax scale * log2(e)
   unsigned int* status;
@@ -112,42 +130,54 @@ __device__ __forceinline__ int row_tiles_of(const Params& p, int tokens) {
   return (tokens + p.tok_tile - 1) / p.tok_tile;
 }
 
-// The work list: tile i of KV head h of request b, b-major, each counted once for every row tile
-// of its request (the CTAs of a range share those). Range k of n is [total k / n, total (k + 1) / n)
-// rounded down to whole tiles; n <= total / row_tiles, so that none is empty.
-struct Ranges {
-  int total, n;
-  __device__ __forceinline__ Ranges(const Params& p, int total_) : total(total_) {
-    n = total == 0 ? 0 : max(1, min(static_cast<int>(gridDim.x) / p.row_tiles, total / p.row_tiles));
-  }
-  __device__ __forceinline__ int start(int k) const {
-    return static_cast<int>(static_cast<long long>(total) * k / n);
-  }
-  // the range of the last tile before position `end`, the end of a unit
-  __device__ __forceinline__ int owner_before(int end) const {
-    return static_cast<int>((static_cast<long long>(end) * n - 1) / total);
-  }
+// A CTA's walk over the segments of its ranges: runs of count() tiles from i0 on of one (request,
+// KV head). Few fields, since the softmax warps keep it beside a row of S. Every warp walks by
+// itself; from the second range on it reads them from a two-entry ring in shared memory that the K
+// producer fills.
+struct Feed {
+  Range* ring;  // [2]
+  uint64_t* full;
+  uint64_t* empty;
+  volatile int* abort;
 };
 
-// A range's walk over its segments: runs of count() tiles from i0 on of one (request, KV head).
-// Few fields, since the softmax warps keep it beside a row of S.
 struct Walk {
   int row, tokens, ctx;  // of the request
   int b, kvh, i0;
   int left;              // of the range from here on, in the work list's count
-  int turn;              // the CTA of the range's that takes the segment's first row tile
+  int turn;              // the member that takes the segment's first row tile
+  int id, member;        // of the item
+  uint32_t taken;        // entries of the ring so far
 
-  __device__ __forceinline__ void set(const Request& r) {
-    row = r.row;
-    tokens = r.tokens;
-    ctx = r.ctx;
-  }
   __device__ __forceinline__ int len() const { return ctx + tokens; }
   __device__ __forceinline__ int tiles() const { return (len() + BN - 1) / BN; }
   __device__ __forceinline__ int count(const Params& p) const {
     return min(tiles() - i0, left / row_tiles_of(p, tokens));
   }
-  __device__ __forceinline__ void next(const Params& p) {
+  // The row tile of the request that falls to this member. Requests have between one and row_tiles
+  // of them: the members take turns, so that each has its share over some segments.
+  __device__ __forceinline__ int row_tile(const Params& p) const {
+    const int k = member - turn;
+    return k < 0 ? k + p.row_tiles : k;
+  }
+  // Drafted tokens of this member's row tile: 0 where the request has fewer.
+  __device__ __forceinline__ int rows(const Params& p) const {
+    return max(0, min(tokens - row_tile(p) * p.tok_tile, p.tok_tile));
+  }
+  __device__ __forceinline__ void set(const Range& r) {
+    b = r.b;
+    kvh = r.kvh;
+    i0 = r.i0;
+    left = r.left;
+    row = r.row;
+    tokens = r.tokens;
+    ctx = r.ctx;
+    id = r.id;
+    member = r.member;
+    turn = 0;
+  }
+  // Past this segment, inside the range.
+  __device__ __forceinline__ void step(const Params& p) {
     const int k = row_tiles_of(p, tokens);
     left -= count(p) * k;
     if (left <= 0) return;
@@ -159,22 +189,58 @@ struct Walk {
       do {  // tiles are left in the range, so a request with some follows
         r = request_of(p, ++b);
       } while (tiles_of(r) == 0);
-      set(r);
+      row = r.row;
+      tokens = r.tokens;
+      ctx = r.ctx;
     }
   }
-  // The row tile of the request that falls to CTA `member` of the range's. Requests have between
-  // one and row_tiles of them: the CTAs take turns, so that each has its share over some segments.
-  __device__ __forceinline__ int row_tile(const Params& p, int member) const {
-    const int k = member - turn;
-    return k < 0 ? k + p.row_tiles : k;
+  // To the range's next segment, this one included, in which the member has rows; left is 0 where
+  // there is none.
+  __device__ __forceinline__ void settle(const Params& p) {
+    while (left > 0 && rows(p) == 0) step(p);
   }
-  // Drafted tokens of row tile rt in the request: 0 where it has fewer.
-  __device__ __forceinline__ int rows(const Params& p, int rt) const {
-    return max(0, min(tokens - rt * p.tok_tile, p.tok_tile));
+  // The CTA's first item; left is 0 where it has none.
+  __device__ __forceinline__ void open(const Params& p) {
+    taken = 0;
+    left = 0;
+    const int share = static_cast<int>(blockIdx.x) / p.row_tiles;
+    if (share >= p.plan->shares) return;
+    const int range = share * p.plan->cuts;
+    Range r = p.ranges[range];
+    r.id = range;
+    r.member = static_cast<int>(blockIdx.x) - share * p.row_tiles;
+    set(r);
   }
-  // To the next segment, this one included, in which CTA `member` has rows.
-  __device__ __forceinline__ void settle(const Params& p, int member) {
-    while (left > 0 && rows(p, row_tile(p, member)) == 0) next(p);
+  // The next range from the ring, by a warp (or by its lane 0 alone); left is 0 at the end.
+  __device__ __forceinline__ void take(const Params& p, const Feed& f, bool alone) {
+    left = 0;
+    const uint32_t at = taken & 1u;
+    if (!mbar_wait(&f.full[at], (taken >> 1) & 1u, f.abort, p.status, SITE_NEXT)) return;
+    set(f.ring[at]);
+    ++taken;
+    if (!alone) __syncwarp();
+    if (alone || (threadIdx.x & 31) == 0) mbar_arrive(&f.empty[at]);
+  }
+  // A first segment with rows, from the first item or a later one.
+  __device__ __forceinline__ void begin(const Params& p, const Feed& f, bool alone = false) {
+    open(p);
+    if (left <= 0) return;
+    settle(p);
+    while (left <= 0) {
+      take(p, f, alone);
+      if (left <= 0) return;
+      settle(p);
+    }
+  }
+  // The next segment with rows, in this range or the next ones.
+  __device__ __forceinline__ void next(const Params& p, const Feed& f, bool alone = false) {
+    step(p);
+    if (left > 0) settle(p);
+    while (left <= 0) {
+      take(p, f, alone);
+      if (left <= 0) return;
+      settle(p);
+    }
   }
 };
 
@@ -237,194 +303,176 @@ __device__ __forceinline__ uint64_t bits_of(const Params& p, int row, int t, int
   return tokens < 64 ? bits & ((1ull << tokens) - 1ull) : bits;
 }
 
-// The start of every CTA, after griddepcontrol.wait and with the barriers initialised: finds its
-// range's first segment and end, by all threads. plan[0..8] and warp_sum[12] are shared memory;
-// rejected requests' rows are zeroed on the way. Synchronises the CTA twice.
-template <int D>
-__device__ __forceinline__ Walk plan_range(const Params& p, int member, volatile int* plan, int* warp_sum) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = (p.batch + NUM_THREADS - 1) / NUM_THREADS;  // requests of a thread
-  const int b0 = min(static_cast<int>(threadIdx.x) * per, p.batch), b1 = min(b0 + per, p.batch);
-  auto work_of = [&](const Request& r) { return tiles_of(r) * p.hkv * row_tiles_of(p, r.tokens); };
-  // a thread's first request is kept: with up to 384 of them nothing is loaded twice
-  Request mine_first = {};
-  int mine = 0;
-  bool bad = false;
-  for (int b = b0; b < b1; ++b) {
-    const Request r = request_of(p, b);
-    if (b == b0) mine_first = r;
-    mine += work_of(r);
-    bad |= r.bad;
-  }
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) warp_sum[warp] = incl;
-  __syncthreads();
-  int before = incl - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < NUM_THREADS / 32; ++w) {
-    if (w < warp) before += warp_sum[w];
-    total += warp_sum[w];
-  }
-  const Ranges rg(p, total);
-  const int range = blockIdx.x / p.row_tiles;
-  const bool busy = range < rg.n;
-  if (busy) {
-    // the range's two ends, by the threads whose requests they fall into
-    const int from = rg.start(range), to = rg.start(range + 1);
-    for (int e = 0; e < 2; ++e) {
-      const int at = e == 0 ? from : to;
-      if (at < before || at >= before + mine) continue;
-      int t = before;
-      for (int b = b0; b < b1; ++b) {
-        const Request r = b == b0 ? mine_first : request_of(p, b);
-        const int n = work_of(r);
-        if (at >= t + n) {
-          t += n;
-          continue;
-        }
-        const int k = row_tiles_of(p, r.tokens), pair = tiles_of(r) * k;
-        const int kvh = (at - t) / pair, off = at - t - kvh * pair;
-        if (e == 0) {
-          plan[0] = b;
-          plan[1] = kvh;
-          plan[2] = off / k;
-          plan[6] = r.row;
-          plan[7] = r.tokens;
-          plan[8] = r.ctx;
-        }
-        plan[3 + e] = at - off % k;
-        break;
-      }
-    }
-    if (threadIdx.x == 0) {
-      if (to == total) plan[4] = total;
-      plan[5] = total;
-    }
-  }
-  if (__syncthreads_or(bad ? 1 : 0)) {
-    // requests that are out of range: their rows that exist become zero
-    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-      if (!request_of(p, b).bad) continue;
-      if (threadIdx.x == 0) record_status(p.status, KTA_ERR_DEVICE_BOUNDS, SITE_REQUEST);
-      const long long a = max(p.offsets[b], 0), z = min(p.offsets[b + 1], p.rows);
-      const long long words = (z - a) * p.hq * (D / 2);
-      uint32_t* o = static_cast<uint32_t*>(p.out) + a * p.hq * (D / 2);
-      for (long long i = threadIdx.x; i < words; i += NUM_THREADS) o[i] = 0u;
-      for (long long i = threadIdx.x; i < (z - a) * p.hq; i += NUM_THREADS) p.lse[a * p.hq + i] = -INFINITY;
-    }
-  }
-  Walk w;
-  w.left = 0;
-  if (busy) {
-    w.b = plan[0];
-    w.kvh = plan[1];
-    w.i0 = plan[2];
-    w.left = plan[4] - plan[3];
-    w.turn = 0;
-    w.row = plan[6];
-    w.tokens = plan[7];
-    w.ctx = plan[8];
-    w.settle(p, member);
-  }
-  return w;
-}
-
-// What the join kernel needs, when a unit starts in the segment `w` and goes on behind the range.
-__device__ __forceinline__ Desc describe(const Params& p, const Walk& w, int rt, int tokens, int slot,
-                                         volatile int* plan) {
-  const Ranges r(p, plan[5]);
-  const int range = blockIdx.x / p.row_tiles;
-  const int end = plan[4] - w.left + w.tiles() * row_tiles_of(p, w.tokens);  // of the unit
-  Desc d = {};
-  d.count = r.owner_before(end) - range + 1;
-  d.slot = slot;
-  d.next = (range + 1) * p.row_tiles + rt;  // a range's first segment is row tile = member
-  d.row = w.row + rt * p.tok_tile;
-  d.tokens = tokens;
-  d.kvh = w.kvh;
-  return d;
-}
-
-// Producer warp of K or V: the range's tiles into a ring of STAGES, lane i loading page i.
+// One K or V producer's loads, into a ring of STAGES: lane i loads page i of a tile.
 template <int D, int STAGES>
-__device__ __forceinline__ void produce_kv(const Params& p, Walk w, int member, const CUtensorMap* map,
-                                           uint8_t* ring, uint64_t* full, uint64_t* empty,
-                                           volatile int* abort_flag) {
-  constexpr int GROUP = D / 64 * 1024, TILE = BN / 8 * GROUP;
-  const int lane = threadIdx.x & 31;
-  const int box = 1 << p.box_log2;
-  const int pages = BN >> p.box_log2;          // boxes of a tile
-  const int split = p.page_log2 - p.box_log2;  // log2 of boxes in a block
-  const int group_box = box / 8;
-  uint32_t n = 0;  // tiles so far
-  bool ok = true;
-  // this lane's block of tile i; only used a tile or two later, so that it stays in flight
-  auto block_of = [&](int i) -> int {
-    const int at = i * pages + lane;
-    if (lane >= pages || at << p.box_log2 >= w.len()) return 0;
-    return p.tables[w.b * p.table_stride + (at >> split)];
-  };
-  for (; w.left > 0 && ok; w.next(p), w.settle(p, member)) {
-    const int end = w.i0 + w.count(p);
-    int id = block_of(w.i0), id1 = w.i0 + 1 < end ? block_of(w.i0 + 1) : 0;
-    for (int i = w.i0; i < end; ++i, ++n) {
-      const int id2 = i + 2 < end ? block_of(i + 2) : 0;
-      const int st = static_cast<int>(n % STAGES);
-      if (!mbar_wait(&empty[st], ((n / STAGES) & 1u) ^ 1u, abort_flag, p.status, SITE_PROD_KV)) {
-        ok = false;
-        break;
-      }
-      const int held = min(pages, (w.len() - i * BN + box - 1) >> p.box_log2);
-      if (lane == 0) mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(held * group_box * GROUP));
-      __syncwarp();
-      if (lane < held) {
-        // the block's first (token, head) row; past the tensor, which reads as zeros, for no block
-        int first = p.num_blocks * p.hkv << p.page_log2;
-        if (id >= 0 && id < p.num_blocks) {
-          first = (id * p.hkv << p.page_log2) + w.kvh;
-        } else {
-          record_status(p.status, KTA_ERR_DEVICE_BOUNDS, SITE_BLOCK);
-        }
-        tma_load_5d(map, &full[st], ring + st * TILE + lane * group_box * GROUP, 0, 0, 0,
-                    ((i * pages + lane) & ((1 << split) - 1)) * group_box, first);
-      }
-      __syncwarp();
-      id = id1;
-      id1 = id2;
-    }
+struct Loader {
+  static constexpr int GROUP = D / 64 * 1024, TILE = BN / 8 * GROUP;
+  const CUtensorMap* map;
+  uint8_t* ring;
+  uint64_t* full;
+  uint64_t* empty;
+  volatile int* abort;
+  uint32_t n;   // tiles so far
+  int id, id1;  // this lane's blocks of the segment's next two tiles, in flight
+
+  // this lane's block of tile i
+  __device__ __forceinline__ int block_of(const Params& p, const Walk& w, int i) const {
+    const int at = i * (BN >> p.box_log2) + static_cast<int>(threadIdx.x & 31);
+    if (static_cast<int>(threadIdx.x & 31) >= BN >> p.box_log2 || at << p.box_log2 >= w.len()) return 0;
+    return p.tables[w.b * p.table_stride + (at >> (p.page_log2 - p.box_log2))];
   }
-  if (*abort_flag != 0 && lane == 0) {
-    // a role gave up: no copy may be in flight when the block ends (bounded like every wait)
+  __device__ __forceinline__ void start(const Params& p, const Walk& w, int end) {
+    id = block_of(p, w, w.i0);
+    id1 = w.i0 + 1 < end ? block_of(p, w, w.i0 + 1) : 0;
+  }
+  // Tile i of the segment that ends before tile `end`.
+  __device__ __forceinline__ bool load(const Params& p, const Walk& w, int i, int end) {
+    const int lane = threadIdx.x & 31;
+    const int box = 1 << p.box_log2, pages = BN >> p.box_log2, group_box = box / 8;
+    const int id2 = i + 2 < end ? block_of(p, w, i + 2) : 0;
+    const int st = static_cast<int>(n % STAGES);
+    if (!mbar_wait(&empty[st], ((n / STAGES) & 1u) ^ 1u, abort, p.status, SITE_PROD_KV)) return false;
+    ++n;
+    const int held = min(pages, (w.len() - i * BN + box - 1) >> p.box_log2);
+    if (lane == 0) mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(held * group_box * GROUP));
+    __syncwarp();
+    if (lane < held) {
+      // the block's first (token, head) row; past the tensor, which reads as zeros, for no block
+      int first = p.num_blocks * p.hkv << p.page_log2;
+      if (id >= 0 && id < p.num_blocks) {
+        first = (id * p.hkv << p.page_log2) + w.kvh;
+      } else {
+        record_status(p.status, KTA_ERR_DEVICE_BOUNDS, SITE_BLOCK);
+      }
+      const int boxes = 1 << (p.page_log2 - p.box_log2);  // of a block
+      tma_load_5d(map, &full[st], ring + st * TILE + lane * group_box * GROUP, 0, 0, 0,
+                  ((i * pages + lane) & (boxes - 1)) * group_box, first);
+    }
+    __syncwarp();
+    id = id1;
+    id1 = id2;
+    return true;
+  }
+  // After another role gave up: no copy may be in flight when the block ends (bounded like every
+  // wait).
+  __device__ __forceinline__ void drain(const Params& p) {
+    if (*abort == 0 || (threadIdx.x & 31) != 0) return;
     int none = 0;
     for (uint32_t k = n > STAGES ? n - STAGES : 0; k < n; ++k) {
       mbar_wait(&full[k % STAGES], (k / STAGES) & 1u, &none, p.status, SITE_PROD_KV);
     }
   }
+};
+
+// V producer warp.
+template <int D, int STAGES>
+__device__ __forceinline__ void produce_v(const Params& p, const Feed& feed, Loader<D, STAGES> ld) {
+  Walk w;
+  bool ok = true;
+  for (w.begin(p, feed); w.left > 0 && ok; w.next(p, feed)) {
+    const int end = w.i0 + w.count(p);
+    ld.start(p, w, end);
+    for (int i = w.i0; i < end && ok; ++i) ok = ld.load(p, w, i, end);
+    if (!ok) break;
+  }
+  ld.drain(p);
+}
+
+// K producer warp, which also takes the CTA's items: the first gridDim.x are the CTAs' own, the
+// others go to whoever comes first. It asks for the next one (an atomic, then a load) some tiles
+// before the range ends, so late that a CTA that is behind leaves it to others and early enough
+// that no tile waits for the answer.
+constexpr int ASK_AHEAD = 6, READ_AHEAD = 3;
+
+template <int D, int STAGES>
+__device__ __forceinline__ void produce_k(const Params& p, const Feed& feed, Loader<D, STAGES> ld) {
+  const int lane = threadIdx.x & 31;
+  const int shares = p.plan->shares, cuts = p.plan->cuts;
+  // the first round's items are the CTAs' own; where there are fewer shares, nothing else is taken
+  const int items = cuts > 1 ? shares * cuts * p.row_tiles : 0;
+  Walk w;
+  w.open(p);
+  uint32_t pushed = 0;
+  bool ok = true;
+  while (w.left > 0 && ok) {
+    int state = 0;  // of the next item: 1 asked for, 2 read
+    int item = 0, word = 0;
+    auto ask = [&]() {
+      item = lane == 0 ? static_cast<int>(gridDim.x + atomicAdd(&p.plan->next, 1u)) : 0;
+      state = 1;
+    };
+    auto read = [&]() {  // lane i gets word i of the entry
+      item = __shfl_sync(0xffffffffu, item, 0);
+      word = 0;
+      if (item >= 0 && item < items) {
+        const int at = item / p.row_tiles, cut = at / shares;
+        const int range = (at - cut * shares) * cuts + cut;
+        if (lane < RANGE_WORDS) word = reinterpret_cast<const int*>(p.ranges + range)[lane];
+        if (lane == offsetof(Range, id) / 4) word = range;
+        if (lane == offsetof(Range, member) / 4) word = item - at * p.row_tiles;
+      }
+      state = 2;
+    };
+    w.settle(p);
+    while (w.left > 0 && ok) {
+      const int tiles = w.count(p), end = w.i0 + tiles;
+      // tiles of the range from here on, as far as this segment tells
+      const bool last = w.left - tiles * row_tiles_of(p, w.tokens) <= 0;
+      ld.start(p, w, end);
+      for (int i = w.i0; i < end && ok; ++i) {
+        if (last && state == 0 && end - i <= ASK_AHEAD) ask();
+        if (last && state == 1 && end - i <= READ_AHEAD) read();
+        ok = ld.load(p, w, i, end);
+      }
+      if (!ok) break;
+      w.step(p);
+      w.settle(p);
+    }
+    if (!ok) break;
+    const uint32_t at = pushed & 1u;
+    if (!mbar_wait(&feed.empty[at], ((pushed >> 1) & 1u) ^ 1u, feed.abort, p.status, SITE_NEXT_FREE)) break;
+    // An item without rows for its member is passed over here: the MMA warp looks one segment ahead
+    // before it issues a segment's last product, and two such items would have it wait for an entry
+    // whose place in the ring the softmax warps only free behind that product.
+    do {
+      if (state == 0) ask();
+      if (state == 1) read();
+      if (lane < RANGE_WORDS) reinterpret_cast<volatile int*>(feed.ring + at)[lane] = word;
+      __syncwarp();
+      w.set(feed.ring[at]);
+      __syncwarp();
+      state = 0;
+      if (w.left <= 0) break;  // no more
+      Walk first = w;
+      first.settle(p);
+      if (first.left > 0) break;
+    } while (true);
+    if (lane == 0) mbar_arrive(&feed.full[at]);
+    ++pushed;
+  }
+  ld.drain(p);
 }
 
 // Producer warp of Q: each segment's query rows, [half][rows][128 B], into one of BUFS buffers.
 template <int D, int BUFS>
-__device__ __forceinline__ void produce_q(const Params& p, Walk w, int member, const CUtensorMap* map,
+__device__ __forceinline__ void produce_q(const Params& p, const Feed& feed, const CUtensorMap* map,
                                           uint8_t* base, int buf_bytes, int half_bytes, uint64_t* full,
-                                          uint64_t* empty, volatile int* abort_flag) {
+                                          uint64_t* empty) {
   if ((threadIdx.x & 31) == 0) {
+    Walk w;
     uint32_t n = 0;  // segments so far
-    for (; w.left > 0; w.next(p), w.settle(p, member), ++n) {
+    for (w.begin(p, feed, true); w.left > 0; w.next(p, feed, true)) {
       const uint32_t buf = n % BUFS;
-      if (!mbar_wait(&empty[buf], ((n / BUFS) & 1u) ^ 1u, abort_flag, p.status, SITE_PROD_Q)) break;
+      if (!mbar_wait(&empty[buf], ((n / BUFS) & 1u) ^ 1u, feed.abort, p.status, SITE_PROD_Q)) break;
+      ++n;
       mbar_arrive_expect_tx(&full[buf], static_cast<uint32_t>(p.box_tokens * p.group * D * 2));
 #pragma unroll
       for (int h = 0; h < D / 64; ++h) {
         tma_load_3d(map, &full[buf], base + buf * buf_bytes + h * half_bytes, h * 64, w.kvh * p.group,
-                    w.row + w.row_tile(p, member) * p.tok_tile);
+                    w.row + w.row_tile(p) * p.tok_tile);
       }
     }
-    if (*abort_flag != 0) {
+    if (*feed.abort != 0) {
       int none = 0;
       for (uint32_t k = n > BUFS ? n - BUFS : 0; k < n; ++k) {
         mbar_wait(&full[k % BUFS], (k / BUFS) & 1u, &none, p.status, SITE_PROD_Q);
@@ -432,6 +480,112 @@ __device__ __forceinline__ void produce_q(const Params& p, Walk w, int member, c
     }
   }
   __syncwarp();
+}
+
+// The slot of a part of a unit (a row tile's tiles of one (request, KV head)) that range `id` holds:
+// one for a unit from an earlier range, one for a unit that goes on in the next.
+__device__ __forceinline__ long long slot_of(const Params& p, int id, int rt, bool from_before) {
+  return 2LL * (static_cast<long long>(id) * p.row_tiles + rt) + (from_before ? 0 : 1);
+}
+
+// The WARPS warps that hold a segment's result, among themselves: sync() orders their earlier
+// writes (shared and global) before their later accesses, with the library's bounded wait.
+template <int WARPS>
+struct Team {
+  uint64_t* bar;  // count WARPS
+  volatile int* abort;
+  volatile int* flag;
+  unsigned int* status;
+  int warp;  // 0 .. WARPS - 1
+  uint32_t phase;
+  __device__ __forceinline__ bool sync() {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+    const bool ok = mbar_wait(bar, phase, abort, status, SITE_JOIN);
+    phase ^= 1u;
+    return ok;
+  }
+};
+
+// After a part's stores: counts it, and where it is the unit's last, joins the parts: M = max m,
+// O = sum 2^(m - M) O_part / sum 2^(m - M) l, in the order of the ranges whoever comes last. A warp
+// takes a row at a time (a lane four dimensions), the loads of four rows and parts together.
+template <bool BF16, int D, int WARPS>
+__device__ __forceinline__ bool join(const Params& p, Team<WARPS>& team, const Walk& w, int rt, int tokens) {
+  const Range* mine = p.ranges + w.id;
+  const int home = w.i0 > 0 ? mine->home : w.id;
+  const int span = p.ranges[home].span;
+  if (!team.sync()) return false;
+  if (team.warp == 0 && (threadIdx.x & 31) == 0) {
+    __threadfence();  // cumulative: the team's stores before this arrival
+    const unsigned int before = atomicAdd(p.arrived + home * p.row_tiles + rt, 1u);
+    __threadfence();
+    *team.flag = before + 1u == static_cast<unsigned int>(span) ? 1 : 0;
+  }
+  if (!team.sync()) return false;
+  if (*team.flag == 0) return true;
+  constexpr int U = 4, PARTS = 4;
+  const int rows = tokens * p.group, lane = threadIdx.x & 31;
+  for (int r0 = team.warp; r0 < rows; r0 += WARPS * U) {
+    float m[U], l[U];
+    float4 o[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      m[u] = -INFINITY;
+      l[u] = 0.f;
+      o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int c0 = 0; c0 < span; c0 += PARTS) {
+      float2 ml[PARTS][U];
+      float4 part[PARTS][U];
+#pragma unroll
+      for (int c = 0; c < PARTS; ++c) {
+        const long long slot = slot_of(p, home + c0 + c, rt, c0 + c > 0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int r = r0 + u * WARPS;
+          ml[c][u] = make_float2(-INFINITY, 0.f);
+          part[c][u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (r < rows && lane < D / 4 && c0 + c < span) {
+            ml[c][u] = __ldcg(p.part_ml + slot * p.row_cap + r);
+            part[c][u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (slot * p.row_cap + r) * D) + lane);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float top = m[u];
+#pragma unroll
+        for (int c = 0; c < PARTS; ++c) top = fmaxf(top, ml[c][u].x);
+        const float base = top == -INFINITY ? 0.f : top, a = ex2(m[u] - base);
+        m[u] = top;
+        l[u] *= a;
+        o[u] = make_float4(o[u].x * a, o[u].y * a, o[u].z * a, o[u].w * a);
+#pragma unroll
+        for (int c = 0; c < PARTS; ++c) {
+          const float b = ex2(ml[c][u].x - base);
+          l[u] = fmaf(ml[c][u].y, b, l[u]);
+          o[u].x = fmaf(part[c][u].x, b, o[u].x);
+          o[u].y = fmaf(part[c][u].y, b, o[u].y);
+          o[u].z = fmaf(part[c][u].z, b, o[u].z);
+          o[u].w = fmaf(part[c][u].w, b, o[u].w);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * WARPS;
+      if (r >= rows || lane >= D / 4) continue;
+      const float inv = l[u] == 0.f ? 0.f : 1.f / l[u];  // a row that sees nothing: O = 0
+      const int tok = r / p.group;
+      const long long at = static_cast<long long>(w.row + rt * p.tok_tile + tok) * p.hq + w.kvh * p.group +
+                           (r - tok * p.group);
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at * D + lane * 4) =
+          make_uint2(pack2<BF16>(o[u].x * inv, o[u].y * inv), pack2<BF16>(o[u].z * inv, o[u].w * inv));
+      if (lane == 0) p.lse[at] = l[u] == 0.f ? -INFINITY : (m[u] + log2f(l[u])) * 0.6931471805599453f;
+    }
+  }
+  return true;
 }
 
 // tree_narrow.cu; the tensor maps are encoded by the caller.

@@ -59,11 +59,13 @@ struct Narrow {
   static constexpr int OFF_WEIGHT = OFF_FACTOR + 2 * SOFTMAX_WARPS * N * 4;  // [N][warp]
   static constexpr int OFF_BAR = OFF_WEIGHT + SOFTMAX_WARPS * N * 4;
   // k_full, k_empty, v_full, v_empty, q_full, q_empty, s_full[2], p_full[2], p_empty[2], pv_done,
-  // corrected, ml_full, ml_empty, o_full, o_free
-  static constexpr int NUM_BARS = 2 * K_RING + 2 * V_RING + 2 * Q_BUFS + 12;
+  // corrected, ml_full, ml_empty, o_full, o_free, team, next_full[2], next_empty[2]
+  static constexpr int NUM_BARS = 2 * K_RING + 2 * V_RING + 2 * Q_BUFS + 17;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
-  // misc: tmem base, abort, non-finite drafts [2], plan [9], correction requests [2][4]
-  static constexpr int TOTAL = OFF_MISC + 96;
+  // misc: tmem base, abort, non-finite drafts [2], correction requests [2][4], the team's flag, the
+  // ring of ranges
+  static constexpr int OFF_NEXT = OFF_MISC + 56;
+  static constexpr int TOTAL = OFF_NEXT + 2 * sizeof(Range);
   static_assert(TOTAL <= 232448, "shared memory budget of one sm_100 CTA");
   // TMEM: S^T of buffer i at i N, O^T of warp w at (2 + w) N
   static constexpr uint32_t COL_O = 2 * N;
@@ -123,10 +125,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {
     pdl_wait();
-    if (threadIdx.x == 0) {
-      record_status(p.status, KTA_ERR_LAUNCH, SITE_SMEM);
-      p.desc[blockIdx.x] = Desc{};
-    }
+    if (threadIdx.x == 0) record_status(p.status, KTA_ERR_LAUNCH, SITE_SMEM);
     return;
   }
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
@@ -144,11 +143,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   uint64_t* ml_empty = ml_full + 1;           // ... and read, and the weights made of them
   uint64_t* o_full = ml_empty + 1;            // the segment's last PV
   uint64_t* o_free = o_full + 1;              // the epilogue has read O
+  uint64_t* team_bar = o_free + 1;
+  uint64_t* next_full = team_bar + 1;
+  uint64_t* next_empty = next_full + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   unsigned int* bad = reinterpret_cast<unsigned int*>(smem + L::OFF_MISC + 8);    // [2]
-  volatile int* plan = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 16);  // [9]
-  volatile int* ask = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 56);   // [buffer][warp]
+  volatile int* ask = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 16);   // [buffer][warp]
+  volatile int* team_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 48);
+  const Feed feed = {reinterpret_cast<Range*>(smem + L::OFF_NEXT), next_full, next_empty, abort_flag};
   float2* ml = reinterpret_cast<float2*>(smem + L::OFF_ML);
   float4* weights = reinterpret_cast<float4*>(smem + L::OFF_WEIGHT);  // [N] of the four warps
   volatile float* factors = reinterpret_cast<volatile float*>(smem + L::OFF_FACTOR);
@@ -179,6 +182,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     mbar_init(ml_empty, OUT_WARPS);
     mbar_init(o_full, 1);
     mbar_init(o_free, OUT_WARPS);
+    mbar_init(team_bar, OUT_WARPS);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&next_full[i], 1);
+      mbar_init(&next_empty[i], SOFTMAX_WARPS + OUT_WARPS + 3);  // and MMA, V, Q
+    }
     *abort_flag = 0;
     bad[0] = bad[1] = 0u;
     fence_barrier_init();
@@ -197,20 +205,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     *reinterpret_cast<uint4*>(smem + L::OFF_Q + i * 16) = make_uint4(0u, 0u, 0u, 0u);
   }
   fence_proxy_async_smem();
-  pdl_wait();  // the previous grid's writes (this launch's inputs) are visible from here on
-  // after the wait: the join kernel may be scheduled now, and waits for this grid itself
-  pdl_launch_dependents();
   tc_fence_before();
-  Walk w = plan_range<D>(p, 0, plan, reinterpret_cast<int*>(smem + L::OFF_ML));
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
+  pdl_launch_dependents();
+  pdl_wait();  // the plan, and the grids before it, are visible from here on
 
   if (warp == K_WARP) {
-    produce_kv<D, L::K_RING>(p, w, 0, &tmK, smem + L::OFF_K, k_full, k_empty, abort_flag);
+    produce_k(p, feed, Loader<D, L::K_RING>{&tmK, smem + L::OFF_K, k_full, k_empty, abort_flag, 0u, 0, 0});
   } else if (warp == V_WARP) {
-    produce_kv<D, L::V_RING>(p, w, 0, &tmV, smem + L::OFF_V, v_full, v_empty, abort_flag);
+    produce_v(p, feed, Loader<D, L::V_RING>{&tmV, smem + L::OFF_V, v_full, v_empty, abort_flag, 0u, 0, 0});
   } else if (warp == Q_WARP) {
-    produce_q<D, L::Q_BUFS>(p, w, 0, &tmQ, smem + L::OFF_Q, L::Q_BUF, L::Q_HALF, q_full, q_empty, abort_flag);
+    produce_q<D, L::Q_BUFS>(p, feed, &tmQ, smem + L::OFF_Q, L::Q_BUF, L::Q_HALF, q_full, q_empty);
   } else if (warp == MMA_WARP) {
     // ------------------------------ MMA issuer ------------------------------
     constexpr uint32_t FMT = BF16 ? 1u : 0u;
@@ -219,6 +226,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // 64 dimensions are one MN block: with a block stride of zero the lanes from 64 on repeat it
     constexpr uint32_t V_BLOCK = D == 128 ? 1024u : 0u;
     // w and j run one tile ahead of the PVs, into the next segment
+    Walk w;
+    w.begin(p, feed);
     int j = 0, tiles = w.left > 0 ? w.count(p) : 0;
     uint32_t segment = 0, o_phase = 0, corrections = 0;
     bool first_segment = true;
@@ -254,8 +263,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     for (uint32_t g = 0; more; ++g) {  // tile g: S and P buffer g & 1, their phase (g >> 1) & 1
       const bool first = j == 0, last = j + 1 == tiles;
       if (last) {
-        w.next(p);
-        w.settle(p, 0);
+        w.next(p, feed);
         j = 0;
         tiles = w.left > 0 ? w.count(p) : 0;
         ++segment;
@@ -309,7 +317,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                            ((((warp & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4);
     uint32_t g = 0, segment = 0;
     bool ok = true;
-    for (; w.left > 0 && ok; w.next(p), w.settle(p, 0), ++segment) {
+    Walk w;
+    for (w.begin(p, feed); w.left > 0 && ok; w.next(p, feed), ++segment) {
       const int tiles = w.count(p);
       // lane r (and r + 32): what row r sees, for the tiles that hold drafted tokens
       constexpr int PER = (N + 31) / 32;
@@ -468,8 +477,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const uint32_t t_o = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + L::COL_O;
     uint32_t g = 0, segment = 0;
     bool ok = true;
-    if (threadIdx.x == SOFTMAX_WARPS * 32) p.desc[blockIdx.x] = Desc{};  // no unit to join so far
-    for (bool first_part = true; w.left > 0 && ok; w.next(p), w.settle(p, 0), ++segment, first_part = false) {
+    Team<OUT_WARPS> team = {team_bar, abort_flag, team_flag, p.status, warp - SOFTMAX_WARPS, 0u};
+    Walk w;
+    for (w.begin(p, feed); w.left > 0 && ok; w.next(p, feed), ++segment) {
       const int tiles = w.count(p);
       for (int j = 0; j < tiles; ++j, ++g) {
         const uint32_t buf = g & 1u;
@@ -516,7 +526,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if (!mbar_wait(ml_full, segment & 1u, abort_flag, p.status, SITE_N_OUT_ML)) break;
       const bool whole = w.i0 == 0 && tiles == w.tiles();
       const int rows = w.tokens * p.group;
-      const int slot = 2 * static_cast<int>(blockIdx.x) + (first_part ? 0 : 1);
+      const long long slot = slot_of(p, w.id, 0, w.i0 > 0);
       // Lane r (and r + 32): the weights of row r's four states. The four warps write the same
       // values; none gets to the next segment's while another reads these (ml_empty).
 #pragma unroll
@@ -540,7 +550,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             p.lse[static_cast<long long>(w.row + tok) * p.hq + w.kvh * p.group + (r - tok * p.group)] =
                 l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
           } else {
-            p.part_ml[static_cast<long long>(slot) * p.row_cap + r] = make_float2(top, l);
+            p.part_ml[slot * p.row_cap + r] = make_float2(top, l);
           }
         }
         // a row that sees nothing: O = 0; a partial stays as it is, for the join to divide
@@ -552,7 +562,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       tc_fence_after();
       uint16_t* out = static_cast<uint16_t*>(p.out) +
                       (static_cast<long long>(w.row) * p.hq + w.kvh * p.group) * D + d;
-      float* part = p.part_o + static_cast<long long>(slot) * p.row_cap * D + d;
+      float* part = p.part_o + slot * p.row_cap * D + d;
       const int gap = (p.hq - p.group) * D;  // from a token's last head to the next token's first
       long long at = 0;
       int head = 0;
@@ -608,15 +618,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
         }
       }
-      if (threadIdx.x == SOFTMAX_WARPS * 32 && !whole && w.i0 == 0) {  // the unit starts here
-        p.desc[blockIdx.x] = describe(p, w, 0, w.tokens, slot, plan);
-      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(ml_empty);
         mbar_arrive(o_free);
       }
+      if (!whole && !join<BF16, D>(p, team, w, 0, w.tokens)) break;
     }
   }
 

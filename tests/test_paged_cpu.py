@@ -120,7 +120,7 @@ def test_tree_attn_argument_checks(dt):
                dict(stride=49), dict(q=4088)):
         assert call(**kw) == INVALID, kw
     for kw in (dict(new=65), dict(d=96), dict(hq=30), dict(hq=136), dict(block=4), dict(block=48),
-               dict(block=512), dict(B=65537), dict(width=1 << 27, stride=1 << 27),
+               dict(block=512), dict(B=2049), dict(width=1 << 27, stride=1 << 27),
                dict(blocks=1 << 24)):
         assert call(**kw) == UNSUPPORTED, kw
     for kw in (dict(ptr={0: ODD8}), dict(ptr={1: ODD8}), dict(ptr={2: ODD8}), dict(ptr={7: ODD8}),
