@@ -56,12 +56,10 @@ struct Layout {
   static constexpr int OFF_ML = OFF_V + RING * TILE;  // [warpgroup][128 rows] (maximum, sum)
   static constexpr int OFF_BAR = OFF_ML + 2 * BM * 8;
   // k_full[R], k_empty[R], v_full[R], v_empty[R], q_full, q_empty, s_full[2], p_full[2][2],
-  // pv_done[2], ml_full, ml_empty, o_done, o_free, team, next_full[2], next_empty[2]
-  static constexpr int NUM_BARS = 4 * RING + 19;
+  // pv_done[2], ml_full, ml_empty, o_done, o_free
+  static constexpr int NUM_BARS = 4 * RING + 14;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
-  // misc: tmem base, abort, non-finite drafts [2], the team's flag, the ring of ranges
-  static constexpr int OFF_NEXT = OFF_MISC + 24;
-  static constexpr int TOTAL = OFF_NEXT + 2 * sizeof(Range);
+  static constexpr int TOTAL = OFF_MISC + 16;  // tmem base, abort, non-finite drafts [2]
   static_assert(TOTAL <= 232448, "shared memory budget of one sm_100 CTA");
 };
 
@@ -151,7 +149,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {
     pdl_wait();
-    if (threadIdx.x == 0) record_status(p.status, KTA_ERR_LAUNCH, SITE_SMEM);
+    pdl_wait();
+    if (threadIdx.x == 0) {
+      record_status(p.status, KTA_ERR_LAUNCH, SITE_SMEM);
+      p.desc[blockIdx.x] = Desc{};
+    }
     return;
   }
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
@@ -167,15 +169,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   uint64_t* ml_empty = ml_full + 1;  // ... and read
   uint64_t* o_done = ml_empty + 1;   // the segment's last PV
   uint64_t* o_free = o_done + 1;     // the epilogue has read both O
-  uint64_t* team_bar = o_free + 1;
-  uint64_t* next_full = team_bar + 1;
-  uint64_t* next_empty = next_full + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   unsigned int* bad = reinterpret_cast<unsigned int*>(smem + L::OFF_MISC + 8);   // [2]
-  volatile int* team_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 16);
   float2* ml = reinterpret_cast<float2*>(smem + L::OFF_ML);
-  const Feed feed = {reinterpret_cast<Range*>(smem + L::OFF_NEXT), next_full, next_empty, abort_flag};
 
   const int warp = warp_id();
   const int lane = threadIdx.x & 31;
@@ -198,11 +195,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     mbar_init(ml_empty, SOFTMAX_WARPS);
     mbar_init(o_done, 1);
     mbar_init(o_free, SOFTMAX_WARPS);
-    mbar_init(team_bar, SOFTMAX_WARPS);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&next_full[i], 1);
-      mbar_init(&next_empty[i], SOFTMAX_WARPS + 3);  // and MMA, V, Q
-    }
     *abort_flag = 0;
     bad[0] = bad[1] = 0u;
     fence_barrier_init();
@@ -220,15 +212,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
+  pdl_wait();  // the previous grid's writes (this launch's inputs) are visible from here on
+  // after the wait: the join kernel may be scheduled now, and waits for this grid itself
   pdl_launch_dependents();
-  pdl_wait();  // the plan, and the grids before it, are visible from here on
+  Walk w = plan<D>(p, smem + L::OFF_K);
 
   if (warp == K_WARP) {
-    produce_k(p, feed, Loader<D, RING>{&tmK, smem + L::OFF_K, k_full, k_empty, abort_flag, 0u, 0, 0});
+    produce_kv(p, w, Loader<D, RING>{&tmK, smem + L::OFF_K, k_full, k_empty, abort_flag,
+                                     l2_policy_evict_normal(), 0u, 0, 0});
   } else if (warp == V_WARP) {
-    produce_v(p, feed, Loader<D, RING>{&tmV, smem + L::OFF_V, v_full, v_empty, abort_flag, 0u, 0, 0});
+    produce_kv(p, w, Loader<D, RING>{&tmV, smem + L::OFF_V, v_full, v_empty, abort_flag,
+                                     l2_policy_evict_normal(), 0u, 0, 0});
   } else if (warp == Q_WARP) {
-    produce_q<D, 1>(p, feed, &tmQ, smem + L::OFF_Q, 0, L::Q_HALF, q_full, q_empty);
+    produce_q<D, 1>(p, w, &tmQ, smem + L::OFF_Q, 0, L::Q_HALF, q_full, q_empty, abort_flag);
   } else if (warp == MMA_WARP) {
     // ------------------------------ MMA issuer ------------------------------
     constexpr uint32_t FMT = BF16 ? 1u : 0u;
@@ -237,8 +233,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // w and j run one tile ahead of the PVs, into the next segment: its first S is ready when the
     // softmax warps come from this one's epilogue.
     const uint64_t qdesc = sdesc_sw128(smem_u32(smem + L::OFF_Q), 16, 1024);
-    Walk w;
-    w.begin(p, feed);
     int j = 0, tiles = w.left > 0 ? w.count(p) : 0;
     uint32_t segment = 0, o_phase = 0;
     bool first_segment = true;
@@ -269,7 +263,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     for (uint32_t g = 0; more; ++g) {  // tile g: S buffer g & 1, its phase (g >> 1) & 1
       const bool first = j == 0, last = j + 1 == tiles;
       if (last) {
-        w.next(p, feed);
+        w.next(p);
         j = 0;
         tiles = w.left > 0 ? w.count(p) : 0;
         ++segment;
@@ -318,9 +312,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     uint32_t g = 0;  // tiles of keys so far
     uint32_t o_phase = 0;
     bool ok = true;
-    Team<SOFTMAX_WARPS> team = {team_bar, abort_flag, team_flag, p.status, warp, 0u};
-    Walk w;
-    for (w.begin(p, feed); w.left > 0 && ok; w.next(p, feed)) {
+    for (; w.left > 0 && ok; w.next(p)) {
       const int rt = w.row_tile(p);
       const int tokens = w.rows(p);
       const int rows = tokens * p.group;
@@ -380,7 +372,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       o_phase ^= 1u;
       tc_fence_after();
       const bool whole = w.i0 == 0 && tiles == w.tiles();
-      const long long slot = slot_of(p, w.id, rt, w.i0 > 0);
+      const long long slot = slot_of(p, static_cast<int>(blockIdx.x) / p.row_tiles, rt, w.i0 > 0);
       const int tok = row / p.group, head = row - tok * p.group;
       const int token = w.row + rt * p.tok_tile + tok;
       const int q_head = w.kvh * p.group + head;
@@ -456,7 +448,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free);
-      if (!whole && !join<BF16, D>(p, team, w, rt, tokens)) break;
     }
   }
 
@@ -468,163 +459,81 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   }
 }
 
-// The work list's ranges, by one CTA, and the counters at zero. The list is b-major over the tiles of
-// every (request, KV head), each counted once for every row tile of its request. Equal shares do not
-// end together (SMs reach between 0.88 and 1.08 of the median bandwidth: shares that took 179 us in
-// the median ended between 165 and 204), so a share is four ranges: the first SHARE percent for its
-// own CTA, and three smaller ones that go, the larger first, to whoever is done. Every share is cut,
-// rather than the end of the list, so that no unit falls into many more parts than the shares make.
-constexpr int PLAN_THREADS = 512;
-__device__ constexpr int SHARE[ROUNDS] = {0, 78, 90, 96};
-// tiles of a share from which on it is cut: its last range has then two or more
-constexpr int ROUNDS_FROM = 64;
+// Joins the parts of a unit that several shares hold: M = max m, O = sum 2^(m - M) O_part /
+// sum 2^(m - M) l, in the shares' order. Block (x, y): the unit that starts in share and row tile x,
+// part y of its elements; a thread takes four elements of a row, a warp the row's 128 back to back,
+// eight parts' loads at a time.
+constexpr int JOIN_THREADS = 128;
+constexpr int JOIN_PARTS = 8;
 
-template <int D>
-__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const Params p, int grid) {
-  __shared__ int first[MAX_BATCH + 1];  // the list's count before each request
-  __shared__ int row[MAX_BATCH], tokens[MAX_BATCH], ctx[MAX_BATCH];
-  __shared__ int warp_sum[PLAN_THREADS / 32];
+template <bool BF16, int D>
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Params p) {
   pdl_launch_dependents();
-  pdl_wait();  // the previous grid's writes (this launch's inputs) are visible from here on
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = (p.batch + PLAN_THREADS - 1) / PLAN_THREADS;
-  const int b0 = min(static_cast<int>(threadIdx.x) * per, p.batch), b1 = min(b0 + per, p.batch);
-  int mine = 0;
-  bool bad = false;
-  for (int b = b0; b < b1; ++b) {
-    const Request r = request_of(p, b);
-    bad |= r.bad;
-    row[b] = r.row;
-    tokens[b] = r.tokens;
-    ctx[b] = r.ctx;
-    const int n = tiles_of(r) * p.hkv * row_tiles_of(p, r.tokens);
-    first[b] = n;
-    mine += n;
-  }
-  int incl = mine;
+  pdl_wait();
+  const Desc d = p.desc[blockIdx.x];
+  if (d.span == 0) return;
+  const int share = static_cast<int>(blockIdx.x) / p.row_tiles;
+  const int rt = static_cast<int>(blockIdx.x) - share * p.row_tiles;
+  const int items = d.tokens * p.group * (D / 4);
+  for (int item = blockIdx.y * JOIN_THREADS + threadIdx.x; item < items;
+       item += gridDim.y * JOIN_THREADS) {
+    const int row = item / (D / 4), d4 = item % (D / 4);
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c0 = 0; c0 < d.span; c0 += JOIN_PARTS) {
+      float2 ml[JOIN_PARTS];
+      float4 part[JOIN_PARTS];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) warp_sum[warp] = incl;
-  const int any_bad = __syncthreads_or(bad ? 1 : 0);
-  int before = incl - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < PLAN_THREADS / 32; ++w) {
-    if (w < warp) before += warp_sum[w];
-    total += warp_sum[w];
-  }
-  for (int b = b0; b < b1; ++b) {
-    const int n = first[b];
-    first[b] = before;
-    before += n;
-  }
-  if (threadIdx.x == 0) first[p.batch] = total;
-  __syncthreads();
-
-  const int groups = grid / p.row_tiles;
-  const int cuts = total / groups >= ROUNDS_FROM * p.row_tiles ? ROUNDS : 1;  // ranges of a share
-  // a range is at least row_tiles long, so that it has a tile however many row tiles that counts
-  const int shares = total == 0 ? 0 : max(1, min(groups, total / p.row_tiles));
-  const int n = shares * cuts;
-  // Where range r starts, before it is rounded down to a tile: any growing function of r that all
-  // threads compute alike will do, so no exact division.
-  const double unit_share = static_cast<double>(total) / (100.0 * max(shares, 1));
-  auto start = [&](int r) -> int {
-    if (r >= n) return total;
-    // the exact value is a multiple of 1 / 16000: no rounding gets it past a whole number
-    return static_cast<int>(unit_share * (100 * (r / cuts) + (cuts > 1 ? SHARE[r % cuts] : 0)) + 1e-5);
-  };
-  // the last range that starts before position x > 0
-  auto range_before = [&](int x) -> int {
-    int r = min(n - 1, (static_cast<int>(x / (100.0 * unit_share)) + 1) * cuts);
-    while (r > 0 && start(r) >= x) --r;
-    return r;
-  };
-  struct Place {
-    int b, kvh, tile, at;  // the tile that holds the position, and its own position
-    int unit, unit_end;    // of its (request, KV head)
-    int k;
-  };
-  auto place_of = [&](int x) -> Place {
-    int lo = 0, hi = p.batch - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (first[mid + 1] > x) {
-        hi = mid;
-      } else {
-        lo = mid + 1;
+      for (int i = 0; i < JOIN_PARTS; ++i) {
+        const int c = c0 + i;
+        ml[i] = make_float2(-INFINITY, 0.f);
+        part[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < d.span) {
+          const long long at = slot_of(p, share + c, rt, c > 0) * p.row_cap + row;
+          ml[i] = __ldcg(p.part_ml + at);
+          part[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D) + d4);
+        }
       }
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < JOIN_PARTS; ++i) top = fmaxf(top, ml[i].x);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float keep = ex2(m - base);
+      l *= keep;
+      o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+#pragma unroll
+      for (int i = 0; i < JOIN_PARTS; ++i) {
+        const float wt = ex2(ml[i].x - base);
+        l = fmaf(wt, ml[i].y, l);
+        o.x = fmaf(wt, part[i].x, o.x);
+        o.y = fmaf(wt, part[i].y, o.y);
+        o.z = fmaf(wt, part[i].z, o.z);
+        o.w = fmaf(wt, part[i].w, o.w);
+      }
+      m = top;
     }
-    Place q;
-    q.b = lo;
-    q.k = row_tiles_of(p, tokens[lo]);
-    const int pair = (ctx[lo] + tokens[lo] + BN - 1) / BN * q.k, rel = x - first[lo];
-    q.kvh = rel / pair;
-    q.unit = first[lo] + q.kvh * pair;
-    q.unit_end = q.unit + pair;
-    q.tile = (x - q.unit) / q.k;
-    q.at = q.unit + q.tile * q.k;
-    return q;
-  };
-  for (int r = threadIdx.x; r < n; r += PLAN_THREADS) {
-    const Place a = place_of(start(r));
-    int end = total, last_unit = 0, last_end = total;  // of the range, and its last tile's unit
-    if (r + 1 < n) {
-      const Place z = place_of(start(r + 1));
-      end = z.at;
-      last_unit = z.unit;
-      last_end = z.at > z.unit ? z.unit_end : z.at;  // cut, or ending with the range
-    }
-    Range g = {};
-    g.b = a.b;
-    g.kvh = a.kvh;
-    g.i0 = a.tile;
-    g.left = end - a.at;
-    g.row = row[a.b];
-    g.tokens = tokens[a.b];
-    g.ctx = ctx[a.b];
-    // a tile lies in the last range whose start comes before the tile's end
-    g.home = a.tile > 0 ? range_before(a.unit + a.k) : r;
-    g.span = last_end > end && last_unit >= a.at ? range_before(last_end) - r + 1 : 0;
-    p.ranges[r] = g;
-  }
-  for (int i = threadIdx.x; i < n * p.row_tiles; i += PLAN_THREADS) p.arrived[i] = 0u;
-  if (threadIdx.x == 0) {
-    p.plan->shares = shares;
-    p.plan->cuts = cuts;
-    p.plan->next = 0u;
-  }
-  if (any_bad) {
-    // requests that are out of range: their rows that exist become zero
-    for (int b = 0; b < p.batch; ++b) {
-      if (!request_of(p, b).bad) continue;
-      if (threadIdx.x == 0) record_status(p.status, KTA_ERR_DEVICE_BOUNDS, SITE_REQUEST);
-      const long long a = max(p.offsets[b], 0), z = min(p.offsets[b + 1], p.rows);
-      const long long words = (z - a) * p.hq * (D / 2);
-      uint32_t* o = static_cast<uint32_t*>(p.out) + a * p.hq * (D / 2);
-      for (long long i = threadIdx.x; i < words; i += PLAN_THREADS) o[i] = 0u;
-      for (long long i = threadIdx.x; i < (z - a) * p.hq; i += PLAN_THREADS) p.lse[a * p.hq + i] = -INFINITY;
-    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: O = 0
+    const int tok = row / p.group;
+    const long long at =
+        static_cast<long long>(d.row + tok) * p.hq + d.kvh * p.group + (row - tok * p.group);
+    uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at * D + d4 * 4);
+    *dst = make_uint2(pack2<BF16>(o.x * inv, o.y * inv), pack2<BF16>(o.z * inv, o.w * inv));
+    if (d4 == 0) p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
   }
 }
 
-// Workspace: the plan, and (maximum, sum) and O of two partial units of every item.
+// Workspace: descriptors, and (maximum, sum) and O of two partial units of every share and row tile.
 struct Workspace {
-  size_t off_ranges, off_arrived, off_ml, off_o, total;
+  size_t off_ml, off_o, total;
   int row_cap;
   Workspace(long long max_new, long long group, long long D) {
     const long long tile = BM / group;
     row_cap = static_cast<int>((std::min(tile, max_new) * group + 7) / 8 * 8);
-    off_ranges = 256;
-    off_arrived = off_ranges + sizeof(Range) * MAX_ITEMS;
-    off_ml = off_arrived + sizeof(unsigned int) * MAX_ITEMS;
-    off_o = off_ml + sizeof(float2) * 2 * MAX_ITEMS * row_cap;
-    total = off_o + sizeof(float) * 2 * MAX_ITEMS * static_cast<size_t>(row_cap) * D;
+    off_ml = sizeof(Desc) * MAX_CTAS;
+    off_o = off_ml + sizeof(float2) * 2 * MAX_CTAS * row_cap;
+    total = off_o + sizeof(float) * 2 * MAX_CTAS * static_cast<size_t>(row_cap) * D;
   }
 };
-static_assert(sizeof(Range) % 16 == 0 && sizeof(Plan) <= 256, "workspace layout");
 
 bool sizes_ok(int64_t max_new, int64_t Hq, int64_t Hkv, int64_t D) {
   return max_new > 0 && max_new <= MAX_DRAFT && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 &&
@@ -656,14 +565,19 @@ int go(Params& p, const void* Q, const void* Kc, const void* Vc, int64_t q_token
   const int sms = std::min(current_sm_count(), MAX_CTAS);
   if (sms < p.row_tiles) return KTA_ERR_UNSUPPORTED;
   const int grid = sms / p.row_tiles * p.row_tiles;
-  s = launch_ex(plan_kernel<D>, dim3(1), dim3(PLAN_THREADS), 0, stream, 1, p, grid);
-  if (s != KTA_OK) return s;
   // One tcgen05 tile has 128 rows in wide_kernel however few are real, and up to 64 in the other.
-  if (p.box_tokens * p.group <= NARROW_ROWS) return launch_narrow<BF16, D>(p, tq, tk, tv, grid, stream);
-  auto kernel = wide_kernel<BF16, D>;
-  s = set_kernel_smem(reinterpret_cast<const void*>(kernel), L::TOTAL);
+  if (p.box_tokens * p.group <= NARROW_ROWS) {
+    s = launch_narrow<BF16, D>(p, tq, tk, tv, grid, stream);
+  } else {
+    auto kernel = wide_kernel<BF16, D>;
+    s = set_kernel_smem(reinterpret_cast<const void*>(kernel), L::TOTAL);
+    if (s != KTA_OK) return s;
+    s = launch_ex(kernel, dim3(grid), dim3(NUM_THREADS), L::TOTAL, stream, 1, tq, tk, tv, p);
+  }
   if (s != KTA_OK) return s;
-  return launch_ex(kernel, dim3(grid), dim3(NUM_THREADS), L::TOTAL, stream, 1, tq, tk, tv, p);
+  // a float4 for a thread, in at most two passes
+  const int parts = std::max(1, std::min(16, p.row_cap * (D / 4) / JOIN_THREADS));
+  return launch_ex(join_kernel<BF16, D>, dim3(grid, parts), dim3(JOIN_THREADS), 0, stream, 1, p);
 }
 
 template <bool BF16>
@@ -688,7 +602,7 @@ int launch(const void* Q, const void* Kc, const void* Vc, const void* tables, co
   }
   // and so does the work list: every request's tiles of keys, for each KV head and row tile
   const long long row_tiles = (max_new + BM / (Hq / Hkv) - 1) / (BM / (Hq / Hkv));
-  if (B * Hkv * row_tiles * ((max_blocks * block + BN - 1) / BN) > (1LL << 31) - 1) {
+  if (B * Hkv * row_tiles * ((max_blocks * block + BN - 1) / BN + SWITCH) > (1LL << 31) - 1) {
     return KTA_ERR_UNSUPPORTED;
   }
   if (q_token < Hq * D) return KTA_ERR_INVALID_ARG;
@@ -713,9 +627,7 @@ int launch(const void* Q, const void* Kc, const void* Vc, const void* tables, co
   p.lse = static_cast<float*>(LSE);
   p.v = Vc;
   uint8_t* base = static_cast<uint8_t*>(workspace);
-  p.plan = reinterpret_cast<Plan*>(base);
-  p.ranges = reinterpret_cast<Range*>(base + ws.off_ranges);
-  p.arrived = reinterpret_cast<unsigned int*>(base + ws.off_arrived);
+  p.desc = reinterpret_cast<Desc*>(base);
   p.part_ml = reinterpret_cast<float2*>(base + ws.off_ml);
   p.part_o = reinterpret_cast<float*>(base + ws.off_o);
   p.table_stride = table_stride;

@@ -3,8 +3,6 @@
 // of V tiles that end inside a page. The operator is described in tree.cu.
 #pragma once
 
-#include <cstddef>
-
 #include "kta_common.cuh"
 #include "kta_host.h"
 
@@ -22,8 +20,6 @@ constexpr int MAX_DRAFT = 64;         // bits of a row of the tree
 constexpr int MAX_GROUP = 16;
 constexpr int MAX_BATCH = 2048;       // the decode entries' limit
 constexpr int MAX_CTAS = 160;         // the workspace is sized for this many
-constexpr int ROUNDS = 4;             // ranges of a CTA, about
-constexpr int MAX_ITEMS = ROUNDS * MAX_CTAS;
 constexpr int NARROW_ROWS = 64;       // up to so many rows of a request: tree_narrow.cu
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units: the maximum moves when it grew > 2^8
 
@@ -43,29 +39,15 @@ enum : unsigned int {
   SITE_SMEM = 0x910,     // shared memory not aligned as declared
   SITE_REQUEST = 0x911,  // lengths or offsets out of range
   SITE_BLOCK = 0x912,    // a block id out of range
-  SITE_NEXT = 0x913,     // the next range's entry
-  SITE_NEXT_FREE = 0x914,
-  SITE_JOIN = 0x915,     // the warps that join a unit, among themselves
 };
 
-// The work list is the 128-key tiles of every (request, KV head), cut into ranges (plan_kernel).
-// An item is a range for one of its row_tiles members.
-struct Range {
-  int b, kvh, i0;        // the first tile
-  int left;              // its length in the work list's count, 0: no more ranges
-  int row, tokens, ctx;  // of request b
-  int home;              // i0 > 0: the range in which the first tile's unit starts
-  int span;              // ranges that hold a part of the unit that starts here and ends later; 0: none
-  int id, member;        // filled in where the item is taken
-  int pad;
-};
-constexpr int RANGE_WORDS = sizeof(Range) / 4;
-
-// Ranges stand in the order of the list, `cuts` of a share one after the other. Items are taken in
-// the order (cut, share, member).
-struct Plan {
-  int shares, cuts;
-  unsigned int next;  // items taken beyond the first gridDim.x
+// What the join kernel needs of a unit (a row tile's tiles of one (request, KV head)) that starts in a
+// share and ends in a later one.
+struct Desc {
+  int span;    // shares that hold a part of it; 0: none
+  int row;     // first query token
+  int tokens;
+  int kvh;
 };
 
 struct Params {
@@ -76,29 +58,29 @@ struct Params {
   void* out;               // [rows, Hq, D]
   float* lse;              // [rows, Hq]
   const void* v;           // the V cache, for drafted rows that are not finite
-  Plan* plan;
-  Range* ranges;           // [MAX_ITEMS]
-  unsigned int* arrived;   // [MAX_ITEMS] parts of the unit that starts in a range, for a row tile
-  float2* part_ml;         // [2 MAX_ITEMS][row_cap] (maximum, sum), log2 units
-  float* part_o;           // [2 MAX_ITEMS][row_cap][D], not normalised
+  Desc* desc;              // [MAX_CTAS] by share and row tile
+  float2* part_ml;         // [2 MAX_CTAS][row_cap] (maximum, sum), log2 units
+  float* part_o;           // [2 MAX_CTAS][row_cap][D], not normalised
   long long table_stride;
   int batch, rows, hq, hkv, group, max_new, max_blocks, num_blocks;
   int page_log2;           // tokens of a block
   int box_log2;            // tokens of a TMA box: min(block, 128)
   int tok_tile;            // drafted tokens of a row tile: 128 / group
   int box_tokens;          // tokens of the Q box: min(tok_tile, max_new)
-  int row_tiles;           // members of a range, a row tile each
+  int row_tiles;           // members of a share
   int row_cap;             // rows of a partial
   float scale_log2;        // softmax scale * log2(e)
   unsigned int* status;
 };
 
-__device__ __forceinline__ void tma_load_5d(const CUtensorMap* map, uint64_t* bar, void* dst, int32_t x,
-                                            int32_t y, int32_t z, int32_t w, int32_t v) {
+__device__ __forceinline__ void tma_load_5d_hint(const CUtensorMap* map, uint64_t* bar, void* dst, int32_t x,
+                                                 int32_t y, int32_t z, int32_t w, int32_t v,
+                                                 uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v),
+      "l"(policy)
       : "memory");
 }
 
@@ -130,29 +112,65 @@ __device__ __forceinline__ int row_tiles_of(const Params& p, int tokens) {
   return (tokens + p.tok_tile - 1) / p.tok_tile;
 }
 
-// A CTA's walk over the segments of its ranges: runs of count() tiles from i0 on of one (request,
-// KV head). Few fields, since the softmax warps keep it beside a row of S. Every warp walks by
-// itself; from the second range on it reads them from a two-entry ring in shared memory that the K
-// producer fills.
-struct Feed {
-  Range* ring;  // [2]
-  uint64_t* full;
-  uint64_t* empty;
-  volatile int* abort;
+// The work list: the 128-key tiles of every (request, KV head), b-major, each counted once for every
+// row tile of its request, in equal shares for `row_tiles` CTAs each (a share's members). A segment's
+// start and end cost a CTA about as much as SWITCH tiles (with equal numbers of tiles, shares of 3
+// segments had their keys at 183 us and shares of 10 at 215), so long lists count every unit with so
+// many more, ahead of its first tile.
+//
+// Shares that are taken as they are finished (the first 78 to 88 % to each CTA, the rest in one to
+// three rounds from a counter) measured 218 to 246 us where these take 202: what a cut unit costs is
+// more than the even end gives.
+constexpr int SWITCH = 3;
+constexpr int SWITCH_FROM = 16;  // tiles of a share from which on they are counted
+
+struct Shares {
+  int total, n, extra;  // extra: what a unit counts beyond its tiles
+  double length;
+  __device__ __forceinline__ Shares(const Params& p, int tiles, int units) {
+    const int groups = static_cast<int>(gridDim.x) / p.row_tiles;
+    extra = tiles / groups >= SWITCH_FROM * p.row_tiles ? SWITCH : 0;
+    total = tiles + extra * units;
+    // a share is at least (1 + extra) row_tiles long, so that it has a tile wherever it starts
+    n = total == 0 ? 0 : max(1, min(groups, total / ((1 + extra) * p.row_tiles)));
+    length = static_cast<double>(total) / max(n, 1);
+  }
+  // Where share r starts, before it is rounded down to a tile: any growing function of r that all
+  // threads compute alike will do, so no exact division. The exact value is a multiple of 1 / 160: no
+  // rounding gets it past a whole number.
+  __device__ __forceinline__ int start(int r) const {
+    return r >= n ? total : static_cast<int>(length * r + 1e-5);
+  }
+  // the last share that starts before position x > 0
+  __device__ __forceinline__ int before(int x) const {
+    int r = min(n - 1, static_cast<int>(x / length) + 1);
+    while (r > 0 && start(r) >= x) --r;
+    return r;
+  }
 };
 
+// The tile that holds a position of the list.
+struct Place {
+  int b, kvh, tile, at;  // at: its own position
+  int unit, unit_end;    // of its (request, KV head)
+  int k;                 // row tiles of the request
+  int row, tokens, ctx;
+};
+constexpr int PLAN_BYTES = 128 + 2 * static_cast<int>(sizeof(Place));  // shared memory of plan()
+
+// A CTA's walk over the segments of its share: runs of count() tiles from i0 on of one (request, KV
+// head). Few fields, since the softmax warps keep it beside a row of S; every warp walks by itself.
 struct Walk {
   int row, tokens, ctx;  // of the request
   int b, kvh, i0;
-  int left;              // of the range from here on, in the work list's count
-  int turn;              // the member that takes the segment's first row tile
-  int id, member;        // of the item
-  uint32_t taken;        // entries of the ring so far
+  int left;              // of the share from here on, in the list's count
+  int extra;             // what a unit counts beyond its tiles
+  int member, turn;      // this CTA in its share; the member with the segment's first row tile
 
   __device__ __forceinline__ int len() const { return ctx + tokens; }
   __device__ __forceinline__ int tiles() const { return (len() + BN - 1) / BN; }
   __device__ __forceinline__ int count(const Params& p) const {
-    return min(tiles() - i0, left / row_tiles_of(p, tokens));
+    return min(tiles() - i0, left / row_tiles_of(p, tokens) - (i0 == 0 ? extra : 0));
   }
   // The row tile of the request that falls to this member. Requests have between one and row_tiles
   // of them: the members take turns, so that each has its share over some segments.
@@ -164,29 +182,26 @@ struct Walk {
   __device__ __forceinline__ int rows(const Params& p) const {
     return max(0, min(tokens - row_tile(p) * p.tok_tile, p.tok_tile));
   }
-  __device__ __forceinline__ void set(const Range& r) {
-    b = r.b;
-    kvh = r.kvh;
-    i0 = r.i0;
-    left = r.left;
-    row = r.row;
-    tokens = r.tokens;
-    ctx = r.ctx;
-    id = r.id;
-    member = r.member;
-    turn = 0;
+  // To the next segment with rows for this member, this one included; left is 0 where there is none.
+  __device__ __forceinline__ void settle(const Params& p) {
+    while (left > 0 && rows(p) == 0) step(p);
   }
-  // Past this segment, inside the range.
+  __device__ __forceinline__ void next(const Params& p) {
+    step(p);
+    settle(p);
+  }
+
+ private:
   __device__ __forceinline__ void step(const Params& p) {
     const int k = row_tiles_of(p, tokens);
-    left -= count(p) * k;
+    left -= (count(p) + (i0 == 0 ? extra : 0)) * k;
     if (left <= 0) return;
     turn = (turn + k) % p.row_tiles;
     i0 = 0;
     if (++kvh == p.hkv) {
       kvh = 0;
       Request r;
-      do {  // tiles are left in the range, so a request with some follows
+      do {  // tiles are left in the share, so a request with some follows
         r = request_of(p, ++b);
       } while (tiles_of(r) == 0);
       row = r.row;
@@ -194,55 +209,146 @@ struct Walk {
       ctx = r.ctx;
     }
   }
-  // To the range's next segment, this one included, in which the member has rows; left is 0 where
-  // there is none.
-  __device__ __forceinline__ void settle(const Params& p) {
-    while (left > 0 && rows(p) == 0) step(p);
-  }
-  // The CTA's first item; left is 0 where it has none.
-  __device__ __forceinline__ void open(const Params& p) {
-    taken = 0;
-    left = 0;
-    const int share = static_cast<int>(blockIdx.x) / p.row_tiles;
-    if (share >= p.plan->shares) return;
-    const int range = share * p.plan->cuts;
-    Range r = p.ranges[range];
-    r.id = range;
-    r.member = static_cast<int>(blockIdx.x) - share * p.row_tiles;
-    set(r);
-  }
-  // The next range from the ring, by a warp (or by its lane 0 alone); left is 0 at the end.
-  __device__ __forceinline__ void take(const Params& p, const Feed& f, bool alone) {
-    left = 0;
-    const uint32_t at = taken & 1u;
-    if (!mbar_wait(&f.full[at], (taken >> 1) & 1u, f.abort, p.status, SITE_NEXT)) return;
-    set(f.ring[at]);
-    ++taken;
-    if (!alone) __syncwarp();
-    if (alone || (threadIdx.x & 31) == 0) mbar_arrive(&f.empty[at]);
-  }
-  // A first segment with rows, from the first item or a later one.
-  __device__ __forceinline__ void begin(const Params& p, const Feed& f, bool alone = false) {
-    open(p);
-    if (left <= 0) return;
-    settle(p);
-    while (left <= 0) {
-      take(p, f, alone);
-      if (left <= 0) return;
-      settle(p);
-    }
-  }
-  // The next segment with rows, in this range or the next ones.
-  __device__ __forceinline__ void next(const Params& p, const Feed& f, bool alone = false) {
-    step(p);
-    if (left > 0) settle(p);
-    while (left <= 0) {
-      take(p, f, alone);
-      if (left <= 0) return;
-      settle(p);
-    }
-  }
 };
+
+// The start of every CTA, after griddepcontrol.wait: places its share and returns the walk over it
+// (left is 0 where it has none); member 0 describes the unit that the share's end cuts. By all
+// threads, which it synchronises; `scratch` is PLAN_BYTES of shared memory. Rows of requests that
+// are out of range become zero.
+template <int D>
+__device__ __forceinline__ Walk plan(const Params& p, uint8_t* scratch) {
+  // The block tables into L2, a line for a thread: a producer that misses it waits behind the
+  // stream's own reads.
+  const int lines = (p.max_blocks * 4 + 127) / 128;
+  const long long line = static_cast<long long>(threadIdx.x) * gridDim.x + blockIdx.x;
+  if (line < static_cast<long long>(lines) * p.batch) {
+    const int b = static_cast<int>(line / lines);
+    const int32_t* at = p.tables + b * p.table_stride + (line - static_cast<long long>(b) * lines) * 32;
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+  }
+  int2* warp_sum = reinterpret_cast<int2*>(scratch);
+  volatile Place* places = reinterpret_cast<volatile Place*>(scratch + 128);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = (p.batch + NUM_THREADS - 1) / NUM_THREADS;  // requests of a thread
+  const int b0 = min(static_cast<int>(threadIdx.x) * per, p.batch), b1 = min(b0 + per, p.batch);
+  // a thread's first request is kept: with up to 384 of them nothing is loaded twice
+  Request kept = {};
+  int2 mine = make_int2(0, 0);  // tiles and units of the thread's requests, for each row tile
+  bool bad = false;
+  for (int b = b0; b < b1; ++b) {
+    const Request r = request_of(p, b);
+    if (b == b0) kept = r;
+    const int k = p.hkv * row_tiles_of(p, r.tokens), n = tiles_of(r);
+    mine.x += n * k;
+    mine.y += n > 0 ? k : 0;
+    bad |= r.bad;
+  }
+  int2 incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, incl.x, o), y = __shfl_up_sync(0xffffffffu, incl.y, o);
+    if (lane >= o) incl = make_int2(incl.x + x, incl.y + y);
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  const int any_bad = __syncthreads_or(bad ? 1 : 0);
+  int2 ahead = make_int2(incl.x - mine.x, incl.y - mine.y), all = make_int2(0, 0);
+#pragma unroll
+  for (int w = 0; w < NUM_THREADS / 32; ++w) {
+    const int2 v = warp_sum[w];
+    if (w < warp) ahead = make_int2(ahead.x + v.x, ahead.y + v.y);
+    all = make_int2(all.x + v.x, all.y + v.y);
+  }
+  const Shares sh(p, all.x, all.y);
+  const int before = ahead.x + sh.extra * ahead.y, sum = mine.x + sh.extra * mine.y;
+  const int share = static_cast<int>(blockIdx.x) / p.row_tiles;
+  const int member = static_cast<int>(blockIdx.x) - share * p.row_tiles;
+  if (share < sh.n && sum > 0) {
+    // the starts of the share and of the next one, by the threads that hold them
+    for (int q = 0; q < 2; ++q) {
+      const int at = sh.start(share + q);
+      if (at < before || at >= before + sum) continue;
+      int t = before;
+      for (int b = b0; b < b1; ++b) {
+        const Request r = b == b0 ? kept : request_of(p, b);
+        const int k = row_tiles_of(p, r.tokens);
+        const int pair = tiles_of(r) > 0 ? (tiles_of(r) + sh.extra) * k : 0;
+        if (at >= t + pair * p.hkv) {
+          t += pair * p.hkv;
+          continue;
+        }
+        volatile Place* z = places + q;
+        const int kvh = (at - t) / pair, unit = t + kvh * pair;
+        const int tile = max((at - unit) / k - sh.extra, 0);
+        z->b = b;
+        z->kvh = kvh;
+        z->tile = tile;
+        z->at = unit + (tile > 0 ? tile + sh.extra : 0) * k;
+        z->unit = unit;
+        z->unit_end = unit + pair;
+        z->k = k;
+        z->row = r.row;
+        z->tokens = r.tokens;
+        z->ctx = r.ctx;
+        break;
+      }
+    }
+  }
+  if (any_bad) {
+    // requests that are out of range: their rows that exist become zero
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+      if (!request_of(p, b).bad) continue;
+      if (threadIdx.x == 0) record_status(p.status, KTA_ERR_DEVICE_BOUNDS, SITE_REQUEST);
+      const long long a = max(p.offsets[b], 0), z = min(p.offsets[b + 1], p.rows);
+      const long long words = (z - a) * p.hq * (D / 2);
+      uint32_t* o = static_cast<uint32_t*>(p.out) + a * p.hq * (D / 2);
+      for (long long i = threadIdx.x; i < words; i += NUM_THREADS) o[i] = 0u;
+      for (long long i = threadIdx.x; i < (z - a) * p.hq; i += NUM_THREADS) p.lse[a * p.hq + i] = -INFINITY;
+    }
+  }
+  __syncthreads();
+  Walk w = {};
+  w.extra = sh.extra;
+  w.member = member;
+  int cut = 0;  // shares that hold a part of the unit that starts in this one and ends later
+  if (share < sh.n) {
+    int end = sh.total;
+    if (share + 1 < sh.n) {
+      end = places[1].at;
+      // the next share starts inside a unit, and that unit starts in this one
+      if (end > places[1].unit && places[1].unit >= places[0].at) {
+        cut = sh.before(places[1].unit_end) - share + 1;
+      }
+    }
+    w.b = places[0].b;
+    w.kvh = places[0].kvh;
+    w.i0 = places[0].tile;
+    w.left = end - places[0].at;
+    w.row = places[0].row;
+    w.tokens = places[0].tokens;
+    w.ctx = places[0].ctx;
+    w.settle(p);
+  }
+  if (member == 0 && threadIdx.x < p.row_tiles) {
+    const int rt = threadIdx.x;
+    Desc d = {};
+    if (cut > 0 && rt < places[1].k) {
+      d.span = cut;
+      d.row = places[1].row + rt * p.tok_tile;
+      d.tokens = min(places[1].tokens - rt * p.tok_tile, p.tok_tile);
+      d.kvh = places[1].kvh;
+    }
+    p.desc[blockIdx.x + rt] = d;
+  }
+  fence_proxy_async_smem();  // the scratch's use comes before TMA writes to the same memory
+  __syncthreads();
+  return w;
+}
+
+// The slot of a part of a unit that a share holds: one for a unit from an earlier share, one for a
+// unit that goes on in the next.
+__device__ __forceinline__ long long slot_of(const Params& p, int share, int rt, bool from_before) {
+  return 2LL * (share * p.row_tiles + rt) + (from_before ? 0 : 1);
+}
 
 // Bits lo .. lo + 31 of a row's view of the keys, lo = first key of the word less ctx: cached
 // keys (negative) are all seen, drafted ones by the row's bits.
@@ -312,6 +418,7 @@ struct Loader {
   uint64_t* full;
   uint64_t* empty;
   volatile int* abort;
+  uint64_t policy;
   uint32_t n;   // tiles so far
   int id, id1;  // this lane's blocks of the segment's next two tiles, in flight
 
@@ -345,8 +452,8 @@ struct Loader {
         record_status(p.status, KTA_ERR_DEVICE_BOUNDS, SITE_BLOCK);
       }
       const int boxes = 1 << (p.page_log2 - p.box_log2);  // of a block
-      tma_load_5d(map, &full[st], ring + st * TILE + lane * group_box * GROUP, 0, 0, 0,
-                  ((i * pages + lane) & (boxes - 1)) * group_box, first);
+      tma_load_5d_hint(map, &full[st], ring + st * TILE + lane * group_box * GROUP, 0, 0, 0,
+                       ((i * pages + lane) & (boxes - 1)) * group_box, first, policy);
     }
     __syncwarp();
     id = id1;
@@ -364,12 +471,11 @@ struct Loader {
   }
 };
 
-// V producer warp.
+// K or V producer warp.
 template <int D, int STAGES>
-__device__ __forceinline__ void produce_v(const Params& p, const Feed& feed, Loader<D, STAGES> ld) {
-  Walk w;
+__device__ __forceinline__ void produce_kv(const Params& p, Walk w, Loader<D, STAGES> ld) {
   bool ok = true;
-  for (w.begin(p, feed); w.left > 0 && ok; w.next(p, feed)) {
+  for (; w.left > 0 && ok; w.next(p)) {
     const int end = w.i0 + w.count(p);
     ld.start(p, w, end);
     for (int i = w.i0; i < end && ok; ++i) ok = ld.load(p, w, i, end);
@@ -378,92 +484,16 @@ __device__ __forceinline__ void produce_v(const Params& p, const Feed& feed, Loa
   ld.drain(p);
 }
 
-// K producer warp, which also takes the CTA's items: the first gridDim.x are the CTAs' own, the
-// others go to whoever comes first. It asks for the next one (an atomic, then a load) some tiles
-// before the range ends, so late that a CTA that is behind leaves it to others and early enough
-// that no tile waits for the answer.
-constexpr int ASK_AHEAD = 6, READ_AHEAD = 3;
-
-template <int D, int STAGES>
-__device__ __forceinline__ void produce_k(const Params& p, const Feed& feed, Loader<D, STAGES> ld) {
-  const int lane = threadIdx.x & 31;
-  const int shares = p.plan->shares, cuts = p.plan->cuts;
-  // the first round's items are the CTAs' own; where there are fewer shares, nothing else is taken
-  const int items = cuts > 1 ? shares * cuts * p.row_tiles : 0;
-  Walk w;
-  w.open(p);
-  uint32_t pushed = 0;
-  bool ok = true;
-  while (w.left > 0 && ok) {
-    int state = 0;  // of the next item: 1 asked for, 2 read
-    int item = 0, word = 0;
-    auto ask = [&]() {
-      item = lane == 0 ? static_cast<int>(gridDim.x + atomicAdd(&p.plan->next, 1u)) : 0;
-      state = 1;
-    };
-    auto read = [&]() {  // lane i gets word i of the entry
-      item = __shfl_sync(0xffffffffu, item, 0);
-      word = 0;
-      if (item >= 0 && item < items) {
-        const int at = item / p.row_tiles, cut = at / shares;
-        const int range = (at - cut * shares) * cuts + cut;
-        if (lane < RANGE_WORDS) word = reinterpret_cast<const int*>(p.ranges + range)[lane];
-        if (lane == offsetof(Range, id) / 4) word = range;
-        if (lane == offsetof(Range, member) / 4) word = item - at * p.row_tiles;
-      }
-      state = 2;
-    };
-    w.settle(p);
-    while (w.left > 0 && ok) {
-      const int tiles = w.count(p), end = w.i0 + tiles;
-      // tiles of the range from here on, as far as this segment tells
-      const bool last = w.left - tiles * row_tiles_of(p, w.tokens) <= 0;
-      ld.start(p, w, end);
-      for (int i = w.i0; i < end && ok; ++i) {
-        if (last && state == 0 && end - i <= ASK_AHEAD) ask();
-        if (last && state == 1 && end - i <= READ_AHEAD) read();
-        ok = ld.load(p, w, i, end);
-      }
-      if (!ok) break;
-      w.step(p);
-      w.settle(p);
-    }
-    if (!ok) break;
-    const uint32_t at = pushed & 1u;
-    if (!mbar_wait(&feed.empty[at], ((pushed >> 1) & 1u) ^ 1u, feed.abort, p.status, SITE_NEXT_FREE)) break;
-    // An item without rows for its member is passed over here: the MMA warp looks one segment ahead
-    // before it issues a segment's last product, and two such items would have it wait for an entry
-    // whose place in the ring the softmax warps only free behind that product.
-    do {
-      if (state == 0) ask();
-      if (state == 1) read();
-      if (lane < RANGE_WORDS) reinterpret_cast<volatile int*>(feed.ring + at)[lane] = word;
-      __syncwarp();
-      w.set(feed.ring[at]);
-      __syncwarp();
-      state = 0;
-      if (w.left <= 0) break;  // no more
-      Walk first = w;
-      first.settle(p);
-      if (first.left > 0) break;
-    } while (true);
-    if (lane == 0) mbar_arrive(&feed.full[at]);
-    ++pushed;
-  }
-  ld.drain(p);
-}
-
 // Producer warp of Q: each segment's query rows, [half][rows][128 B], into one of BUFS buffers.
 template <int D, int BUFS>
-__device__ __forceinline__ void produce_q(const Params& p, const Feed& feed, const CUtensorMap* map,
-                                          uint8_t* base, int buf_bytes, int half_bytes, uint64_t* full,
-                                          uint64_t* empty) {
+__device__ __forceinline__ void produce_q(const Params& p, Walk w, const CUtensorMap* map, uint8_t* base,
+                                          int buf_bytes, int half_bytes, uint64_t* full, uint64_t* empty,
+                                          volatile int* abort_flag) {
   if ((threadIdx.x & 31) == 0) {
-    Walk w;
     uint32_t n = 0;  // segments so far
-    for (w.begin(p, feed, true); w.left > 0; w.next(p, feed, true)) {
+    for (; w.left > 0; w.next(p)) {
       const uint32_t buf = n % BUFS;
-      if (!mbar_wait(&empty[buf], ((n / BUFS) & 1u) ^ 1u, feed.abort, p.status, SITE_PROD_Q)) break;
+      if (!mbar_wait(&empty[buf], ((n / BUFS) & 1u) ^ 1u, abort_flag, p.status, SITE_PROD_Q)) break;
       ++n;
       mbar_arrive_expect_tx(&full[buf], static_cast<uint32_t>(p.box_tokens * p.group * D * 2));
 #pragma unroll
@@ -472,7 +502,7 @@ __device__ __forceinline__ void produce_q(const Params& p, const Feed& feed, con
                     w.row + w.row_tile(p) * p.tok_tile);
       }
     }
-    if (*feed.abort != 0) {
+    if (*abort_flag != 0) {
       int none = 0;
       for (uint32_t k = n > BUFS ? n - BUFS : 0; k < n; ++k) {
         mbar_wait(&full[k % BUFS], (k / BUFS) & 1u, &none, p.status, SITE_PROD_Q);
@@ -480,112 +510,6 @@ __device__ __forceinline__ void produce_q(const Params& p, const Feed& feed, con
     }
   }
   __syncwarp();
-}
-
-// The slot of a part of a unit (a row tile's tiles of one (request, KV head)) that range `id` holds:
-// one for a unit from an earlier range, one for a unit that goes on in the next.
-__device__ __forceinline__ long long slot_of(const Params& p, int id, int rt, bool from_before) {
-  return 2LL * (static_cast<long long>(id) * p.row_tiles + rt) + (from_before ? 0 : 1);
-}
-
-// The WARPS warps that hold a segment's result, among themselves: sync() orders their earlier
-// writes (shared and global) before their later accesses, with the library's bounded wait.
-template <int WARPS>
-struct Team {
-  uint64_t* bar;  // count WARPS
-  volatile int* abort;
-  volatile int* flag;
-  unsigned int* status;
-  int warp;  // 0 .. WARPS - 1
-  uint32_t phase;
-  __device__ __forceinline__ bool sync() {
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-    const bool ok = mbar_wait(bar, phase, abort, status, SITE_JOIN);
-    phase ^= 1u;
-    return ok;
-  }
-};
-
-// After a part's stores: counts it, and where it is the unit's last, joins the parts: M = max m,
-// O = sum 2^(m - M) O_part / sum 2^(m - M) l, in the order of the ranges whoever comes last. A warp
-// takes a row at a time (a lane four dimensions), the loads of four rows and parts together.
-template <bool BF16, int D, int WARPS>
-__device__ __forceinline__ bool join(const Params& p, Team<WARPS>& team, const Walk& w, int rt, int tokens) {
-  const Range* mine = p.ranges + w.id;
-  const int home = w.i0 > 0 ? mine->home : w.id;
-  const int span = p.ranges[home].span;
-  if (!team.sync()) return false;
-  if (team.warp == 0 && (threadIdx.x & 31) == 0) {
-    __threadfence();  // cumulative: the team's stores before this arrival
-    const unsigned int before = atomicAdd(p.arrived + home * p.row_tiles + rt, 1u);
-    __threadfence();
-    *team.flag = before + 1u == static_cast<unsigned int>(span) ? 1 : 0;
-  }
-  if (!team.sync()) return false;
-  if (*team.flag == 0) return true;
-  constexpr int U = 4, PARTS = 4;
-  const int rows = tokens * p.group, lane = threadIdx.x & 31;
-  for (int r0 = team.warp; r0 < rows; r0 += WARPS * U) {
-    float m[U], l[U];
-    float4 o[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      m[u] = -INFINITY;
-      l[u] = 0.f;
-      o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    for (int c0 = 0; c0 < span; c0 += PARTS) {
-      float2 ml[PARTS][U];
-      float4 part[PARTS][U];
-#pragma unroll
-      for (int c = 0; c < PARTS; ++c) {
-        const long long slot = slot_of(p, home + c0 + c, rt, c0 + c > 0);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int r = r0 + u * WARPS;
-          ml[c][u] = make_float2(-INFINITY, 0.f);
-          part[c][u] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (r < rows && lane < D / 4 && c0 + c < span) {
-            ml[c][u] = __ldcg(p.part_ml + slot * p.row_cap + r);
-            part[c][u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (slot * p.row_cap + r) * D) + lane);
-          }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float top = m[u];
-#pragma unroll
-        for (int c = 0; c < PARTS; ++c) top = fmaxf(top, ml[c][u].x);
-        const float base = top == -INFINITY ? 0.f : top, a = ex2(m[u] - base);
-        m[u] = top;
-        l[u] *= a;
-        o[u] = make_float4(o[u].x * a, o[u].y * a, o[u].z * a, o[u].w * a);
-#pragma unroll
-        for (int c = 0; c < PARTS; ++c) {
-          const float b = ex2(ml[c][u].x - base);
-          l[u] = fmaf(ml[c][u].y, b, l[u]);
-          o[u].x = fmaf(part[c][u].x, b, o[u].x);
-          o[u].y = fmaf(part[c][u].y, b, o[u].y);
-          o[u].z = fmaf(part[c][u].z, b, o[u].z);
-          o[u].w = fmaf(part[c][u].w, b, o[u].w);
-        }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * WARPS;
-      if (r >= rows || lane >= D / 4) continue;
-      const float inv = l[u] == 0.f ? 0.f : 1.f / l[u];  // a row that sees nothing: O = 0
-      const int tok = r / p.group;
-      const long long at = static_cast<long long>(w.row + rt * p.tok_tile + tok) * p.hq + w.kvh * p.group +
-                           (r - tok * p.group);
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at * D + lane * 4) =
-          make_uint2(pack2<BF16>(o[u].x * inv, o[u].y * inv), pack2<BF16>(o[u].z * inv, o[u].w * inv));
-      if (lane == 0) p.lse[at] = l[u] == 0.f ? -INFINITY : (m[u] + log2f(l[u])) * 0.6931471805599453f;
-    }
-  }
-  return true;
 }
 
 // tree_narrow.cu; the tensor maps are encoded by the caller.

@@ -59,13 +59,11 @@ struct Narrow {
   static constexpr int OFF_WEIGHT = OFF_FACTOR + 2 * SOFTMAX_WARPS * N * 4;  // [N][warp]
   static constexpr int OFF_BAR = OFF_WEIGHT + SOFTMAX_WARPS * N * 4;
   // k_full, k_empty, v_full, v_empty, q_full, q_empty, s_full[2], p_full[2], p_empty[2], pv_done,
-  // corrected, ml_full, ml_empty, o_full, o_free, team, next_full[2], next_empty[2]
-  static constexpr int NUM_BARS = 2 * K_RING + 2 * V_RING + 2 * Q_BUFS + 17;
+  // corrected, ml_full, ml_empty, o_full, o_free
+  static constexpr int NUM_BARS = 2 * K_RING + 2 * V_RING + 2 * Q_BUFS + 12;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
-  // misc: tmem base, abort, non-finite drafts [2], correction requests [2][4], the team's flag, the
-  // ring of ranges
-  static constexpr int OFF_NEXT = OFF_MISC + 56;
-  static constexpr int TOTAL = OFF_NEXT + 2 * sizeof(Range);
+  // misc: tmem base, abort, non-finite drafts [2], correction requests [2][4]
+  static constexpr int TOTAL = OFF_MISC + 48;
   static_assert(TOTAL <= 232448, "shared memory budget of one sm_100 CTA");
   // TMEM: S^T of buffer i at i N, O^T of warp w at (2 + w) N
   static constexpr uint32_t COL_O = 2 * N;
@@ -125,7 +123,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {
     pdl_wait();
-    if (threadIdx.x == 0) record_status(p.status, KTA_ERR_LAUNCH, SITE_SMEM);
+    pdl_wait();
+    if (threadIdx.x == 0) {
+      record_status(p.status, KTA_ERR_LAUNCH, SITE_SMEM);
+      p.desc[blockIdx.x] = Desc{};
+    }
     return;
   }
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
@@ -143,15 +145,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   uint64_t* ml_empty = ml_full + 1;           // ... and read, and the weights made of them
   uint64_t* o_full = ml_empty + 1;            // the segment's last PV
   uint64_t* o_free = o_full + 1;              // the epilogue has read O
-  uint64_t* team_bar = o_free + 1;
-  uint64_t* next_full = team_bar + 1;
-  uint64_t* next_empty = next_full + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   unsigned int* bad = reinterpret_cast<unsigned int*>(smem + L::OFF_MISC + 8);    // [2]
   volatile int* ask = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 16);   // [buffer][warp]
-  volatile int* team_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 48);
-  const Feed feed = {reinterpret_cast<Range*>(smem + L::OFF_NEXT), next_full, next_empty, abort_flag};
   float2* ml = reinterpret_cast<float2*>(smem + L::OFF_ML);
   float4* weights = reinterpret_cast<float4*>(smem + L::OFF_WEIGHT);  // [N] of the four warps
   volatile float* factors = reinterpret_cast<volatile float*>(smem + L::OFF_FACTOR);
@@ -182,11 +179,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     mbar_init(ml_empty, OUT_WARPS);
     mbar_init(o_full, 1);
     mbar_init(o_free, OUT_WARPS);
-    mbar_init(team_bar, OUT_WARPS);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&next_full[i], 1);
-      mbar_init(&next_empty[i], SOFTMAX_WARPS + OUT_WARPS + 3);  // and MMA, V, Q
-    }
     *abort_flag = 0;
     bad[0] = bad[1] = 0u;
     fence_barrier_init();
@@ -209,15 +201,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
+  pdl_wait();  // the previous grid's writes (this launch's inputs) are visible from here on
+  // after the wait: the join kernel may be scheduled now, and waits for this grid itself
   pdl_launch_dependents();
-  pdl_wait();  // the plan, and the grids before it, are visible from here on
+  Walk w = plan<D>(p, smem + L::OFF_K);
 
+  // K and V are read once: evict first, and the tables, partials and code stay in L2
   if (warp == K_WARP) {
-    produce_k(p, feed, Loader<D, L::K_RING>{&tmK, smem + L::OFF_K, k_full, k_empty, abort_flag, 0u, 0, 0});
+    produce_kv(p, w, Loader<D, L::K_RING>{&tmK, smem + L::OFF_K, k_full, k_empty, abort_flag,
+                                          l2_policy_evict_first(), 0u, 0, 0});
   } else if (warp == V_WARP) {
-    produce_v(p, feed, Loader<D, L::V_RING>{&tmV, smem + L::OFF_V, v_full, v_empty, abort_flag, 0u, 0, 0});
+    produce_kv(p, w, Loader<D, L::V_RING>{&tmV, smem + L::OFF_V, v_full, v_empty, abort_flag,
+                                          l2_policy_evict_first(), 0u, 0, 0});
   } else if (warp == Q_WARP) {
-    produce_q<D, L::Q_BUFS>(p, feed, &tmQ, smem + L::OFF_Q, L::Q_BUF, L::Q_HALF, q_full, q_empty);
+    produce_q<D, L::Q_BUFS>(p, w, &tmQ, smem + L::OFF_Q, L::Q_BUF, L::Q_HALF, q_full, q_empty, abort_flag);
   } else if (warp == MMA_WARP) {
     // ------------------------------ MMA issuer ------------------------------
     constexpr uint32_t FMT = BF16 ? 1u : 0u;
@@ -226,8 +223,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // 64 dimensions are one MN block: with a block stride of zero the lanes from 64 on repeat it
     constexpr uint32_t V_BLOCK = D == 128 ? 1024u : 0u;
     // w and j run one tile ahead of the PVs, into the next segment
-    Walk w;
-    w.begin(p, feed);
     int j = 0, tiles = w.left > 0 ? w.count(p) : 0;
     uint32_t segment = 0, o_phase = 0, corrections = 0;
     bool first_segment = true;
@@ -263,7 +258,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     for (uint32_t g = 0; more; ++g) {  // tile g: S and P buffer g & 1, their phase (g >> 1) & 1
       const bool first = j == 0, last = j + 1 == tiles;
       if (last) {
-        w.next(p, feed);
+        w.next(p);
         j = 0;
         tiles = w.left > 0 ? w.count(p) : 0;
         ++segment;
@@ -317,8 +312,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                            ((((warp & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4);
     uint32_t g = 0, segment = 0;
     bool ok = true;
-    Walk w;
-    for (w.begin(p, feed); w.left > 0 && ok; w.next(p, feed), ++segment) {
+    for (; w.left > 0 && ok; w.next(p), ++segment) {
       const int tiles = w.count(p);
       // lane r (and r + 32): what row r sees, for the tiles that hold drafted tokens
       constexpr int PER = (N + 31) / 32;
@@ -477,9 +471,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const uint32_t t_o = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + L::COL_O;
     uint32_t g = 0, segment = 0;
     bool ok = true;
-    Team<OUT_WARPS> team = {team_bar, abort_flag, team_flag, p.status, warp - SOFTMAX_WARPS, 0u};
-    Walk w;
-    for (w.begin(p, feed); w.left > 0 && ok; w.next(p, feed), ++segment) {
+    for (; w.left > 0 && ok; w.next(p), ++segment) {
       const int tiles = w.count(p);
       for (int j = 0; j < tiles; ++j, ++g) {
         const uint32_t buf = g & 1u;
@@ -526,7 +518,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if (!mbar_wait(ml_full, segment & 1u, abort_flag, p.status, SITE_N_OUT_ML)) break;
       const bool whole = w.i0 == 0 && tiles == w.tiles();
       const int rows = w.tokens * p.group;
-      const long long slot = slot_of(p, w.id, 0, w.i0 > 0);
+      const long long slot = slot_of(p, blockIdx.x, 0, w.i0 > 0);
       // Lane r (and r + 32): the weights of row r's four states. The four warps write the same
       // values; none gets to the next segment's while another reads these (ml_empty).
 #pragma unroll
@@ -624,7 +616,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         mbar_arrive(ml_empty);
         mbar_arrive(o_free);
       }
-      if (!whole && !join<BF16, D>(p, team, w, 0, w.tokens)) break;
     }
   }
 
