@@ -325,7 +325,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       for (int j = 0; j < tiles; ++j, ++g) {
         const int k0 = (w.i0 + j) * BN;
         const bool masked = k0 + BN > w.ctx;
+        if (!mbar_wait(&s_full[g & 1u], (g >> 1) & 1u, abort_flag, p.status, SITE_SM_S)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
         if (masked) {
+          // behind S of this tile: the V tile before in this place has been waited for by then, so that
+          // the phase is the right one
           const int st = static_cast<int>(g % RING);
           if (!mbar_wait(&v_full[st], (g / RING) & 1u, abort_flag, p.status, SITE_SM_V)) {
             ok = false;
@@ -335,11 +342,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                            row, bad);
           fence_proxy_async_smem();
         }
-        if (!mbar_wait(&s_full[g & 1u], (g >> 1) & 1u, abort_flag, p.status, SITE_SM_S)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
         if (warp_on) {
           const uint32_t at = t_s + (g & 1u) * BN;
           uint32_t view[2];
@@ -429,12 +431,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               dst[i] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
             }
           } else if (live) {
-            float4* dst = reinterpret_cast<float4*>(
-                p.part_o + (slot * p.row_cap + row) * D + c);
+            float4* dst = reinterpret_cast<float4*>(p.part_o) +
+                          (slot * (D / 4) + c / 4) * p.row_cap + row;  // a warp's rows back to back
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                   __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+              dst[i * p.row_cap] =
+                  make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                              __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
             }
           }
         }
@@ -461,12 +464,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 
 // Joins the parts of a unit that several shares hold: M = max m, O = sum 2^(m - M) O_part /
 // sum 2^(m - M) l, in the shares' order. Block (x, y): the unit that starts in share and row tile x,
-// part y of its elements; a thread takes four elements of a row, a warp the row's 128 back to back,
-// eight parts' loads at a time.
+// part y of its elements; a thread takes four elements of a row, eight parts' loads at a time.
 constexpr int JOIN_THREADS = 128;
 constexpr int JOIN_PARTS = 8;
 
-template <bool BF16, int D>
+template <bool BF16, int D, bool WIDE>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Params p) {
   pdl_launch_dependents();
   pdl_wait();
@@ -474,10 +476,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Params p) {
   if (d.span == 0) return;
   const int share = static_cast<int>(blockIdx.x) / p.row_tiles;
   const int rt = static_cast<int>(blockIdx.x) - share * p.row_tiles;
-  const int items = d.tokens * p.group * (D / 4);
+  const int rows = d.tokens * p.group, items = rows * (D / 4);
   for (int item = blockIdx.y * JOIN_THREADS + threadIdx.x; item < items;
        item += gridDim.y * JOIN_THREADS) {
-    const int row = item / (D / 4), d4 = item % (D / 4);
+    // in the order that the part's kernel wrote, [d / 4][row] or [row][d / 4]
+    const int row = WIDE ? item % rows : item / (D / 4), d4 = WIDE ? item / rows : item % (D / 4);
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c0 = 0; c0 < d.span; c0 += JOIN_PARTS) {
@@ -489,9 +492,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Params p) {
         ml[i] = make_float2(-INFINITY, 0.f);
         part[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (c < d.span) {
-          const long long at = slot_of(p, share + c, rt, c > 0) * p.row_cap + row;
-          ml[i] = __ldcg(p.part_ml + at);
-          part[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D) + d4);
+          const long long slot = slot_of(p, share + c, rt, c > 0);
+          ml[i] = __ldcg(p.part_ml + slot * p.row_cap + row);
+          part[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o) +
+                           (WIDE ? (slot * (D / 4) + d4) * p.row_cap + row
+                                 : (slot * p.row_cap + row) * (D / 4) + d4));
         }
       }
       float top = m;
@@ -566,7 +571,8 @@ int go(Params& p, const void* Q, const void* Kc, const void* Vc, int64_t q_token
   if (sms < p.row_tiles) return KTA_ERR_UNSUPPORTED;
   const int grid = sms / p.row_tiles * p.row_tiles;
   // One tcgen05 tile has 128 rows in wide_kernel however few are real, and up to 64 in the other.
-  if (p.box_tokens * p.group <= NARROW_ROWS) {
+  const bool narrow = p.box_tokens * p.group <= NARROW_ROWS;
+  if (narrow) {
     s = launch_narrow<BF16, D>(p, tq, tk, tv, grid, stream);
   } else {
     auto kernel = wide_kernel<BF16, D>;
@@ -577,7 +583,8 @@ int go(Params& p, const void* Q, const void* Kc, const void* Vc, int64_t q_token
   if (s != KTA_OK) return s;
   // a float4 for a thread, in at most two passes
   const int parts = std::max(1, std::min(16, p.row_cap * (D / 4) / JOIN_THREADS));
-  return launch_ex(join_kernel<BF16, D>, dim3(grid, parts), dim3(JOIN_THREADS), 0, stream, 1, p);
+  auto join = narrow ? join_kernel<BF16, D, false> : join_kernel<BF16, D, true>;
+  return launch_ex(join, dim3(grid, parts), dim3(JOIN_THREADS), 0, stream, 1, p);
 }
 
 template <bool BF16>

@@ -60,7 +60,7 @@ struct Params {
   const void* v;           // the V cache, for drafted rows that are not finite
   Desc* desc;              // [MAX_CTAS] by share and row tile
   float2* part_ml;         // [2 MAX_CTAS][row_cap] (maximum, sum), log2 units
-  float* part_o;           // [2 MAX_CTAS][row_cap][D], not normalised
+  float* part_o;           // [2 MAX_CTAS][row_cap][D] or [D / 4][row_cap][4], not normalised
   long long table_stride;
   int batch, rows, hq, hkv, group, max_new, max_blocks, num_blocks;
   int page_log2;           // tokens of a block

@@ -335,7 +335,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const int k0 = (w.i0 + j) * BN;
         const uint32_t buf = g & 1u;
         const bool masked = k0 + BN > w.ctx;
+        if (!mbar_wait(&s_full[buf], (g >> 1) & 1u, abort_flag, p.status, SITE_SM_S)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
         if (masked) {
+          // behind S of this tile: the V tile before in this place has been waited for by then, so that
+          // the phase is the right one
           const int st = static_cast<int>(g % L::V_RING);
           if (!mbar_wait(&v_full[st], (g / L::V_RING) & 1u, abort_flag, p.status, SITE_SM_V)) {
             ok = false;
@@ -344,11 +351,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           clean_v<BF16, D>(smem + L::OFF_V + st * L::TILE, 0, BN, w.ctx - k0, w.len() - k0, k0 - w.ctx,
                            threadIdx.x, bad);
         }
-        if (!mbar_wait(&s_full[buf], (g >> 1) & 1u, abort_flag, p.status, SITE_SM_S)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
         uint32_t s[2][N / 2];  // [16 keys][4 c + e]
         tmem_ld_16x256b<N>(t_s + buf * N, s[0]);
         tmem_ld_16x256b<N>(t_s + buf * N + (16u << 16), s[1]);
