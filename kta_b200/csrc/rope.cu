@@ -15,6 +15,12 @@
 // for all heads (64 pairs against 32 or more heads), then rotate. A work item is two 16-byte
 // vectors half a region apart (rotated region or rest), which is the pair of the half layout and
 // in every layout keeps a warp's loads and stores contiguous.
+//
+// Small CTAs with two items to a thread in flight, and streaming loads and stores: 32768 x 32 heads
+// take 90.8 us (5920 GB/s; a plain copy of as many bytes 82.5) against 97.6 with 256 threads and
+// four items, 101 to 127 with 512 threads or without the streaming hints. Few tokens are latency:
+// there a thread has one item, and a token's heads are spread over several CTAs (512 tokens of 48
+// heads: 4.3 us with one item to a thread, 5.6 with 256 threads and four).
 #include <algorithm>
 #include <cmath>
 
@@ -24,8 +30,7 @@
 namespace kta {
 namespace rope {
 
-constexpr int THREADS = 256;
-constexpr int UNROLL = 4;        // items of a thread whose loads are in flight together
+constexpr int THREADS = 128;
 constexpr int MAX_D = 1024;
 constexpr int MAX_TOKENS = 8;    // tokens of a CTA
 constexpr int VEC = 8;           // 16-byte vectors of 16-bit elements
@@ -120,7 +125,9 @@ __device__ __forceinline__ Item<T> item_at(const Params& p, int token0, int toke
   return it;
 }
 
-template <typename T, bool INTER, bool CACHE>
+// UNROLL: items of a thread whose loads are in flight together. SPREAD: a token's items over
+// gridDim.y CTAs, one for a thread.
+template <typename T, bool INTER, bool CACHE, int UNROLL, bool SPREAD>
 __global__ void __launch_bounds__(THREADS) rope_kernel(const Params p) {
   extern __shared__ float2 turn[];  // [tokens of the CTA][rot / 2] scale * (cos, sin)
   __shared__ long long slot[MAX_TOKENS];
@@ -143,8 +150,9 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const Params p) {
   // The thread's first item, and how far the next one lies (in items, rows and tokens): steps
   // with a carry instead of two divisions for each item.
   const int d_piece = THREADS % p.items, d_row = THREADS / p.items;
-  int piece = threadIdx.x % p.items;
-  int row = threadIdx.x / p.items;
+  const int first = (SPREAD ? blockIdx.y * THREADS : 0) + threadIdx.x;
+  int piece = first % p.items;
+  int row = first / p.items;
   int token = row / p.rows;
   row -= token * p.rows;
   bool table = false;
@@ -220,7 +228,7 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const Params p) {
       __stcs(reinterpret_cast<uint4*>(it[u].dst), a);
       __stcs(reinterpret_cast<uint4*>(it[u].dst + it[u].second), b);
     }
-    if (token >= tokens) break;
+    if (SPREAD || token >= tokens) break;
   }
 }
 
@@ -260,6 +268,14 @@ int pointers_status(const void* positions, int64_t pos_bytes, const void* freqs)
   return KTA_OK;
 }
 
+template <typename T, bool CACHE, int UNROLL, bool SPREAD>
+int start(const Params& p, dim3 grid, bool interleaved, cudaStream_t stream) {
+  const size_t smem = static_cast<size_t>(p.per_cta) * (p.rot / 2) * sizeof(float2);
+  auto kernel = interleaved ? rope_kernel<T, true, CACHE, UNROLL, SPREAD>
+                            : rope_kernel<T, false, CACHE, UNROLL, SPREAD>;
+  return launch_ex(kernel, grid, dim3(THREADS), smem, stream, 1, p);
+}
+
 template <typename T, bool CACHE>
 int go(Params& p, int64_t D, bool interleaved, cudaStream_t stream) {
   int s = require_sm100();
@@ -272,21 +288,19 @@ int go(Params& p, int64_t D, bool interleaved, cudaStream_t stream) {
     p.items = p.rot_items;
   }
   p.status = device_status_ptr();
-  // Tokens of a CTA: enough items for a full round of loads of every thread, but never fewer
-  // CTAs than SMs.
   const long long per_token = static_cast<long long>(p.rows) * p.items;
+  const int sms = current_sm_count();
+  // One item to a thread while all of them are resident at once (2048 threads to an SM).
+  if (p.tokens * per_token <= 2048LL * sms) {
+    p.per_cta = 1;
+    const dim3 grid(p.tokens, static_cast<unsigned>((per_token + THREADS - 1) / THREADS));
+    return start<T, CACHE, 1, true>(p, grid, interleaved, stream);
+  }
+  // Tokens of a CTA: four items for a thread, but never fewer CTAs than fill the SMs.
   int per = 1;
-  while (per < MAX_TOKENS && per * per_token < THREADS * UNROLL &&
-         p.tokens / (2 * per) >= current_sm_count()) {
-    per *= 2;
-  }
+  while (per < MAX_TOKENS && per * per_token < 4 * THREADS && p.tokens / (2 * per) >= 8 * sms) per *= 2;
   p.per_cta = per;
-  const int grid = (p.tokens + per - 1) / per;
-  const size_t smem = static_cast<size_t>(per) * (p.rot / 2) * sizeof(float2);
-  if (interleaved) {
-    return launch_ex(rope_kernel<T, true, CACHE>, dim3(grid), dim3(THREADS), smem, stream, 1, p);
-  }
-  return launch_ex(rope_kernel<T, false, CACHE>, dim3(grid), dim3(THREADS), smem, stream, 1, p);
+  return start<T, CACHE, 2, false>(p, dim3((p.tokens + per - 1) / per), interleaved, stream);
 }
 
 template <typename T>

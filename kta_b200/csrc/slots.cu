@@ -24,7 +24,6 @@ namespace slots {
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_BATCH = 2048;  // the decode entries' limit; three int tables in shared memory
-constexpr int ROUND = 4;         // tokens of a thread whose loads are in flight together
 
 enum : unsigned int {
   SITE_LENGTH = 0x801,  // a length below zero or past the table
@@ -43,6 +42,7 @@ struct Params {
   int32_t* used;         // [1]
   long long table_stride;
   int batch, max_blocks, pool_size, block, rows;
+  int token_ctas;  // the others write table entries
   unsigned int* status;
 };
 
@@ -145,46 +145,35 @@ __global__ void __launch_bounds__(THREADS) slots_kernel(const Params p) {
     }
   }
 
-  // ---- the token map: rows strided by 256 in a round, stores of a warp back to back ----
-  const int step = static_cast<int>(gridDim.x) * THREADS;
-  for (long long base = blockIdx.x * THREADS + threadIdx.x; base < p.rows;
-       base += static_cast<long long>(step) * ROUND) {
-    int pos[ROUND], id[ROUND];
-#pragma unroll
-    for (int i = 0; i < ROUND; ++i) {
-      const long long row = base + static_cast<long long>(i) * step;
-      pos[i] = 0;
-      id[i] = -1;
+  if (static_cast<int>(blockIdx.x) < p.token_ctas) {
+    // ---- the token map ----
+    const int step = p.token_ctas * THREADS;
+    for (int row = blockIdx.x * THREADS + threadIdx.x; row < p.rows; row += step) {
+      int pos = 0, id = -1;
       if (row < total) {
-        const int b = owner_of(row0, p.batch, static_cast<int>(row));
+        const int b = owner_of(row0, p.batch, row);
         const int c = held_tokens[b];
-        pos[i] = c + (static_cast<int>(row) - row0[b]);
-        const int j = static_cast<int>(static_cast<unsigned>(pos[i]) / static_cast<unsigned>(p.block));
+        pos = c + (row - row0[b]);
+        const int j = static_cast<int>(static_cast<unsigned>(pos) / static_cast<unsigned>(p.block));
         const int held = blocks_of(c, p.block);
         if (j < held) {
-          id[i] = p.tables[b * p.table_stride + j];
+          id = p.tables[b * p.table_stride + j];
         } else {
           const long long k = static_cast<long long>(blk0[b]) + (j - held);
-          if (k < p.pool_size) id[i] = p.pool[k];
+          if (k < p.pool_size) id = p.pool[k];
         }
       }
+      p.slots[row] = id < 0 ? -1 : static_cast<long long>(id) * p.block + pos % p.block;
+      p.positions[row] = pos;
     }
-#pragma unroll
-    for (int i = 0; i < ROUND; ++i) {
-      const long long row = base + static_cast<long long>(i) * step;
-      if (row < p.rows) {
-        p.slots[row] =
-            id[i] < 0 ? -1 : static_cast<long long>(id[i]) * p.block + pos[i] % p.block;
-        p.positions[row] = pos[i];
-      }
+  } else {
+    // ---- the new table entries ----
+    const int step = (static_cast<int>(gridDim.x) - p.token_ctas) * THREADS;
+    for (long long k = (blockIdx.x - p.token_ctas) * THREADS + threadIdx.x; k < total_blks; k += step) {
+      const int b = owner_of(blk0, p.batch, static_cast<int>(k));
+      const long long j = blocks_of(held_tokens[b], p.block) + (k - blk0[b]);
+      p.tables[b * p.table_stride + j] = k < p.pool_size ? p.pool[k] : -1;
     }
-  }
-
-  // ---- the new table entries ----
-  for (long long k = blockIdx.x * THREADS + threadIdx.x; k < total_blks; k += step) {
-    const int b = owner_of(blk0, p.batch, static_cast<int>(k));
-    const long long j = blocks_of(held_tokens[b], p.block) + (k - blk0[b]);
-    p.tables[b * p.table_stride + j] = k < p.pool_size ? p.pool[k] : -1;
   }
 }
 
@@ -229,9 +218,12 @@ int launch(const void* ctx, const void* fresh, void* tables, const void* pool, v
   prm.block = static_cast<int>(block);
   prm.rows = static_cast<int>(rows);
   prm.status = device_status_ptr();
-  // one round of tokens per thread, at most two CTAs on each SM
-  const long long want = (rows + THREADS * ROUND - 1) / (THREADS * ROUND);
-  const int grid = static_cast<int>(std::max(1LL, std::min<long long>(want, 2LL * current_sm_count())));
+  // a token or an entry for a thread, at most eight CTAs on each SM
+  const auto ctas = [](long long n) {
+    return static_cast<int>(std::max(1LL, std::min((n + THREADS - 1) / THREADS, 4LL * current_sm_count())));
+  };
+  prm.token_ctas = ctas(rows);
+  const int grid = prm.token_ctas + ctas(rows / block + B);
   const size_t smem = (3 * static_cast<size_t>(B) + 2) * sizeof(int);
   return launch_ex(slots_kernel, dim3(grid), dim3(THREADS), smem, stream, 1, prm);
 }
