@@ -99,7 +99,7 @@ def _build_binding(verbose: bool) -> None:
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{INCLUDE}", f"-I{torch_dir}/include",
            f"-I{torch_dir}/include/torch/csrc/api/include", f"-I{cuda}/include",
            f"-I{sysconfig.get_paths()['include']}", str(src), "-o", str(BINDING),
-           f"-L{torch_dir}/lib", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           f"-L{torch_dir}/lib", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
            f"-L{PKG}", "-l:libkta_b200.so", "-Wl,-rpath,$ORIGIN"]
     version = (torch_dir / "version.py").read_bytes()
     h = hashlib.sha256(" ".join(cmd).encode() + src.read_bytes() + version)

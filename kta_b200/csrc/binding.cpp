@@ -11,6 +11,7 @@
 #include <string>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -75,7 +76,7 @@ class On {
     }
   }
   at::Tensor empty(at::IntArrayRef size, at::ScalarType type) const {
-    return at::empty(size, at::TensorOptions().dtype(type).device(device_));
+    return at::detail::empty_cuda(size, type, device_, c10::nullopt);  // without the dispatcher
   }
   void* stream() const { return c10::cuda::getCurrentCUDAStream(device_.index()).stream(); }
 
