@@ -216,6 +216,7 @@ int kta_rope_cache_bf16(const void* Q, const void* K, const void* V, const void*
  * drafted tokens, more tokens than its table's row holds) gets O = 0 and LSE = -inf; a block id
  * outside [0, num_blocks) reads as zeros. D = 64 or 128, Hq / Hkv <= 16, block_size a power of two
  * from 8 to 256, B <= 2048, max_blocks * block_size <= 2^30, num_blocks * block_size * Hkv < 2^31.
+ * Q, Kc, Vc 16-byte and O 32-byte aligned, q_token % 8 == 0.
  * `workspace`: kta_tree_attn_workspace_bytes(...) bytes, 16-byte aligned, of any contents; calls
  * that may run at the same time (two streams, two graphs) need one each. */
 size_t kta_tree_attn_workspace_bytes(int64_t max_new, int64_t Hq, int64_t Hkv, int64_t D);

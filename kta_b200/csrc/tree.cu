@@ -140,6 +140,13 @@ __device__ __forceinline__ bool softmax_step(uint32_t t_s, uint32_t t_o, const u
   return true;
 }
 
+// 32 bytes, 32-byte aligned
+__device__ __forceinline__ void st_global_v8(void* dst, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 template <bool BF16, int D>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -312,14 +319,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     uint32_t g = 0;  // tiles of keys so far
     uint32_t o_phase = 0;
     bool ok = true;
-    for (; w.left > 0 && ok; w.next(p)) {
+    // what this thread's row of a segment sees
+    auto bits_at = [&](const Walk& v) -> uint64_t {
+      if (v.left <= 0 || row >= v.rows(p) * p.group) return 0ull;
+      return bits_of(p, v.row, v.row_tile(p) * p.tok_tile + row / p.group, v.tokens);
+    };
+    uint64_t bits = bits_at(w);
+    while (w.left > 0 && ok) {
       const int rt = w.row_tile(p);
       const int tokens = w.rows(p);
       const int rows = tokens * p.group;
       const bool live = row < rows;
       const bool warp_on = quarter * 32 < rows;
-      uint64_t bits = 0;
-      if (live) bits = bits_of(p, w.row, rt * p.tok_tile + row / p.group, w.tokens);
       const int tiles = w.count(p);
       float m_used = -INFINITY, lsum = 0.f;
       for (int j = 0; j < tiles; ++j, ++g) {
@@ -362,6 +373,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       }
       if (!ok) break;
       // ---- epilogue: the two warpgroups' states become one, each for half of D ----
+      Walk following = w;  // its loads come behind the last products
+      following.next(p);
+      const uint64_t following_bits = bits_at(following);
       if (!mbar_wait(ml_empty, o_phase ^ 1u, abort_flag, p.status, SITE_SM_ML)) break;
       ml[wg * BM + row] = make_float2(m_used, lsum);
       __syncwarp();
@@ -419,16 +433,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             }
           }
           if (live && whole) {
-            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) +
-                                                  (static_cast<long long>(token) * p.hq + q_head) * D + c);
+            uint16_t* dst = static_cast<uint16_t*>(p.out) +
+                            (static_cast<long long>(token) * p.hq + q_head) * D + c;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t pk[4];
+            for (int i = 0; i < 2; ++i) {  // a sector at a time
+              uint32_t pk[8];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                pk[e] = pack2<BF16>(__uint_as_float(o[8 * i + 2 * e]), __uint_as_float(o[8 * i + 2 * e + 1]));
+              for (int e = 0; e < 8; ++e) {
+                pk[e] = pack2<BF16>(__uint_as_float(o[16 * i + 2 * e]), __uint_as_float(o[16 * i + 2 * e + 1]));
               }
-              dst[i] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+              st_global_v8(dst + 16 * i, pk);
             }
           } else if (live) {
             float4* dst = reinterpret_cast<float4*>(p.part_o) +
@@ -451,6 +465,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free);
+      w = following;
+      bits = following_bits;
     }
   }
 
@@ -613,7 +629,8 @@ int launch(const void* Q, const void* Kc, const void* Vc, const void* tables, co
     return KTA_ERR_UNSUPPORTED;
   }
   if (q_token < Hq * D) return KTA_ERR_INVALID_ARG;
-  if (q_token % 8 != 0 || !aligned16(Q) || !aligned16(Kc) || !aligned16(Vc) || !aligned16(O)) {
+  if (q_token % 8 != 0 || !aligned16(Q) || !aligned16(Kc) || !aligned16(Vc) ||
+      (reinterpret_cast<uintptr_t>(O) & 31) != 0) {  // O is written a sector at a time
     return KTA_ERR_ALIGN;
   }
   for (const void* q : {tables, ctx, offsets, static_cast<const void*>(LSE)}) {

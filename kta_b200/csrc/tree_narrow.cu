@@ -312,7 +312,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                            ((((warp & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4);
     uint32_t g = 0, segment = 0;
     bool ok = true;
-    for (; w.left > 0 && ok; w.next(p), ++segment) {
+    Walk following;
+    for (; w.left > 0 && ok; w = following, ++segment) {
       const int tiles = w.count(p);
       // lane r (and r + 32): what row r sees, for the tiles that hold drafted tokens
       constexpr int PER = (N + 31) / 32;
@@ -335,6 +336,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const int k0 = (w.i0 + j) * BN;
         const uint32_t buf = g & 1u;
         const bool masked = k0 + BN > w.ctx;
+        if (j + 1 == tiles) {  // the next segment's request, while this one's last tile comes
+          following = w;
+          following.next(p);
+        }
         if (!mbar_wait(&s_full[buf], (g >> 1) & 1u, abort_flag, p.status, SITE_SM_S)) {
           ok = false;
           break;

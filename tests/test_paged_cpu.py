@@ -123,7 +123,7 @@ def test_tree_attn_argument_checks(dt):
                dict(block=512), dict(B=2049), dict(width=1 << 27, stride=1 << 27),
                dict(blocks=1 << 24)):
         assert call(**kw) == UNSUPPORTED, kw
-    for kw in (dict(ptr={0: ODD8}), dict(ptr={1: ODD8}), dict(ptr={2: ODD8}), dict(ptr={7: ODD8}),
+    for kw in (dict(ptr={0: ODD8}), dict(ptr={1: ODD8}), dict(ptr={2: ODD8}), dict(ptr={7: ODD8}), dict(ptr={7: A + 16}),
                dict(ptr={3: ODD2}), dict(ptr={4: ODD2}), dict(ptr={5: ODD2}), dict(ptr={6: ODD4}),
                dict(ptr={8: ODD2}), dict(q=4100)):
         assert call(**kw) == ALIGN, kw
