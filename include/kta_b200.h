@@ -160,8 +160,8 @@ int kta_decode_gqa_bf16_noalloc(const void* Q, const void* Kc, const void* Vc,
  * KTA_ERR_DEVICE_BOUNDS: a request with a negative length or more tokens than its table's row
  * holds is listed without new tokens; blocks past num_free are entered as -1, and their tokens'
  * slots are -1; tokens past max_tokens are cut off (offsets end at max_tokens). B <= 2048,
- * max_blocks * block_size < 2^31, max_tokens <= 2^30. The free list must not overlap the
- * tables. */
+ * max_blocks * block_size < 2^31, max_tokens <= 2^30. No output overlaps an input or another
+ * output. */
 int kta_cache_slots(const void* context_lens, const void* new_lens, void* block_tables,
                     const void* free_blocks, void* slots, void* positions, void* offsets, void* used,
                     int64_t B, int64_t max_blocks, int64_t table_stride, int64_t num_free,
@@ -216,7 +216,7 @@ int kta_rope_cache_bf16(const void* Q, const void* K, const void* V, const void*
  * drafted tokens, more tokens than its table's row holds) gets O = 0 and LSE = -inf; a block id
  * outside [0, num_blocks) reads as zeros. D = 64 or 128, Hq / Hkv <= 16, block_size a power of two
  * from 8 to 256, B <= 2048, max_blocks * block_size <= 2^30, num_blocks * block_size * Hkv < 2^31.
- * Q, Kc, Vc 16-byte and O 32-byte aligned, q_token % 8 == 0.
+ * Q, Kc, Vc 16-byte and O 32-byte aligned, q_token % 8 == 0; O overlaps no input (Q: refused).
  * `workspace`: kta_tree_attn_workspace_bytes(...) bytes, 16-byte aligned, of any contents; calls
  * that may run at the same time (two streams, two graphs) need one each. */
 size_t kta_tree_attn_workspace_bytes(int64_t max_new, int64_t Hq, int64_t Hkv, int64_t D);

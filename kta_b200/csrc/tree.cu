@@ -637,6 +637,10 @@ int launch(const void* Q, const void* Kc, const void* Vc, const void* tables, co
     if (reinterpret_cast<uintptr_t>(q) & 3) return KTA_ERR_ALIGN;
   }
   if (reinterpret_cast<uintptr_t>(tree) & 7) return KTA_ERR_ALIGN;
+  // a CTA may still read rows of Q where another has written O
+  const uintptr_t q0 = reinterpret_cast<uintptr_t>(Q), o0 = reinterpret_cast<uintptr_t>(O);
+  const uintptr_t q1 = q0 + 2 * static_cast<uintptr_t>((tokens - 1) * q_token + Hq * D);
+  if (o0 < q1 && q0 < o0 + 2 * static_cast<uintptr_t>(tokens * Hq * D)) return KTA_ERR_INVALID_ARG;
   const long long group = Hq / Hkv;
   const Workspace ws(max_new, group, D);
   if (workspace == nullptr || ws_bytes < ws.total || !aligned16(workspace)) return KTA_ERR_WORKSPACE;

@@ -355,8 +355,9 @@ def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: tor
                out: torch.Tensor | None = None) -> torch.Tensor:
     """Rotary positions of a step's Q [tokens, Hq, D] and K [tokens, Hkv, D] (``rope``), with the
     rotated K and the V written to ``slots`` (int64 [tokens], ``cache_slots``) of the paged caches
-    [num_blocks, block_size, Hkv, D]; a negative slot writes nothing. Returns the rotated Q
-    (``out`` may be Q itself). Q, K and V may be slices of one fused tensor."""
+    [num_blocks, block_size, Hkv, D]; a negative slot writes nothing, and one that occurs twice
+    holds either token's values. Returns the rotated Q (``out`` may be Q itself). Q, K and V may be
+    slices of one fused tensor."""
     return (_native or _bind()).rope_cache(q, k, v, positions, slots, freqs, k_cache, v_cache,
                                            interleaved, scale, out)
 
@@ -380,8 +381,10 @@ def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     with attention over other keys); a row that sees nothing has O = 0 and LSE = -inf, rows of no
     request are left as they were.
 
-    ``workspace`` (uint8, ``tree_attn_workspace_bytes``, any contents) is allocated on the current
-    stream where none is given; calls that may run at the same time need one each."""
+    Q's heads are contiguous, its tokens at any stride (a slice of a fused tensor will do); ``out``
+    and ``lse`` are contiguous and overlap no input. ``workspace`` (uint8,
+    ``tree_attn_workspace_bytes``, any contents) is allocated on the current stream where none is
+    given; calls that may run at the same time need one each."""
     return (_native or _bind()).tree_attn(q, k_cache, v_cache, block_tables, context_lens, offsets,
                                           max_new, tree, scale, out, lse, workspace)
 

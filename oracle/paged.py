@@ -88,3 +88,15 @@ def attention(q, k, v, sight, scale: float):
         pv[i], tiny[i] = (e / total) @ np.abs(vi), np.abs(vi).sum(0) / total
         smax[i], dot[i] = np.abs(s).max(), scale * (np.abs(ki) @ np.abs(q[i])).max()
     return o, lse, pv, tiny, smax, dot
+
+
+def attention_bounds(sight, eps: float, sub: float, o, lse, pv, tiny, smax, dot):
+    """How far O [R, D] and LSE [R] of the 16-bit kernel may be from attention()'s results (the rest
+    of the arguments). eps: half a step of the storage type; sub: half a subnormal step of the
+    weights' type. In fp32 a score of D products is off by D 2^-24 sum |q||k| scale, the exponent by
+    roundings of |s|, 2^x by 2 ulp: d32 relative, on a weight and again on the sum."""
+    D, keys = o.shape[1], sight.sum(1)
+    d32 = D * 2.0 ** -24 * dot + 6 * smax * 2.0 ** -24 + 2.0 ** -22
+    f = pv * (eps + 2 * d32 + keys * 2.0 ** -24)[:, None] + sub * tiny
+    z = np.where(keys == 0, 0, lse)
+    return f + eps * (np.abs(o) + f) + 2.0 ** -25, d32 + (keys + 2 * np.abs(z)) * 2.0 ** -24

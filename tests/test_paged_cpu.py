@@ -109,6 +109,7 @@ def test_tree_attn_argument_checks(dt):
     def call(ptr=(), n=32, B=4, hq=32, hkv=8, d=128, q=4096, blocks=100, block=16, width=50, stride=50,
              new=8, scale=0.1, ws=A, size=full):
         p = [A] * 9  # Q, Kc, Vc, tables, ctx, offsets, tree, O, LSE
+        p[7] = A + (1 << 20)
         for i, v in dict(ptr).items():
             p[i] = v
         return f(*p, n, B, hq, hkv, d, q, blocks, block, width, stride, new, scale, ws, size, None)
@@ -123,15 +124,22 @@ def test_tree_attn_argument_checks(dt):
                dict(block=512), dict(B=2049), dict(width=1 << 27, stride=1 << 27),
                dict(blocks=1 << 24)):
         assert call(**kw) == UNSUPPORTED, kw
-    for kw in (dict(ptr={0: ODD8}), dict(ptr={1: ODD8}), dict(ptr={2: ODD8}), dict(ptr={7: ODD8}), dict(ptr={7: A + 16}),
+    for kw in (dict(ptr={0: ODD8}), dict(ptr={1: ODD8}), dict(ptr={2: ODD8}), dict(ptr={7: A + (1 << 20) + 8}),
+               dict(ptr={7: A + (1 << 20) + 16}),
                dict(ptr={3: ODD2}), dict(ptr={4: ODD2}), dict(ptr={5: ODD2}), dict(ptr={6: ODD4}),
                dict(ptr={8: ODD2}), dict(q=4100)):
         assert call(**kw) == ALIGN, kw
+    # Q is 32 rows of 8192 bytes, or as many 16384 bytes apart
+    high, size = A + (1 << 20), 32 * 8192
+    for at in (high, high + size - 32, high - size + 32):
+        assert call({0: high, 7: at}) == INVALID
+    assert call({0: high, 7: high + size}, q=8192) == INVALID
     need = L.kta_tree_attn_workspace_bytes(8, 32, 8, 128)
     assert call(ws=None) == WORKSPACE and call(size=need - 1) == WORKSPACE and call(ws=ODD8) == WORKSPACE
     if NO_GPU:
         assert call(size=need) == NO_DEVICE and call({6: None}) == NO_DEVICE
         assert call(B=1, stride=0) == NO_DEVICE
+        assert call({0: high, 7: high + size}) == call({0: high, 7: high - size}) == NO_DEVICE
 
 
 def test_wrappers_refuse_wrong_tensors():

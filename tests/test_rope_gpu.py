@@ -56,6 +56,23 @@ def test_forward_and_gradient(cuda_device, n, h, d, rot, interleaved, dtype):
         _close(got, x.double().numpy(), want, scale, rot, interleaved, dtype)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("n,h,d,rot", [(5000, 8, 128, 128), (20001, 2, 128, 96), (2400, 20, 256, 64)])
+def test_more_than_a_wave(cuda_device, n, h, d, rot, interleaved):
+    """Several items to a thread, and several tokens to a CTA; in place, what does not turn stays."""
+    from kta_b200 import ops
+
+    x = _x((n, h, d), torch.bfloat16, 3)
+    freqs, _ = ops.rope_freqs(rot, device="cpu")
+    pos = torch.randint(0, 100000, (n,), generator=torch.Generator().manual_seed(1)).to(torch.int32)
+    dev, at, turn = x.to(cuda_device), pos.to(cuda_device), freqs.to(cuda_device)
+    got = ops.rope(dev, at, turn, interleaved=interleaved, scale=0.75)
+    want = paged.rope(x.double().numpy(), pos.tolist(), freqs.tolist(), interleaved, False, 0.75)
+    _close(got, x.double().numpy(), want, 0.75, rot, interleaved, torch.bfloat16)
+    assert ops.rope(dev, at, turn, interleaved=interleaved, scale=0.75, out=dev) is dev
+    assert torch.equal(dev, got)
+
+
 def test_far_and_negative_positions(cuda_device):
     from kta_b200 import ops
 
@@ -139,7 +156,8 @@ def test_views_in_place_streams_and_replay(cuda_device):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("n,hq,hkv,d,rot,bs", [(1, 1, 1, 16, 16, 16), (9, 8, 2, 128, 128, 16),
-                                               (65, 5, 5, 64, 32, 8), (700, 32, 8, 128, 64, 64)])
+                                               (65, 5, 5, 64, 32, 8), (700, 32, 8, 128, 64, 64),
+                                               (3001, 8, 4, 128, 96, 32), (1000, 32, 8, 128, 128, 16)])
 def test_rope_cache(cuda_device, n, hq, hkv, d, rot, bs, interleaved, dtype):
     from kta_b200 import lib, ops
 

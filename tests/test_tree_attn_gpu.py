@@ -82,19 +82,14 @@ class Case:
             for h in range(self.hq):
                 o, z, pv, tiny, smax, dot = paged.attention(q[a:a + n, h], k[:, h // group],
                                                             v[:, h // group], sight, scale)
-                keys = sight.sum(1)
-                d32 = self.d * 2.0 ** -24 * dot + 6 * smax * 2.0 ** -24 + 2.0 ** -22
-                f = pv * (eps + 2 * d32 + keys * 2.0 ** -24)[:, None]
-                if self.dtype == F16:
-                    f = f + 2.0 ** -25 * tiny
-                tol = f + eps * (np.abs(o) + f) + 2.0 ** -25
+                far, far_lse = paged.attention_bounds(sight, eps, 2.0 ** -25 if self.dtype == F16 else 0.0,
+                                                      o, z, pv, tiny, smax, dot)
                 err = np.abs(out[a:a + n, h] - o)
-                assert (err <= tol).all(), (b, h, float((err / tol).max()), float(err.max()))
-                none = keys == 0
+                assert (err <= far).all(), (b, h, float((err / far).max()), float(err.max()))
+                none = ~sight.any(1)
                 assert np.array_equal(lse[a:a + n, h][none], z[none])
                 off = np.abs(lse[a:a + n, h][~none] - z[~none])
-                assert (off <= (d32 + (keys + 2 * np.abs(np.where(none, 0, z))) * 2.0 ** -24)[~none]).all(), \
-                    (b, h, float(off.max()))
+                assert (off <= far_lse[~none]).all(), (b, h, float(off.max()))
 
 
 def _status():
@@ -114,6 +109,10 @@ def _status():
     ([511, 1000], [33, 40], 16, 1, 128, 128),                   # groups of 16: several row tiles
     ([700, 129], [26, 64], 10, 2, 64, 256),                     # groups of five, blocks of 256
     ([0, 3000, 0], [0, 6, 0], 4, 1, 128, 16),                   # requests without rows around one
+    ([300, 17, 90], [2, 1, 2], 35, 5, 128, 8),                  # few rows: blocks of 8, 128 and 256
+    ([511, 1000, 40], [4, 3, 5], 16, 4, 128, 128),
+    ([700, 129, 255], [8, 4, 12], 10, 2, 64, 256),
+    ([200, 77], [8, 7], 16, 2, 128, 8),
 ])
 def test_against_the_formula(cuda_device, ctx, new, hq, hkv, d, block, dtype):
     c = Case(ctx, new, hq, hkv, d, block, dtype)
@@ -145,6 +144,23 @@ def test_split_ranges(cuda_device, ctx, new, hq, hkv):
     assert _status() == 0
 
 
+@pytest.mark.parametrize("hq,most,max_new", [(16, 3, 3), (64, 16, 16), (128, 16, 16)])
+def test_long_lists_weigh_their_requests(cuda_device, hq, most, max_new):
+    """Sixteen tiles and more to a CTA: units count more than their tiles. One row tile the one way
+    round and the other, and two row tiles of which most requests have one."""
+    g = np.random.default_rng(hq)
+    # ragged, with some of the shortest between them
+    ctx = (g.integers(2200, 2900, 20) * (np.arange(20) % 7 != 3)).tolist()
+    new = g.integers(1, 4, 20).tolist()
+    new[5], new[12] = most, 0
+    c = Case(ctx, new, hq, 8, 64, 64, BF16, seed=2)
+    out, lse = c.run(cuda_device, max_new=max_new)
+    c.check(out, lse)
+    again = c.run(cuda_device, max_new=max_new)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+    assert _status() == 0
+
+
 def test_rows_that_see_nothing_and_rows_of_no_request(cuda_device):
     c = Case([0, 40], [5, 5], 8, 2, 128, 16, BF16, gap=4)
     c.bits[1] = 0          # nothing at all
@@ -161,7 +177,8 @@ def test_rows_that_see_nothing_and_rows_of_no_request(cuda_device):
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("ctx", [0, 100, 127])
-def test_values_that_a_row_does_not_see_do_not_reach_it(cuda_device, ctx, dtype):
+@pytest.mark.parametrize("max_new", [7, 64])  # one kernel and the other
+def test_values_that_a_row_does_not_see_do_not_reach_it(cuda_device, max_new, ctx, dtype):
     """Infinities and NaN in drafted K and V: rows that do not see the token stay exact, rows that
     do have what the formula gives."""
     c = Case([ctx, 30], [7, 3], 4, 2, 128, 16, dtype, seed=3)
@@ -174,7 +191,7 @@ def test_values_that_a_row_does_not_see_do_not_reach_it(cuda_device, ctx, dtype)
                               (c.vc, 5, float("inf"))):
         block, place = slot(0, ctx + tok)
         cache[block, place, 0, 3:9] = value
-    out, lse = c.run(cuda_device)
+    out, lse = c.run(cuda_device, max_new=max_new)
     # KV head 0: token 1 (and 3 through it) has a NaN key, 2 (and 4) a NaN value, 5 (and 6) an
     # infinite one in dimensions 3..8
     o = out[:7, :2].double().cpu()
@@ -182,7 +199,7 @@ def test_values_that_a_row_does_not_see_do_not_reach_it(cuda_device, ctx, dtype)
     assert torch.isnan(o[[2, 4], :, 3:9]).all() and torch.isinf(o[[5, 6], :, 3:9]).all()
     c.kc[torch.isnan(c.kc)] = 0
     c.vc[~torch.isfinite(c.vc)] = 0
-    clean_out, clean_lse = c.run(cuda_device)
+    clean_out, clean_lse = c.run(cuda_device, max_new=max_new)
     c.check(clean_out, clean_lse)
     for row, ok in ((0, slice(None)), (2, [0, 1, 2, 9, 127]), (4, [0, 2, 10]), (5, [1, 9]), (6, [0])):
         assert torch.equal(out[row, :2][:, ok], clean_out[row, :2][:, ok])
@@ -190,19 +207,21 @@ def test_values_that_a_row_does_not_see_do_not_reach_it(cuda_device, ctx, dtype)
     assert _status() == 0
 
 
-def test_large_scores(cuda_device):
+@pytest.mark.parametrize("max_new", [6, 32])
+def test_large_scores(cuda_device, max_new):
     """Scores up to some hundreds: the running maximum has to move, and O with it."""
     for dtype in (F16, BF16):
         c = Case([900, 600], [6, 6], 8, 2, 128, 16, dtype, seed=4)
         c.q *= 8
         grow = torch.linspace(0.1, 3.0, c.blocks)[torch.randperm(c.blocks)].to(dtype)
         c.kc *= grow[:, None, None, None]
-        c.check(*c.run(cuda_device))
+        c.check(*c.run(cuda_device, max_new=max_new))
 
 
-def test_out_of_range_requests_and_blocks(cuda_device):
+@pytest.mark.parametrize("hq", [8, 64])
+def test_out_of_range_requests_and_blocks(cuda_device, hq):
     dev = cuda_device
-    good = Case([40, 300, 7], [4, 4, 4], 8, 2, 128, 16, BF16, wide=1)
+    good = Case([40, 300, 7], [4, 4, 4], hq, 2, 128, 16, BF16, wide=1)
     good.run(dev)
     assert _status() == 0
     q, kc, vc, tables, ctx, offsets = good.dev
