@@ -7,20 +7,17 @@
 //
 // One drafted token is the decode step of a paged cache; a chain is the tree 1, 11, 111, ...
 //
-//   * A KV head's query rows of one request (tokens x heads of the group, up to 128 in a row
-//     tile) share its K and V, so they are the rows of one tcgen05 tile: S = Q K^T is 128 x 128
-//     per 128 keys however few of them are real. At 128 rows the tensor core needs ~1000 cycles
-//     for a tile of keys, the softmax ~1500 and the HBM stream ~2800 (64 KB at an SM's share), so
-//     the padding of few rows is free and one kernel serves from 1 to 128 rows at HBM speed.
-//   * Work is the list of 128-key tiles of every (request, KV head), in contiguous ranges of
-//     equal length, one range per CTA (or per `row_tiles` CTAs with a row tile each, which then
-//     read the same K and V at about the same time: the second reader finds them in L2). Ragged
-//     lengths balance to a tile; what a range cuts is joined by a second small kernel from fp32
-//     partials (O, maximum, sum) in the workspace: no counters to keep at zero between calls.
-//   * Six roles in 192 threads: warps 0-3 softmax (thread = query row = TMEM lane), warp 4 TMA
-//     producer, warp 5 TMEM owner and MMA issuer. K and V tiles share a ring of six slots in the
-//     order the tensor core takes them, K(0) K(1) V(0) K(2) V(1) ...: S of the next tile is
-//     computed while the softmax works, in the other of two S buffers.
+// Two kernels compute it, by the query rows of a KV head that a request can have (drafted tokens x
+// heads of the group): up to 32 of them are the narrow side of the products (tree_narrow.cu), more are
+// row tiles of 128 (wide_kernel here). Common to both:
+//
+//   * Work is the list of 128-key tiles of every (request, KV head), in equal shares, one for a CTA
+//     (or for `row_tiles` CTAs, which take the row tiles of the share's units in turn and find each
+//     other's K and V in L2). What a share cuts is joined by a second small kernel from fp32 partials
+//     (O, maximum, sum) in the workspace: no counters to keep at zero between calls, no order of
+//     arrival in the result. Every CTA finds its share by itself from the lengths (a separate plan
+//     kernel: 9 to 13 us more; the last arriver joining instead of a kernel: 22 us where one request
+//     of 8 tokens over 1024 keys takes 13.3).
 //   * Pages: a box of the tensor map is one page (up to 128 tokens) of one head, with the token
 //     index split as (8, page / 8): shared memory gets 8-token groups of both 64-wide halves of
 //     the head, [group][half][8 tokens][128 B], which for every page size is one uniform stride
@@ -31,6 +28,21 @@
 //     V row that is not finite is zeroed and handed to the rows that see it alone.
 //   * Out-of-range lengths, offsets and block ids become status KTA_ERR_DEVICE_BOUNDS: such a
 //     request's rows are zero (LSE -inf), such a block reads as zeros. Every wait is bounded.
+//
+// wide_kernel, tensor- and power-bound. 32 trees of 33 to 64 tokens with 8 heads to a KV head, over
+// 2048 to 8192 keys: 350 to 400 us (800 to 700 TFLOP/s of the rows that exist, 14 % more with their
+// padding), the SMs at 1.54 to 1.6 GHz under the 1000 W cap and ~1930 cycles to a 128 x 128 tile.
+//
+//   * Warps 0-3 and 4-7 are two softmax warpgroups: each takes 64 keys of every tile (thread = query
+//     row = TMEM lane) and has its own O, maximum and sum, so that neither waits for the other before
+//     the segment's end, where the states are joined through shared memory. A row of 64 in registers
+//     leaves room for P and two S buffers: S of the next tile is computed beside the softmax.
+//   * Warp 8 issues the MMAs (S = Q K^T from shared memory, O += P V with P in the S columns of
+//     TMEM), warps 9-11 produce K, V and Q. K and V have rings of three tiles each.
+//   * Measured and not kept: two row tiles to a CTA over shared K and V, a warpgroup each (355
+//     against 349 us in one run, 417 against 384 at 64 tokens to a tree); S issued for 64 keys at a
+//     time (407 to 418 against 395); a part of the exponentials on the FMA pipe, whose power costs
+//     more clock than the wait for the MUFU pipe (437 against 423 sustained).
 #include <algorithm>
 #include <cmath>
 
@@ -156,7 +168,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {
     pdl_wait();
-    pdl_wait();
     if (threadIdx.x == 0) {
       record_status(p.status, KTA_ERR_LAUNCH, SITE_SMEM);
       p.desc[blockIdx.x] = Desc{};
@@ -223,13 +234,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   // after the wait: the join kernel may be scheduled now, and waits for this grid itself
   pdl_launch_dependents();
   Walk w = plan<D>(p, smem + L::OFF_K);
+  // K and V that one row tile reads once leave L2 first (64 requests of 8 tokens, 8 heads to a KV head,
+  // 1024 to 8192 keys: 197 us, 205 without); members of a share find them there.
+  const uint64_t policy = p.row_tiles > 1 ? l2_policy_evict_normal() : l2_policy_evict_first();
 
   if (warp == K_WARP) {
     produce_kv(p, w, Loader<D, RING>{&tmK, smem + L::OFF_K, k_full, k_empty, abort_flag,
-                                     l2_policy_evict_normal(), 0u, 0, 0});
+                                     policy, 0u, 0, 0});
   } else if (warp == V_WARP) {
     produce_kv(p, w, Loader<D, RING>{&tmV, smem + L::OFF_V, v_full, v_empty, abort_flag,
-                                     l2_policy_evict_normal(), 0u, 0, 0});
+                                     policy, 0u, 0, 0});
   } else if (warp == Q_WARP) {
     produce_q<D, 1>(p, w, &tmQ, smem + L::OFF_Q, 0, L::Q_HALF, q_full, q_empty, abort_flag);
   } else if (warp == MMA_WARP) {

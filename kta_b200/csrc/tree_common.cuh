@@ -1,4 +1,4 @@
-// What the two tree-attention kernels (tree.cu: many query rows, tree_narrow.cu: up to 64) share:
+// What the two tree-attention kernels (tree.cu: many query rows, tree_narrow.cu: up to 32) share:
 // the work list of a launch, the walk of a CTA over its range, the TMA producers, and the clean-up
 // of V tiles that end inside a page. The operator is described in tree.cu.
 #pragma once
@@ -20,7 +20,7 @@ constexpr int MAX_DRAFT = 64;         // bits of a row of the tree
 constexpr int MAX_GROUP = 16;
 constexpr int MAX_BATCH = 2048;       // the decode entries' limit
 constexpr int MAX_CTAS = 160;         // the workspace is sized for this many
-constexpr int NARROW_ROWS = 64;       // up to so many rows of a request: tree_narrow.cu
+constexpr int NARROW_ROWS = 32;       // up to so many rows of a request: tree_narrow.cu
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units: the maximum moves when it grew > 2^8
 
 enum : unsigned int {
@@ -115,14 +115,16 @@ __device__ __forceinline__ int row_tiles_of(const Params& p, int tokens) {
 // The work list: the 128-key tiles of every (request, KV head), b-major, each counted once for every
 // row tile of its request, in equal shares for `row_tiles` CTAs each (a share's members). A segment's
 // start and end cost a CTA about as much as SWITCH tiles (with equal numbers of tiles, shares of 3
-// segments had their keys at 183 us and shares of 10 at 215), so long lists count every unit with so
-// many more, ahead of its first tile.
+// segments had their keys at 183 us and shares of 10 at 215), so every unit counts so many more, ahead
+// of its first tile: 64 single tokens of 8 KV heads over 64 to 512 keys 36.6 us, 42.0 with equal
+// numbers of tiles; 32 over 256 to 1024 keys 29.9 and 32.2. Not where a share has less than a tile
+// (one request of 4 tokens over 1024 keys 15.0 us, 16.3 with them counted).
 //
 // Shares that are taken as they are finished (the first 78 to 88 % to each CTA, the rest in one to
 // three rounds from a counter) measured 218 to 246 us where these take 202: what a cut unit costs is
 // more than the even end gives.
 constexpr int SWITCH = 3;
-constexpr int SWITCH_FROM = 16;  // tiles of a share from which on they are counted
+constexpr int SWITCH_FROM = 1;  // tiles of a share from which on they are counted
 
 struct Shares {
   int total, n, extra;  // extra: what a unit counts beyond its tiles

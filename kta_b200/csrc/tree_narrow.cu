@@ -1,8 +1,8 @@
-// Tree attention over pages for up to 64 query rows of a KV head (drafted tokens x heads of the
+// Tree attention over pages for up to 32 query rows of a KV head (drafted tokens x heads of the
 // group): decode steps and small trees, HBM-bound on K and V. The operator, its work list and its
 // join are described in tree.cu.
 //
-// The query rows are the narrow side of both products (N = 16, 32 or 64 instead of 128 lanes that
+// The query rows are the narrow side of both products (N = 16 or 32 instead of 128 lanes that
 // are mostly padding), so keys and head dimensions are the 128 lanes:
 //
 //   S^T [128 keys, N] = K Q^T          (A = K tile, B = Q, both K-major in shared memory)
@@ -45,14 +45,13 @@ struct Narrow {
   static constexpr int HALVES = D / 64;
   static constexpr int GROUP = HALVES * 1024;
   static constexpr int TILE = BN / 8 * GROUP;
-  // 64 rows leave room for one V tile less and a single Q buffer
-  static constexpr int K_RING = 3, V_RING = N == 64 ? 2 : 3, Q_BUFS = N == 64 ? 1 : 2;
+  static constexpr int RING = 3, Q_BUFS = 2;
   static constexpr int Q_HALF = N * 128;
   static constexpr int Q_BUF = HALVES * Q_HALF;
   static constexpr int P_BUF = 2 * N * 128;  // [64 keys of a half][N rows][128 B]
   static constexpr int OFF_K = 0;
-  static constexpr int OFF_V = OFF_K + K_RING * TILE;
-  static constexpr int OFF_Q = OFF_V + V_RING * TILE;
+  static constexpr int OFF_V = OFF_K + RING * TILE;
+  static constexpr int OFF_Q = OFF_V + RING * TILE;
   static constexpr int OFF_P = OFF_Q + Q_BUFS * Q_BUF;
   static constexpr int OFF_ML = OFF_P + 2 * P_BUF;                   // [warp][N] (maximum, sum)
   static constexpr int OFF_FACTOR = OFF_ML + SOFTMAX_WARPS * N * 8;  // [buffer][warp][N]
@@ -60,14 +59,14 @@ struct Narrow {
   static constexpr int OFF_BAR = OFF_WEIGHT + SOFTMAX_WARPS * N * 4;
   // k_full, k_empty, v_full, v_empty, q_full, q_empty, s_full[2], p_full[2], p_empty[2], pv_done,
   // corrected, ml_full, ml_empty, o_full, o_free
-  static constexpr int NUM_BARS = 2 * K_RING + 2 * V_RING + 2 * Q_BUFS + 12;
+  static constexpr int NUM_BARS = 4 * RING + 2 * Q_BUFS + 12;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
   // misc: tmem base, abort, non-finite drafts [2], correction requests [2][4]
   static constexpr int TOTAL = OFF_MISC + 48;
   static_assert(TOTAL <= 232448, "shared memory budget of one sm_100 CTA");
   // TMEM: S^T of buffer i at i N, O^T of warp w at (2 + w) N
   static constexpr uint32_t COL_O = 2 * N;
-  static constexpr uint32_t TMEM_COLS = N == 16 ? 128 : N == 32 ? 256 : 512;
+  static constexpr uint32_t TMEM_COLS = N == 16 ? 128 : 256;
 };
 
 // 16 lanes (from taddr's) x N columns: register 4 c + e is lane (lane / 4) + 8 (e / 2), column
@@ -123,7 +122,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {
     pdl_wait();
-    pdl_wait();
     if (threadIdx.x == 0) {
       record_status(p.status, KTA_ERR_LAUNCH, SITE_SMEM);
       p.desc[blockIdx.x] = Desc{};
@@ -131,10 +129,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     return;
   }
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
-  uint64_t* k_empty = k_full + L::K_RING;
-  uint64_t* v_full = k_empty + L::K_RING;
-  uint64_t* v_empty = v_full + L::V_RING;
-  uint64_t* q_full = v_empty + L::V_RING;     // [Q buffer]
+  uint64_t* k_empty = k_full + L::RING;
+  uint64_t* v_full = k_empty + L::RING;
+  uint64_t* v_empty = v_full + L::RING;
+  uint64_t* q_full = v_empty + L::RING;       // [Q buffer]
   uint64_t* q_empty = q_full + L::Q_BUFS;     // [Q buffer]: the segment's last S has read Q
   uint64_t* s_full = q_empty + L::Q_BUFS;     // [buffer]
   uint64_t* p_full = s_full + 2;              // [buffer]: P, and a V tile's clean-up, are written
@@ -156,11 +154,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const int warp = warp_id();
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < L::K_RING; ++s) {
+    for (int s = 0; s < L::RING; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
-    }
-    for (int s = 0; s < L::V_RING; ++s) {
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
     }
@@ -208,11 +204,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 
   // K and V are read once: evict first, and the tables, partials and code stay in L2
   if (warp == K_WARP) {
-    produce_kv(p, w, Loader<D, L::K_RING>{&tmK, smem + L::OFF_K, k_full, k_empty, abort_flag,
-                                          l2_policy_evict_first(), 0u, 0, 0});
+    produce_kv(p, w, Loader<D, L::RING>{&tmK, smem + L::OFF_K, k_full, k_empty, abort_flag,
+                                        l2_policy_evict_first(), 0u, 0, 0});
   } else if (warp == V_WARP) {
-    produce_kv(p, w, Loader<D, L::V_RING>{&tmV, smem + L::OFF_V, v_full, v_empty, abort_flag,
-                                          l2_policy_evict_first(), 0u, 0, 0});
+    produce_kv(p, w, Loader<D, L::RING>{&tmV, smem + L::OFF_V, v_full, v_empty, abort_flag,
+                                        l2_policy_evict_first(), 0u, 0, 0});
   } else if (warp == Q_WARP) {
     produce_q<D, L::Q_BUFS>(p, w, &tmQ, smem + L::OFF_Q, L::Q_BUF, L::Q_HALF, q_full, q_empty, abort_flag);
   } else if (warp == MMA_WARP) {
@@ -234,8 +230,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           !mbar_wait(&q_full[buf], (segment / L::Q_BUFS) & 1u, abort_flag, p.status, SITE_MMA_Q)) {
         return false;
       }
-      const int st = static_cast<int>(t % L::K_RING);
-      if (!mbar_wait(&k_full[st], (t / L::K_RING) & 1u, abort_flag, p.status, SITE_MMA_K)) return false;
+      const int st = static_cast<int>(t % L::RING);
+      if (!mbar_wait(&k_full[st], (t / L::RING) & 1u, abort_flag, p.status, SITE_MMA_K)) return false;
       tc_fence_after();
       const uint64_t kdesc = sdesc_sw128(smem_u32(smem + L::OFF_K + st * L::TILE), 16, L::GROUP);
       const uint64_t qdesc = sdesc_sw128(smem_u32(smem + L::OFF_Q + buf * L::Q_BUF), 16, 1024);
@@ -268,8 +264,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       more = w.left > 0;
       if (more && !issue_s(g + 1)) break;
       const uint32_t buf = g & 1u;
-      const int st = static_cast<int>(g % L::V_RING);
-      if (!mbar_wait(&v_full[st], (g / L::V_RING) & 1u, abort_flag, p.status, SITE_MMA_V)) break;
+      const int st = static_cast<int>(g % L::RING);
+      if (!mbar_wait(&v_full[st], (g / L::RING) & 1u, abort_flag, p.status, SITE_MMA_V)) break;
       if (!mbar_wait(&p_full[buf], (g >> 1) & 1u, abort_flag, p.status, SITE_MMA_P)) break;
       if (first && !first_segment) {  // the last segment's O has been read
         if (!mbar_wait(o_free, o_phase, abort_flag, p.status, SITE_MMA_OFREE)) break;
@@ -348,8 +344,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (masked) {
           // behind S of this tile: the V tile before in this place has been waited for by then, so that
           // the phase is the right one
-          const int st = static_cast<int>(g % L::V_RING);
-          if (!mbar_wait(&v_full[st], (g / L::V_RING) & 1u, abort_flag, p.status, SITE_SM_V)) {
+          const int st = static_cast<int>(g % L::RING);
+          if (!mbar_wait(&v_full[st], (g / L::RING) & 1u, abort_flag, p.status, SITE_SM_V)) {
             ok = false;
             break;
           }
@@ -643,9 +639,8 @@ int launch_narrow(const Params& p, const CUtensorMap& tq, const CUtensorMap& tk,
     return launch_ex(kernel, dim3(grid), dim3(NUM_THREADS), smem, stream, 1, tq, tk, tv, p);
   };
   const int rows = p.box_tokens * p.group;
-  if (rows <= 16) return go(narrow_kernel<BF16, D, 16>, Narrow<D, 16>::TOTAL);
-  if (rows <= 32) return go(narrow_kernel<BF16, D, 32>, Narrow<D, 32>::TOTAL);
-  return go(narrow_kernel<BF16, D, 64>, Narrow<D, 64>::TOTAL);
+  return rows <= 16 ? go(narrow_kernel<BF16, D, 16>, Narrow<D, 16>::TOTAL)
+                    : go(narrow_kernel<BF16, D, 32>, Narrow<D, 32>::TOTAL);
 }
 
 template int launch_narrow<false, 64>(const Params&, const CUtensorMap&, const CUtensorMap&,
