@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   pdl_wait();  // the previous grid's writes (this launch's inputs) are visible from here on
   // after the wait: the join kernel may be scheduled now, and waits for this grid itself
   pdl_launch_dependents();
-  Walk w = plan<D>(p, smem + L::OFF_K);
+  Walk<false> w = plan<D, false>(p, smem + L::OFF_K);
   // K and V that one row tile reads once leave L2 first (64 requests of 8 tokens, 8 heads to a KV head,
   // 1024 to 8192 keys: 197 us, 205 without); members of a share find them there.
   const uint64_t policy = p.row_tiles > 1 ? l2_policy_evict_normal() : l2_policy_evict_first();
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // w and j run one tile ahead of the PVs, into the next segment: its first S is ready when the
     // softmax warps come from this one's epilogue.
     const uint64_t qdesc = sdesc_sw128(smem_u32(smem + L::OFF_Q), 16, 1024);
-    int j = 0, tiles = w.left > 0 ? w.count(p) : 0;
+    int j = 0, tiles = w.left > 0 ? w.count() : 0;
     uint32_t segment = 0, o_phase = 0;
     bool first_segment = true;
     // S of tile t into buffer t & 1, which holds P of tile t - 2 until its PV has read it: that was
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if (last) {
         w.next(p);
         j = 0;
-        tiles = w.left > 0 ? w.count(p) : 0;
+        tiles = w.left > 0 ? w.count() : 0;
         ++segment;
       } else {
         ++j;
@@ -326,6 +326,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // ------------- softmax, O correction and epilogue (thread = query row) -------------
     const int wg = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
+    const int tok = row / p.group, head = row - tok * p.group;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t t_s = tmem + lane_base + wg * HK;  // this half of S buffer 0
     const uint32_t t_o = tmem + lane_base + COL_O;    // O of warpgroup 0; the other's is BN columns on
@@ -334,9 +335,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     uint32_t o_phase = 0;
     bool ok = true;
     // what this thread's row of a segment sees
-    auto bits_at = [&](const Walk& v) -> uint64_t {
+    auto bits_at = [&](const Walk<false>& v) -> uint64_t {
       if (v.left <= 0 || row >= v.rows(p) * p.group) return 0ull;
-      return bits_of(p, v.row, v.row_tile(p) * p.tok_tile + row / p.group, v.tokens);
+      return bits_of(p, v.row, v.row_tile(p) * p.tok_tile + tok, v.tokens);
     };
     uint64_t bits = bits_at(w);
     while (w.left > 0 && ok) {
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int rows = tokens * p.group;
       const bool live = row < rows;
       const bool warp_on = quarter * 32 < rows;
-      const int tiles = w.count(p);
+      const int tiles = w.count();
       float m_used = -INFINITY, lsum = 0.f;
       for (int j = 0; j < tiles; ++j, ++g) {
         const int k0 = (w.i0 + j) * BN;
@@ -387,7 +388,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       }
       if (!ok) break;
       // ---- epilogue: the two warpgroups' states become one, each for half of D ----
-      Walk following = w;  // its loads come behind the last products
+      Walk<false> following = w;  // its loads come behind the last products
       following.next(p);
       const uint64_t following_bits = bits_at(following);
       if (!mbar_wait(ml_empty, o_phase ^ 1u, abort_flag, p.status, SITE_SM_ML)) break;
@@ -403,7 +404,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       tc_fence_after();
       const bool whole = w.i0 == 0 && tiles == w.tiles();
       const long long slot = slot_of(p, static_cast<int>(blockIdx.x) / p.row_tiles, rt, w.i0 > 0);
-      const int tok = row / p.group, head = row - tok * p.group;
       const int token = w.row + rt * p.tok_tile + tok;
       const int q_head = w.kvh * p.group + head;
       const uint64_t lost = bits & (static_cast<uint64_t>(bad[1]) << 32 | bad[0]);

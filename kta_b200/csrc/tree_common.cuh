@@ -161,32 +161,45 @@ struct Place {
 constexpr int PLAN_BYTES = 128 + 2 * static_cast<int>(sizeof(Place));  // shared memory of plan()
 
 // A CTA's walk over the segments of its share: runs of count() tiles from i0 on of one (request, KV
-// head). Few fields, since the softmax warps keep it beside a row of S; every warp walks by itself.
+// head). Every warp walks by itself, beside its work: what a request's tiles are is kept, no division
+// is left where there is one row tile (ONE: always), and few fields, since the softmax warps keep them
+// beside a row of S. With two or three divisions to a step each role spent 2000 to 4000 cycles on it:
+// 148 single tokens over 100 keys, eight one-tile segments to a CTA, took 39 us.
+template <bool ONE>
 struct Walk {
   int row, tokens, ctx;  // of the request
   int b, kvh, i0;
   int left;              // of the share from here on, in the list's count
   int extra;             // what a unit counts beyond its tiles
+  int n, k;              // tiles of the request, and row tiles
   int member, turn;      // this CTA in its share; the member with the segment's first row tile
 
+  __device__ __forceinline__ void enter(const Params& p, int row_, int tokens_, int ctx_) {
+    row = row_;
+    tokens = tokens_;
+    ctx = ctx_;
+    n = (ctx + tokens + BN - 1) / BN;
+    k = ONE ? 1 : row_tiles_of(p, tokens);
+  }
   __device__ __forceinline__ int len() const { return ctx + tokens; }
-  __device__ __forceinline__ int tiles() const { return (len() + BN - 1) / BN; }
-  __device__ __forceinline__ int count(const Params& p) const {
-    return min(tiles() - i0, left / row_tiles_of(p, tokens) - (i0 == 0 ? extra : 0));
+  __device__ __forceinline__ int tiles() const { return n; }
+  __device__ __forceinline__ int count() const {
+    return min(n - i0, (ONE || k == 1 ? left : left / k) - (i0 == 0 ? extra : 0));
   }
   // The row tile of the request that falls to this member. Requests have between one and row_tiles
   // of them: the members take turns, so that each has its share over some segments.
   __device__ __forceinline__ int row_tile(const Params& p) const {
-    const int k = member - turn;
-    return k < 0 ? k + p.row_tiles : k;
+    if (ONE) return 0;
+    const int t = member - turn;
+    return t < 0 ? t + p.row_tiles : t;
   }
   // Drafted tokens of this member's row tile: 0 where the request has fewer.
   __device__ __forceinline__ int rows(const Params& p) const {
-    return max(0, min(tokens - row_tile(p) * p.tok_tile, p.tok_tile));
+    return ONE ? tokens : max(0, min(tokens - row_tile(p) * p.tok_tile, p.tok_tile));
   }
   // To the next segment with rows for this member, this one included; left is 0 where there is none.
   __device__ __forceinline__ void settle(const Params& p) {
-    while (left > 0 && rows(p) == 0) step(p);
+    while (!ONE && left > 0 && rows(p) == 0) step(p);
   }
   __device__ __forceinline__ void next(const Params& p) {
     step(p);
@@ -195,10 +208,13 @@ struct Walk {
 
  private:
   __device__ __forceinline__ void step(const Params& p) {
-    const int k = row_tiles_of(p, tokens);
-    left -= (count(p) + (i0 == 0 ? extra : 0)) * k;
+    const int some = count() + (i0 == 0 ? extra : 0);
+    left -= ONE ? some : some * k;
     if (left <= 0) return;
-    turn = (turn + k) % p.row_tiles;
+    if (!ONE) {
+      turn += k;
+      turn = turn >= p.row_tiles ? turn - p.row_tiles : turn;
+    }
     i0 = 0;
     if (++kvh == p.hkv) {
       kvh = 0;
@@ -206,9 +222,7 @@ struct Walk {
       do {  // tiles are left in the share, so a request with some follows
         r = request_of(p, ++b);
       } while (tiles_of(r) == 0);
-      row = r.row;
-      tokens = r.tokens;
-      ctx = r.ctx;
+      enter(p, r.row, r.tokens, r.ctx);
     }
   }
 };
@@ -217,8 +231,8 @@ struct Walk {
 // (left is 0 where it has none); member 0 describes the unit that the share's end cuts. By all
 // threads, which it synchronises; `scratch` is PLAN_BYTES of shared memory. Rows of requests that
 // are out of range become zero.
-template <int D>
-__device__ __forceinline__ Walk plan(const Params& p, uint8_t* scratch) {
+template <int D, bool ONE>
+__device__ __forceinline__ Walk<ONE> plan(const Params& p, uint8_t* scratch) {
   // The block tables into L2, a line for a thread: a producer that misses it waits behind the
   // stream's own reads.
   const int lines = (p.max_blocks * 4 + 127) / 128;
@@ -308,7 +322,7 @@ __device__ __forceinline__ Walk plan(const Params& p, uint8_t* scratch) {
     }
   }
   __syncthreads();
-  Walk w = {};
+  Walk<ONE> w = {};
   w.extra = sh.extra;
   w.member = member;
   int cut = 0;  // shares that hold a part of the unit that starts in this one and ends later
@@ -325,9 +339,7 @@ __device__ __forceinline__ Walk plan(const Params& p, uint8_t* scratch) {
     w.kvh = places[0].kvh;
     w.i0 = places[0].tile;
     w.left = end - places[0].at;
-    w.row = places[0].row;
-    w.tokens = places[0].tokens;
-    w.ctx = places[0].ctx;
+    w.enter(p, places[0].row, places[0].tokens, places[0].ctx);
     w.settle(p);
   }
   if (member == 0 && threadIdx.x < p.row_tiles) {
@@ -425,17 +437,20 @@ struct Loader {
   int id, id1;  // this lane's blocks of the segment's next two tiles, in flight
 
   // this lane's block of tile i
-  __device__ __forceinline__ int block_of(const Params& p, const Walk& w, int i) const {
+  template <typename W>
+  __device__ __forceinline__ int block_of(const Params& p, const W& w, int i) const {
     const int at = i * (BN >> p.box_log2) + static_cast<int>(threadIdx.x & 31);
     if (static_cast<int>(threadIdx.x & 31) >= BN >> p.box_log2 || at << p.box_log2 >= w.len()) return 0;
     return p.tables[w.b * p.table_stride + (at >> (p.page_log2 - p.box_log2))];
   }
-  __device__ __forceinline__ void start(const Params& p, const Walk& w, int end) {
+  template <typename W>
+  __device__ __forceinline__ void start(const Params& p, const W& w, int end) {
     id = block_of(p, w, w.i0);
     id1 = w.i0 + 1 < end ? block_of(p, w, w.i0 + 1) : 0;
   }
   // Tile i of the segment that ends before tile `end`.
-  __device__ __forceinline__ bool load(const Params& p, const Walk& w, int i, int end) {
+  template <typename W>
+  __device__ __forceinline__ bool load(const Params& p, const W& w, int i, int end) {
     const int lane = threadIdx.x & 31;
     const int box = 1 << p.box_log2, pages = BN >> p.box_log2, group_box = box / 8;
     const int id2 = i + 2 < end ? block_of(p, w, i + 2) : 0;
@@ -474,11 +489,11 @@ struct Loader {
 };
 
 // K or V producer warp.
-template <int D, int STAGES>
-__device__ __forceinline__ void produce_kv(const Params& p, Walk w, Loader<D, STAGES> ld) {
+template <int D, int STAGES, typename W>
+__device__ __forceinline__ void produce_kv(const Params& p, W w, Loader<D, STAGES> ld) {
   bool ok = true;
   for (; w.left > 0 && ok; w.next(p)) {
-    const int end = w.i0 + w.count(p);
+    const int end = w.i0 + w.count();
     ld.start(p, w, end);
     for (int i = w.i0; i < end && ok; ++i) ok = ld.load(p, w, i, end);
     if (!ok) break;
@@ -487,8 +502,8 @@ __device__ __forceinline__ void produce_kv(const Params& p, Walk w, Loader<D, ST
 }
 
 // Producer warp of Q: each segment's query rows, [half][rows][128 B], into one of BUFS buffers.
-template <int D, int BUFS>
-__device__ __forceinline__ void produce_q(const Params& p, Walk w, const CUtensorMap* map, uint8_t* base,
+template <int D, int BUFS, typename W>
+__device__ __forceinline__ void produce_q(const Params& p, W w, const CUtensorMap* map, uint8_t* base,
                                           int buf_bytes, int half_bytes, uint64_t* full, uint64_t* empty,
                                           volatile int* abort_flag) {
   if ((threadIdx.x & 31) == 0) {

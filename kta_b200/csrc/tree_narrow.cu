@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   pdl_wait();  // the previous grid's writes (this launch's inputs) are visible from here on
   // after the wait: the join kernel may be scheduled now, and waits for this grid itself
   pdl_launch_dependents();
-  Walk w = plan<D>(p, smem + L::OFF_K);
+  Walk<true> w = plan<D, true>(p, smem + L::OFF_K);
 
   // K and V are read once: evict first, and the tables, partials and code stay in L2
   if (warp == K_WARP) {
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // 64 dimensions are one MN block: with a block stride of zero the lanes from 64 on repeat it
     constexpr uint32_t V_BLOCK = D == 128 ? 1024u : 0u;
     // w and j run one tile ahead of the PVs, into the next segment
-    int j = 0, tiles = w.left > 0 ? w.count(p) : 0;
+    int j = 0, tiles = w.left > 0 ? w.count() : 0;
     uint32_t segment = 0, o_phase = 0, corrections = 0;
     bool first_segment = true;
     // S^T of tile t into buffer t & 1: the softmax has read tile t - 2 from it, since that tile's P
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if (last) {
         w.next(p);
         j = 0;
-        tiles = w.left > 0 ? w.count(p) : 0;
+        tiles = w.left > 0 ? w.count() : 0;
         ++segment;
       } else {
         ++j;
@@ -308,19 +308,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                            ((((warp & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4);
     uint32_t g = 0, segment = 0;
     bool ok = true;
-    Walk following;
-    for (; w.left > 0 && ok; w = following, ++segment) {
-      const int tiles = w.count(p);
-      // lane r (and r + 32): what row r sees, for the tiles that hold drafted tokens
-      constexpr int PER = (N + 31) / 32;
-      uint64_t bits[PER];
-#pragma unroll
-      for (int u = 0; u < PER; ++u) {
-        const int r = lane + 32 * u;
-        bits[u] = r < w.tokens * p.group && (w.i0 + tiles) * BN > w.ctx
-                      ? bits_of(p, w.row, r / p.group, w.tokens)
-                      : 0ull;
-      }
+    Walk<true> following;
+    // lane r: what row r of a segment sees
+    const int tok = lane / p.group;
+    auto bits_at = [&](const Walk<true>& v) -> uint64_t {
+      return v.left > 0 && tok < v.tokens ? bits_of(p, v.row, tok, v.tokens) : 0ull;
+    };
+    uint64_t bits = bits_at(w), following_bits = 0;
+    for (; w.left > 0 && ok; w = following, bits = following_bits, ++segment) {
+      const int tiles = w.count();
       float m[C8][2];
       uint64_t sum[C8];
 #pragma unroll
@@ -335,6 +331,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (j + 1 == tiles) {  // the next segment's request, while this one's last tile comes
           following = w;
           following.next(p);
+          following_bits = bits_at(following);
         }
         if (!mbar_wait(&s_full[buf], (g >> 1) & 1u, abort_flag, p.status, SITE_SM_S)) {
           ok = false;
@@ -364,7 +361,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           for (int c = 0; c < C8; ++c) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const uint64_t view = __shfl_sync(0xffffffffu, bits[c / 4], (8 * c + col0 + e) & 31);
+              const uint64_t view = __shfl_sync(0xffffffffu, bits, 8 * c + col0 + e);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int k = key + 8 * i;
@@ -471,11 +468,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // --------------- correction and epilogue (thread = head dimension) ---------------
     const int quarter = warp & 3;
     const int d = quarter * 32 + lane;
+    const int tok_r = lane / p.group;  // of row `lane`
     const uint32_t t_o = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + L::COL_O;
     uint32_t g = 0, segment = 0;
     bool ok = true;
     for (; w.left > 0 && ok; w.next(p), ++segment) {
-      const int tiles = w.count(p);
+      const int tiles = w.count();
       for (int j = 0; j < tiles; ++j, ++g) {
         const uint32_t buf = g & 1u;
         if (!mbar_wait(&p_full[buf], (g >> 1) & 1u, abort_flag, p.status, SITE_N_OUT_P)) {
@@ -522,12 +520,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const bool whole = w.i0 == 0 && tiles == w.tiles();
       const int rows = w.tokens * p.group;
       const long long slot = slot_of(p, blockIdx.x, 0, w.i0 > 0);
-      // Lane r (and r + 32): the weights of row r's four states. The four warps write the same
-      // values; none gets to the next segment's while another reads these (ml_empty).
-#pragma unroll
-      for (int u = 0; u < (N + 31) / 32; ++u) {
-        const int r = lane + 32 * u;
-        if (r >= N) continue;
+      // Lane r: the weights of row r's four states. The four warps write the same values; none gets
+      // to the next segment's while another reads these (ml_empty).
+      if (lane < N) {
+        const int r = lane;
         float wt[SOFTMAX_WARPS];
         float top = -INFINITY, l = 0.f;
 #pragma unroll
@@ -541,8 +537,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         if (r < rows && quarter == 0) {
           if (whole) {
-            const int tok = r / p.group;
-            p.lse[static_cast<long long>(w.row + tok) * p.hq + w.kvh * p.group + (r - tok * p.group)] =
+            p.lse[static_cast<long long>(w.row + tok_r) * p.hq + w.kvh * p.group + (r - tok_r * p.group)] =
                 l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
           } else {
             p.part_ml[slot * p.row_cap + r] = make_float2(top, l);
