@@ -599,7 +599,8 @@ int go(Params& p, const void* Q, const void* Kc, const void* Vc, int64_t q_token
   if (s != KTA_OK) return s;
   const int sms = std::min(current_sm_count(), MAX_CTAS);
   if (sms < p.row_tiles) return KTA_ERR_UNSUPPORTED;
-  const int grid = sms / p.row_tiles * p.row_tiles;
+  p.groups = sms / p.row_tiles;
+  const int grid = p.groups * p.row_tiles;
   // One tcgen05 tile has 128 rows in wide_kernel however few are real, and up to 64 in the other.
   const bool narrow = p.box_tokens * p.group <= NARROW_ROWS;
   if (narrow) {

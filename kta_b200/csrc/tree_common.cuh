@@ -68,6 +68,7 @@ struct Params {
   int tok_tile;            // drafted tokens of a row tile: 128 / group
   int box_tokens;          // tokens of the Q box: min(tok_tile, max_new)
   int row_tiles;           // members of a share
+  int groups;              // shares: one for as many CTAs
   int row_cap;             // rows of a partial
   float scale_log2;        // softmax scale * log2(e)
   unsigned int* status;
@@ -128,26 +129,22 @@ constexpr int SWITCH_FROM = 1;  // tiles of a share from which on they are count
 
 struct Shares {
   int total, n, extra;  // extra: what a unit counts beyond its tiles
-  double length;
+  int length, longer;   // of a share, before it is rounded down to tiles; the first `longer` have one more
   __device__ __forceinline__ Shares(const Params& p, int tiles, int units) {
-    const int groups = static_cast<int>(gridDim.x) / p.row_tiles;
-    extra = tiles / groups >= SWITCH_FROM * p.row_tiles ? SWITCH : 0;
+    extra = tiles >= SWITCH_FROM * p.row_tiles * p.groups ? SWITCH : 0;
     total = tiles + extra * units;
     // a share is at least (1 + extra) row_tiles long, so that it has a tile wherever it starts
-    n = total == 0 ? 0 : max(1, min(groups, total / ((1 + extra) * p.row_tiles)));
-    length = static_cast<double>(total) / max(n, 1);
+    const int least = (1 + extra) * p.row_tiles;
+    n = total >= p.groups * least ? p.groups : total == 0 ? 0 : max(1, total / least);
+    length = n == 0 ? 0 : static_cast<int>(static_cast<unsigned>(total) / static_cast<unsigned>(n));
+    longer = total - length * n;
   }
-  // Where share r starts, before it is rounded down to a tile: any growing function of r that all
-  // threads compute alike will do, so no exact division. The exact value is a multiple of 1 / 160: no
-  // rounding gets it past a whole number.
-  __device__ __forceinline__ int start(int r) const {
-    return r >= n ? total : static_cast<int>(length * r + 1e-5);
-  }
+  // Where share r starts, before it is rounded down to a tile.
+  __device__ __forceinline__ int start(int r) const { return r >= n ? total : length * r + min(r, longer); }
   // the last share that starts before position x > 0
   __device__ __forceinline__ int before(int x) const {
-    int r = min(n - 1, static_cast<int>(x / length) + 1);
-    while (r > 0 && start(r) >= x) --r;
-    return r;
+    const int y = x - longer * (length + 1);  // into the shorter ones
+    return y <= 0 ? (x - 1) / (length + 1) : min(n - 1, longer + (y - 1) / length);
   }
 };
 
@@ -254,7 +251,7 @@ __device__ __forceinline__ Walk<ONE> plan(const Params& p, uint8_t* scratch) {
   for (int b = b0; b < b1; ++b) {
     const Request r = request_of(p, b);
     if (b == b0) kept = r;
-    const int k = p.hkv * row_tiles_of(p, r.tokens), n = tiles_of(r);
+    const int k = p.hkv * (ONE ? 1 : row_tiles_of(p, r.tokens)), n = tiles_of(r);
     mine.x += n * k;
     mine.y += n > 0 ? k : 0;
     bad |= r.bad;
@@ -276,8 +273,8 @@ __device__ __forceinline__ Walk<ONE> plan(const Params& p, uint8_t* scratch) {
   }
   const Shares sh(p, all.x, all.y);
   const int before = ahead.x + sh.extra * ahead.y, sum = mine.x + sh.extra * mine.y;
-  const int share = static_cast<int>(blockIdx.x) / p.row_tiles;
-  const int member = static_cast<int>(blockIdx.x) - share * p.row_tiles;
+  const int share = ONE ? blockIdx.x : static_cast<int>(blockIdx.x) / p.row_tiles;
+  const int member = ONE ? 0 : static_cast<int>(blockIdx.x) - share * p.row_tiles;
   if (share < sh.n && sum > 0) {
     // the starts of the share and of the next one, by the threads that hold them
     for (int q = 0; q < 2; ++q) {
@@ -286,7 +283,7 @@ __device__ __forceinline__ Walk<ONE> plan(const Params& p, uint8_t* scratch) {
       int t = before;
       for (int b = b0; b < b1; ++b) {
         const Request r = b == b0 ? kept : request_of(p, b);
-        const int k = row_tiles_of(p, r.tokens);
+        const int k = ONE ? 1 : row_tiles_of(p, r.tokens);
         const int pair = tiles_of(r) > 0 ? (tiles_of(r) + sh.extra) * k : 0;
         if (at >= t + pair * p.hkv) {
           t += pair * p.hkv;
@@ -388,10 +385,11 @@ template <bool BF16, int D>
 __device__ __forceinline__ void clean_v(uint8_t* tile, int from, int count, int first, int valid, int token0,
                                         int tid, unsigned int* bad) {
   constexpr int CHUNKS = D / 8;  // 16-byte pieces of a row
-  for (int i = tid + max(first, from) * CHUNKS; i < (from + count) * CHUNKS; i += 128) {
-    const int row = i / CHUNKS, ch = i % CHUNKS;
-    uint4* at = reinterpret_cast<uint4*>(tile + (row >> 3) * (D / 64 * 1024) + (ch >> 3) * 1024 +
-                                         (row & 7) * 128 + (ch & 7) * 16);
+  const int ch = tid % CHUNKS;
+  uint8_t* piece = tile + (ch >> 3) * 1024 + (ch & 7) * 16;
+#pragma unroll 1
+  for (int row = max(first, from) + tid / CHUNKS; row < from + count; row += 128 / CHUNKS) {
+    uint4* at = reinterpret_cast<uint4*>(piece + (row >> 3) * (D / 64 * 1024) + (row & 7) * 128);
     if (row >= valid) {
       *at = make_uint4(0u, 0u, 0u, 0u);
       continue;

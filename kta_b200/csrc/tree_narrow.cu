@@ -361,12 +361,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           for (int c = 0; c < C8; ++c) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const uint64_t view = __shfl_sync(0xffffffffu, bits, 8 * c + col0 + e);
+              const uint32_t view = view_word(__shfl_sync(0xffffffffu, bits, 8 * c + col0 + e), key);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const int k = key + 8 * i;
-                const bool sees = k < 0 || (k < 64 && ((view >> k) & 1ull) != 0);
-                if (!sees) s[i >> 1][4 * c + 2 * (i & 1) + e] = __float_as_uint(-INFINITY);
+                if (!((view >> (8 * i)) & 1u)) s[i >> 1][4 * c + 2 * (i & 1) + e] = __float_as_uint(-INFINITY);
               }
             }
           }
