@@ -114,7 +114,7 @@ __device__ __forceinline__ bool softmax_step(uint32_t t_s, uint32_t t_o, const u
   }
   lsum *= factor;
   if (__any_sync(0xffffffffu, rescale)) {
-    if (!mbar_wait(pv_done, pv_parity, abort, status, SITE_SM_PV)) return false;
+    if (!wait_for(pv_done, pv_parity, abort, status, SITE_SM_PV)) return false;
     tc_fence_after();
     const float f = rescale ? factor : 1.f;
 #pragma unroll 1
@@ -260,9 +260,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // S of tile t into buffer t & 1, which holds P of tile t - 2 until its PV has read it: that was
     // issued before and ends before this begins.
     auto issue_s = [&](uint32_t t) -> bool {
-      if (j == 0 && !mbar_wait(q_full, segment & 1u, abort_flag, p.status, SITE_MMA_Q)) return false;
+      if (j == 0 && !wait_for(q_full, segment & 1u, abort_flag, p.status, SITE_MMA_Q)) return false;
       const int st = static_cast<int>(t % RING);
-      if (!mbar_wait(&k_full[st], (t / RING) & 1u, abort_flag, p.status, SITE_MMA_K)) return false;
+      if (!wait_for(&k_full[st], (t / RING) & 1u, abort_flag, p.status, SITE_MMA_K)) return false;
       tc_fence_after();
       const uint64_t kdesc = sdesc_sw128(smem_u32(smem + L::OFF_K + st * L::TILE), 16, L::GROUP);
       if (elect_one_sync()) {
@@ -294,14 +294,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       more = w.left > 0;
       if (more && !issue_s(g + 1)) break;
       const int st = static_cast<int>(g % RING);
-      if (!mbar_wait(&v_full[st], (g / RING) & 1u, abort_flag, p.status, SITE_MMA_V)) break;
+      if (!wait_for(&v_full[st], (g / RING) & 1u, abort_flag, p.status, SITE_MMA_V)) break;
       const uint64_t vdesc = sdesc_sw128(smem_u32(smem + L::OFF_V + st * L::TILE), 1024, L::GROUP);
       bool ok = true;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // the warpgroups' halves of the keys, into their own O
-        ok = ok && mbar_wait(&p_full[2 * (g & 1u) + h], (g >> 1) & 1u, abort_flag, p.status, SITE_MMA_P);
+        ok = ok && wait_for(&p_full[2 * (g & 1u) + h], (g >> 1) & 1u, abort_flag, p.status, SITE_MMA_P);
         if (first && h == 0 && !first_segment) {  // the last segment's O has been read
-          ok = ok && mbar_wait(o_free, o_phase, abort_flag, p.status, SITE_MMA_OFREE);
+          ok = ok && wait_for(o_free, o_phase, abort_flag, p.status, SITE_MMA_OFREE);
           o_phase ^= 1u;
         }
         if (!ok) break;
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       for (int j = 0; j < tiles; ++j, ++g) {
         const int k0 = (w.i0 + j) * BN;
         const bool masked = k0 + BN > w.ctx;
-        if (!mbar_wait(&s_full[g & 1u], (g >> 1) & 1u, abort_flag, p.status, SITE_SM_S)) {
+        if (!wait_for(&s_full[g & 1u], (g >> 1) & 1u, abort_flag, p.status, SITE_SM_S)) {
           ok = false;
           break;
         }
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           // behind S of this tile: the V tile before in this place has been waited for by then, so that
           // the phase is the right one
           const int st = static_cast<int>(g % RING);
-          if (!mbar_wait(&v_full[st], (g / RING) & 1u, abort_flag, p.status, SITE_SM_V)) {
+          if (!wait_for(&v_full[st], (g / RING) & 1u, abort_flag, p.status, SITE_SM_V)) {
             ok = false;
             break;
           }
@@ -391,15 +391,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       Walk<false> following = w;  // its loads come behind the last products
       following.next(p);
       const uint64_t following_bits = bits_at(following);
-      if (!mbar_wait(ml_empty, o_phase ^ 1u, abort_flag, p.status, SITE_SM_ML)) break;
+      if (!wait_for(ml_empty, o_phase ^ 1u, abort_flag, p.status, SITE_SM_ML)) break;
       ml[wg * BM + row] = make_float2(m_used, lsum);
       __syncwarp();
       if (lane == 0) mbar_arrive(ml_full);
-      if (!mbar_wait(ml_full, o_phase, abort_flag, p.status, SITE_SM_ML)) break;
+      if (!wait_for(ml_full, o_phase, abort_flag, p.status, SITE_SM_ML)) break;
       const float2 ml_a = ml[row], ml_b = ml[BM + row];
       __syncwarp();
       if (lane == 0) mbar_arrive(ml_empty);
-      if (!mbar_wait(o_done, o_phase, abort_flag, p.status, SITE_SM_O)) break;
+      if (!wait_for(o_done, o_phase, abort_flag, p.status, SITE_SM_O)) break;
       o_phase ^= 1u;
       tc_fence_after();
       const bool whole = w.i0 == 0 && tiles == w.tiles();

@@ -41,6 +41,18 @@ enum : unsigned int {
   SITE_BLOCK = 0x912,    // a block id out of range
 };
 
+// mbar_wait() with all behind the first try in one place: the roles' code, inlined many times, has to
+// pass through the SM's instruction caches for every segment (148 single tokens over 100 keys 28.4 us
+// with it inlined, 25.0 so).
+static __device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                     unsigned int* status, unsigned int site) {
+  return mbar_wait(bar, parity, abort, status, site);
+}
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                         unsigned int* status, unsigned int site) {
+  return mbar_try_wait(smem_u32(bar), parity) || wait_on(bar, parity, abort, status, site);
+}
+
 // What the join kernel needs of a unit (a row tile's tiles of one (request, KV head)) that starts in a
 // share and ends in a later one.
 struct Desc {
@@ -453,7 +465,7 @@ struct Loader {
     const int box = 1 << p.box_log2, pages = BN >> p.box_log2, group_box = box / 8;
     const int id2 = i + 2 < end ? block_of(p, w, i + 2) : 0;
     const int st = static_cast<int>(n % STAGES);
-    if (!mbar_wait(&empty[st], ((n / STAGES) & 1u) ^ 1u, abort, p.status, SITE_PROD_KV)) return false;
+    if (!wait_for(&empty[st], ((n / STAGES) & 1u) ^ 1u, abort, p.status, SITE_PROD_KV)) return false;
     ++n;
     const int held = min(pages, (w.len() - i * BN + box - 1) >> p.box_log2);
     if (lane == 0) mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(held * group_box * GROUP));
@@ -481,7 +493,7 @@ struct Loader {
     if (*abort == 0 || (threadIdx.x & 31) != 0) return;
     int none = 0;
     for (uint32_t k = n > STAGES ? n - STAGES : 0; k < n; ++k) {
-      mbar_wait(&full[k % STAGES], (k / STAGES) & 1u, &none, p.status, SITE_PROD_KV);
+      wait_for(&full[k % STAGES], (k / STAGES) & 1u, &none, p.status, SITE_PROD_KV);
     }
   }
 };
@@ -508,7 +520,7 @@ __device__ __forceinline__ void produce_q(const Params& p, W w, const CUtensorMa
     uint32_t n = 0;  // segments so far
     for (; w.left > 0; w.next(p)) {
       const uint32_t buf = n % BUFS;
-      if (!mbar_wait(&empty[buf], ((n / BUFS) & 1u) ^ 1u, abort_flag, p.status, SITE_PROD_Q)) break;
+      if (!wait_for(&empty[buf], ((n / BUFS) & 1u) ^ 1u, abort_flag, p.status, SITE_PROD_Q)) break;
       ++n;
       mbar_arrive_expect_tx(&full[buf], static_cast<uint32_t>(p.box_tokens * p.group * D * 2));
 #pragma unroll
@@ -520,7 +532,7 @@ __device__ __forceinline__ void produce_q(const Params& p, W w, const CUtensorMa
     if (*abort_flag != 0) {
       int none = 0;
       for (uint32_t k = n > BUFS ? n - BUFS : 0; k < n; ++k) {
-        mbar_wait(&full[k % BUFS], (k / BUFS) & 1u, &none, p.status, SITE_PROD_Q);
+        wait_for(&full[k % BUFS], (k / BUFS) & 1u, &none, p.status, SITE_PROD_Q);
       }
     }
   }

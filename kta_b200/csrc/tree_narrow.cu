@@ -227,11 +227,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     auto issue_s = [&](uint32_t t) -> bool {
       const uint32_t buf = segment % L::Q_BUFS;
       if (j == 0 &&
-          !mbar_wait(&q_full[buf], (segment / L::Q_BUFS) & 1u, abort_flag, p.status, SITE_MMA_Q)) {
+          !wait_for(&q_full[buf], (segment / L::Q_BUFS) & 1u, abort_flag, p.status, SITE_MMA_Q)) {
         return false;
       }
       const int st = static_cast<int>(t % L::RING);
-      if (!mbar_wait(&k_full[st], (t / L::RING) & 1u, abort_flag, p.status, SITE_MMA_K)) return false;
+      if (!wait_for(&k_full[st], (t / L::RING) & 1u, abort_flag, p.status, SITE_MMA_K)) return false;
       tc_fence_after();
       const uint64_t kdesc = sdesc_sw128(smem_u32(smem + L::OFF_K + st * L::TILE), 16, L::GROUP);
       const uint64_t qdesc = sdesc_sw128(smem_u32(smem + L::OFF_Q + buf * L::Q_BUF), 16, 1024);
@@ -265,14 +265,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if (more && !issue_s(g + 1)) break;
       const uint32_t buf = g & 1u;
       const int st = static_cast<int>(g % L::RING);
-      if (!mbar_wait(&v_full[st], (g / L::RING) & 1u, abort_flag, p.status, SITE_MMA_V)) break;
-      if (!mbar_wait(&p_full[buf], (g >> 1) & 1u, abort_flag, p.status, SITE_MMA_P)) break;
+      if (!wait_for(&v_full[st], (g / L::RING) & 1u, abort_flag, p.status, SITE_MMA_V)) break;
+      if (!wait_for(&p_full[buf], (g >> 1) & 1u, abort_flag, p.status, SITE_MMA_P)) break;
       if (first && !first_segment) {  // the last segment's O has been read
-        if (!mbar_wait(o_free, o_phase, abort_flag, p.status, SITE_MMA_OFREE)) break;
+        if (!wait_for(o_free, o_phase, abort_flag, p.status, SITE_MMA_OFREE)) break;
         o_phase ^= 1u;
       }
       if (ask[buf * 4] | ask[buf * 4 + 1] | ask[buf * 4 + 2] | ask[buf * 4 + 3]) {
-        if (!mbar_wait(corrected, corrections & 1u, abort_flag, p.status, SITE_N_MMA_CORR)) break;
+        if (!wait_for(corrected, corrections & 1u, abort_flag, p.status, SITE_N_MMA_CORR)) break;
         ++corrections;
       }
       tc_fence_after();
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           following.next(p);
           following_bits = bits_at(following);
         }
-        if (!mbar_wait(&s_full[buf], (g >> 1) & 1u, abort_flag, p.status, SITE_SM_S)) {
+        if (!wait_for(&s_full[buf], (g >> 1) & 1u, abort_flag, p.status, SITE_SM_S)) {
           ok = false;
           break;
         }
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           // behind S of this tile: the V tile before in this place has been waited for by then, so that
           // the phase is the right one
           const int st = static_cast<int>(g % L::RING);
-          if (!mbar_wait(&v_full[st], (g / L::RING) & 1u, abort_flag, p.status, SITE_SM_V)) {
+          if (!wait_for(&v_full[st], (g / L::RING) & 1u, abort_flag, p.status, SITE_SM_V)) {
             ok = false;
             break;
           }
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
         }
         // the buffer of P and of the factors: the PV two tiles ago has read the one, warps 4-7 the other
-        if (!mbar_wait(&p_empty[buf], ((g >> 1) & 1u) ^ 1u, abort_flag, p.status, SITE_N_SM_P)) {
+        if (!wait_for(&p_empty[buf], ((g >> 1) & 1u) ^ 1u, abort_flag, p.status, SITE_N_SM_P)) {
           ok = false;
           break;
         }
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       }
       if (!ok) break;
       // ---- the segment's maxima and sums ----
-      if (!mbar_wait(ml_empty, (segment & 1u) ^ 1u, abort_flag, p.status, SITE_N_SM_ML)) break;
+      if (!wait_for(ml_empty, (segment & 1u) ^ 1u, abort_flag, p.status, SITE_N_SM_ML)) break;
 #pragma unroll
       for (int c = 0; c < C8; ++c) {
         float l[2];
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int tiles = w.count();
       for (int j = 0; j < tiles; ++j, ++g) {
         const uint32_t buf = g & 1u;
-        if (!mbar_wait(&p_full[buf], (g >> 1) & 1u, abort_flag, p.status, SITE_N_OUT_P)) {
+        if (!wait_for(&p_full[buf], (g >> 1) & 1u, abort_flag, p.status, SITE_N_OUT_P)) {
           ok = false;
           break;
         }
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           continue;
         }
         // the PV before; the one before that is complete, since this tile's S came behind it
-        if (!mbar_wait(pv_done, (g - 1) & 1u, abort_flag, p.status, SITE_N_OUT_PV)) {
+        if (!wait_for(pv_done, (g - 1) & 1u, abort_flag, p.status, SITE_N_OUT_PV)) {
           ok = false;
           break;
         }
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
       }
       if (!ok) break;
-      if (!mbar_wait(ml_full, segment & 1u, abort_flag, p.status, SITE_N_OUT_ML)) break;
+      if (!wait_for(ml_full, segment & 1u, abort_flag, p.status, SITE_N_OUT_ML)) break;
       const bool whole = w.i0 == 0 && tiles == w.tiles();
       const int rows = w.tokens * p.group;
       const long long slot = slot_of(p, blockIdx.x, 0, w.i0 > 0);
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         weights[r] = make_float4(wt[0] * inv, wt[1] * inv, wt[2] * inv, wt[3] * inv);
       }
       __syncwarp();
-      if (!mbar_wait(o_full, segment & 1u, abort_flag, p.status, SITE_N_OUT_O)) break;
+      if (!wait_for(o_full, segment & 1u, abort_flag, p.status, SITE_N_OUT_O)) break;
       tc_fence_after();
       uint16_t* out = static_cast<uint16_t*>(p.out) +
                       (static_cast<long long>(w.row) * p.hq + w.kvh * p.group) * D + d;
