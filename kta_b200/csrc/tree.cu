@@ -37,6 +37,8 @@
 //     row = TMEM lane) and has its own O, maximum and sum, so that neither waits for the other before
 //     the segment's end, where the states are joined through shared memory. A row of 64 in registers
 //     leaves room for P and two S buffers: S of the next tile is computed beside the softmax.
+//   * The two warps of a scheduler take turns with their exponentials (`turn`): the one's loads, maxima
+//     and stores run beside the other's MUFU work (402 us sustained, 412 in step).
 //   * Warp 8 issues the MMAs (S = Q K^T from shared memory, O += P V with P in the S columns of
 //     TMEM), warps 9-11 produce K, V and Q. K and V have rings of three tiles each.
 //   * Measured and not kept: two row tiles to a CTA over shared K and V, a warpgroup each (355
@@ -68,8 +70,8 @@ struct Layout {
   static constexpr int OFF_ML = OFF_V + RING * TILE;  // [warpgroup][128 rows] (maximum, sum)
   static constexpr int OFF_BAR = OFF_ML + 2 * BM * 8;
   // k_full[R], k_empty[R], v_full[R], v_empty[R], q_full, q_empty, s_full[2], p_full[2][2],
-  // pv_done[2], ml_full, ml_empty, o_done, o_free
-  static constexpr int NUM_BARS = 4 * RING + 14;
+  // pv_done[2], ml_full, ml_empty, o_done, o_free, turn[8]
+  static constexpr int NUM_BARS = 4 * RING + 22;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
   static constexpr int TOTAL = OFF_MISC + 16;  // tmem base, abort, non-finite drafts [2]
   static_assert(TOTAL <= 232448, "shared memory budget of one sm_100 CTA");
@@ -78,11 +80,13 @@ struct Layout {
 // Half an S tile of one query row (64 keys; this thread's TMEM lane): P = 2^(S sl - m) over the
 // first 32 columns, the running maximum m (log2 units) and the row sum l of this half. m moves only
 // when the true maximum grew by more than 2^8, so O is rescaled rarely; that waits for the PV
-// before. pv_done is at most one phase behind: S of this tile was issued behind the PV before that.
+// before. The exponentials start with this warp's turn and then hand it to `other`'s.
+// pv_done is at most one phase behind: S of this tile was issued behind the PV before that.
 template <bool MASKED, bool BF16, int D>
 __device__ __forceinline__ bool softmax_step(uint32_t t_s, uint32_t t_o, const uint32_t (&view)[2],
                                              float sl, float& m_used, float& lsum, uint64_t* pv_done,
-                                             uint32_t pv_parity, volatile int* abort,
+                                             uint32_t pv_parity, uint64_t* turn, uint64_t* other,
+                                             uint32_t turn_parity, volatile int* abort,
                                              unsigned int* status) {
   uint32_t r[HK];
 #pragma unroll
@@ -128,6 +132,7 @@ __device__ __forceinline__ bool softmax_step(uint32_t t_s, uint32_t t_o, const u
       tmem_st_32x32b_x16(t_o + c, o);
     }
   }
+  if (!wait_for(turn, turn_parity, abort, status, SITE_SM_TURN)) return false;
   // a row that has seen nothing keeps m = -inf: subtract 0 there, every exponential is 2^-inf
   const float m = m_used == -INFINITY ? 0.f : m_used;
   const uint64_t sl2 = f2(sl, sl);
@@ -143,6 +148,8 @@ __device__ __forceinline__ bool softmax_step(uint32_t t_s, uint32_t t_o, const u
     sum2[i & 3] = add2(sum2[i & 3], f2(e0, e1));
     pk[i] = pack2<BF16>(e0, e1);
   }
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(other);
   tmem_st_32x32b_x32(t_s, pk);
   tmem_st_wait();
   const uint64_t s01 = add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3]));
@@ -187,6 +194,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   uint64_t* ml_empty = ml_full + 1;  // ... and read
   uint64_t* o_done = ml_empty + 1;   // the segment's last PV
   uint64_t* o_free = o_done + 1;     // the epilogue has read both O
+  uint64_t* turn = o_free + 1;       // [softmax warp]: the exponentials of a tile are its own
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   unsigned int* bad = reinterpret_cast<unsigned int*>(smem + L::OFF_MISC + 8);   // [2]
@@ -213,6 +221,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     mbar_init(ml_empty, SOFTMAX_WARPS);
     mbar_init(o_done, 1);
     mbar_init(o_free, SOFTMAX_WARPS);
+    for (int i = 0; i < SOFTMAX_WARPS; ++i) mbar_init(&turn[i], 1);
     *abort_flag = 0;
     bad[0] = bad[1] = 0u;
     fence_barrier_init();
@@ -332,6 +341,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const uint32_t t_o = tmem + lane_base + COL_O;    // O of warpgroup 0; the other's is BN columns on
     const float sl = p.scale_log2;
     uint32_t g = 0;  // tiles of keys so far
+    uint32_t turns = 0;
     uint32_t o_phase = 0;
     bool ok = true;
     // what this thread's row of a segment sees
@@ -375,11 +385,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             view[0] = view_word(bits, k0 + wg * HK - w.ctx);
             view[1] = view_word(bits, k0 + wg * HK + 32 - w.ctx);
             ok = softmax_step<true, BF16, D>(at, t_o + wg * BN, view, sl, m_used, lsum, &pv_done[wg],
-                                             (g - 1) & 1u, abort_flag, p.status);
+                                             (g - 1) & 1u, &turn[warp], &turn[warp ^ 4],
+                                              (turns + wg + 1) & 1u, abort_flag, p.status);
           } else {
             ok = softmax_step<false, BF16, D>(at, t_o + wg * BN, view, sl, m_used, lsum, &pv_done[wg],
-                                              (g - 1) & 1u, abort_flag, p.status);
+                                              (g - 1) & 1u, &turn[warp], &turn[warp ^ 4],
+                                              (turns + wg + 1) & 1u, abort_flag, p.status);
           }
+          ++turns;
           if (!ok) break;
         }
         tc_fence_before();

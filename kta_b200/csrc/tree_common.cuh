@@ -36,6 +36,7 @@ enum : unsigned int {
   SITE_SM_ML = 0x909,
   SITE_SM_O = 0x90A,
   SITE_SM_PV = 0x90B,
+  SITE_SM_TURN = 0x90D,
   SITE_SMEM = 0x910,     // shared memory not aligned as declared
   SITE_REQUEST = 0x911,  // lengths or offsets out of range
   SITE_BLOCK = 0x912,    // a block id out of range
