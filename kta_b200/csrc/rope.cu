@@ -20,7 +20,8 @@
 // take 90.8 us (5920 GB/s; a plain copy of as many bytes 82.5) against 97.6 with 256 threads and
 // four items, 101 to 127 with 512 threads or without the streaming hints. Few tokens are latency:
 // there a thread has one item, and a token's heads are spread over several CTAs (512 tokens of 48
-// heads: 4.3 us with one item to a thread, 5.6 with 256 threads and four).
+// heads: 4.3 us with one item to a thread, 5.6 with 256 threads and four; 64 tokens 1.85 us). With the
+// cache write, 16384 tokens of 48 heads: 64.3 us, 6260 GB/s.
 #include <algorithm>
 #include <cmath>
 

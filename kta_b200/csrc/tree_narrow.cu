@@ -8,9 +8,16 @@
 //   S^T [128 keys, N] = K Q^T          (A = K tile, B = Q, both K-major in shared memory)
 //   O^T [D, N]       += V^T P^T        (A = V tile, MN-major; B = P, K-major in shared memory)
 //
-// The tensor work of a key tile falls with N. That matters although it was hidden before: with 128
-// rows of padding the SMs ran into the 1000 W cap at 1260 MHz and the stream with them (a context
-// of 131071 keys, 4 x 8 KV heads, one token: 396 us sustained, 330 us for short runs).
+// The tensor work of a key tile falls with N: with 128 rows of padding the SMs run into the 1000 W
+// cap at 1260 MHz, and the stream with them. From 33 rows on wide_kernel is faster all the same, since
+// the softmax here does a column at a time (64 rows: 235 us with N = 64, 197 there; 32 rows: 196 here,
+// 201 there; one request of 32 rows over 1000 keys 15.0 and 16.3).
+//
+// Measured: 4 x 131071 keys, 8 KV heads, one token of 4 heads: 330 us, 6500 GB/s (396 at 128 rows,
+// sustained). 64 requests of 8 tokens x 4 heads over 1k-8k keys, 8 KV heads: 197 us, 6180 GB/s. One
+// request of 8 tokens over 1000 keys: 11.3 us with its join, of which the launches and the plan are 5,
+// the loads' latency 2, one tile's chain of products and softmax 2, the join 2. 148 single tokens over
+// 100 keys: 25 us; a segment is a chain of ~3000 cycles there, a third of it walk and clean-up.
 //
 //   * Warps 0-3 softmax: warp w has keys 32 w .. 32 w + 31 of every tile, 16 keys at a time in the
 //     accumulator layout of 16x256b loads (a thread holds keys lane / 4 + 8 i and neighbouring
