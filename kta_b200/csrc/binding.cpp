@@ -3,7 +3,7 @@
 //
 // A decode step's small calls run for 2 to 5 us on the GPU. The same checks in Python with a ctypes
 // call took 18.5 us (rope), 21 us (cache_slots), 26 us (rope_cache) and 30 us (tree_attn) of host
-// time a call; here they take 4.7, 6.9, 5.0 and 11 (two launches and three tensor maps). Every function takes all its arguments by
+// time a call; here they take 3.8, 4.4, 5.0 and 10 (two launches and three tensor maps). Every function takes all its arguments by
 // position (ops.py holds the signatures and documents them), raises ValueError for tensors that do
 // not fit and kta_b200.lib.KtaError for a status code, launches on the current stream of the
 // tensors' device with that device current, and allocates what was not given with torch.
@@ -77,6 +77,19 @@ class On {
   }
   at::Tensor empty(at::IntArrayRef size, at::ScalarType type) const {
     return at::detail::empty_cuda(size, type, device_, c10::nullopt);  // without the dispatcher
+  }
+  // A tensor of n elements in `whole`, from byte `at` on; the next one starts on a 16-byte boundary.
+  static at::Tensor part(const at::Tensor& whole, int64_t& at, int64_t n, at::ScalarType type) {
+    const auto meta = c10::scalarTypeToTypeMeta(type);
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
+        c10::Storage(whole.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), meta);
+    t.unsafeGetTensorImpl()->set_storage_offset(at / static_cast<int64_t>(meta.itemsize()));
+    t.unsafeGetTensorImpl()->generic_set_sizes_contiguous(at::IntArrayRef(&n, 1));
+    at += bytes_of(n, type);
+    return t;
+  }
+  static int64_t bytes_of(int64_t n, at::ScalarType type) {
+    return (n * static_cast<int64_t>(c10::elementSize(type)) + 15) / 16 * 16;
   }
   void* stream() const { return c10::cuda::getCurrentCUDAStream(device_.index()).stream(); }
 
@@ -185,8 +198,18 @@ PyObject* cache_slots(PyObject*, PyObject* const* args, Py_ssize_t n) {
     vector(pool, at::kInt, -1, "free_blocks");
     block_tables(tables, batch);
     if (rows <= 0) refuse("max_tokens must be positive");
+    // What is not given is one allocation: with four a call takes 6.9 us of host time, so 4.4, and 3.0
+    // where all are given.
+    at::Tensor whole;
+    int64_t at = 0;
     auto made = [&](int i, int64_t size, at::ScalarType type, const char* name) -> at::Tensor {
-      if (!a.given(i)) return dev.empty({size}, type);
+      if (!a.given(i)) {
+        if (!whole.defined()) {
+          whole = dev.empty({On::bytes_of(rows, at::kLong) + On::bytes_of(rows, at::kInt) +
+                             On::bytes_of(batch + 1, at::kInt) + On::bytes_of(1, at::kInt)}, at::kByte);
+        }
+        return On::part(whole, at, size, type);
+      }
       const at::Tensor& t = a.tensor(i, name);
       dev.also(t);
       vector(t, type, size, name);

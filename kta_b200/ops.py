@@ -285,8 +285,9 @@ def cache_slots(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tables
     other entries are not touched). Returns, request after request, ``slots`` (int64
     [max_tokens], block * block_size + place) and ``positions`` (int32 [max_tokens]) of the new
     tokens, -1 and 0 behind the last one; ``offsets`` (int32 [B + 1], first row of each
-    request); ``used`` (int32 [1], blocks taken). What does not fit (a table's row, the free
-    list, max_tokens) is cut off and recorded in the device status block."""
+    request); ``used`` (int32 [1], blocks taken). What of them is not given shares one allocation.
+    What does not fit (a table's row, the free list, max_tokens) is cut off and recorded in the
+    device status block."""
     return (_native or _bind()).cache_slots(context_lens, new_lens, block_tables, free_blocks,
                                             block_size, max_tokens, slots, positions, offsets, used)
 

@@ -207,6 +207,33 @@ def test_values_that_a_row_does_not_see_do_not_reach_it(cuda_device, max_new, ct
     assert _status() == 0
 
 
+@pytest.mark.parametrize("max_new", [5, 64])
+def test_queries_that_are_not_finite_stay_in_their_rows(cuda_device, max_new):
+    c = Case([500, 90], [5, 3], 4, 2, 128, 16, BF16, seed=8)
+    want, want_lse = c.run(cuda_device, max_new=max_new)
+    c.check(want, want_lse)
+    keep = c.q.clone()
+    c.q[1, 2] = float("nan")
+    c.q[3, 0, 5] = float("inf")
+    c.q[6] = -float("inf")
+    out, lse = c.run(cuda_device, max_new=max_new)
+    same = torch.ones(8, 4, dtype=torch.bool)
+    same[1, 2] = same[3, 0] = same[6] = False
+    c.q = keep
+    assert torch.equal(out.cpu()[same], want.cpu()[same])
+    assert torch.equal(lse.cpu()[same], want_lse.cpu()[same])
+    assert torch.isnan(out.cpu()[1, 2]).all() and torch.isnan(out.cpu()[3, 0]).all()
+    assert _status() == 0
+
+
+def test_most_requests(cuda_device):
+    g = np.random.default_rng(9)
+    c = Case(g.integers(0, 40, 2048).tolist(), g.integers(0, 3, 2048).tolist(), 2, 1, 64, 8, F16, seed=9)
+    out, lse = c.run(cuda_device)
+    c.check(out, lse)
+    assert _status() == 0
+
+
 @pytest.mark.parametrize("max_new", [6, 32])
 def test_large_scores(cuda_device, max_new):
     """Scores up to some hundreds: the running maximum has to move, and O with it."""
