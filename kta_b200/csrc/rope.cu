@@ -17,10 +17,12 @@
 // in every layout keeps a warp's loads and stores contiguous.
 //
 // Small CTAs with two items to a thread in flight, and streaming loads and stores: 32768 x 32 heads
-// take 90.8 us (5920 GB/s; a plain copy of as many bytes 82.5) against 97.6 with 256 threads and
+// take 89.3 us (6010 GB/s; a plain copy of as many bytes 82.5) against 97.6 with 256 threads and
 // four items, 101 to 127 with 512 threads or without the streaming hints. Few tokens are latency:
 // there a thread has one item, and a token's heads are spread over several CTAs (512 tokens of 48
-// heads: 4.3 us with one item to a thread, 5.6 with 256 threads and four; 64 tokens 1.85 us). With the
+// heads: 4.3 us with one item to a thread, 5.6 with 256 threads and four; 64 tokens 1.85 us). With few
+// heads the angles are the work: a thread keeps its pair where it can, and its frequency's fraction
+// (32768 tokens of one head 13.6 us without, 9.8 so with more tokens to a CTA). With the
 // cache write, 16384 tokens of 48 heads: 64.3 us, 6260 GB/s.
 #include <algorithm>
 #include <cmath>
@@ -33,7 +35,7 @@ namespace rope {
 
 constexpr int THREADS = 128;
 constexpr int MAX_D = 1024;
-constexpr int MAX_TOKENS = 8;    // tokens of a CTA
+constexpr int MAX_TOKENS = 32;   // tokens of a CTA
 constexpr int VEC = 8;           // 16-byte vectors of 16-bit elements
 
 enum : unsigned int { SITE_SLOT = 0x811 };
@@ -54,6 +56,7 @@ struct Params {
   int pos64, rot, items, rot_items;  // items of a row, those of them that rotate
   int rest;                // vectors between an item's two in the region that is copied
   int per_cta;             // tokens of a CTA
+  int half_log2;           // of rot / 2 where that divides THREADS, else -1
   float scale, sign;
   unsigned int* status;
 };
@@ -183,16 +186,25 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const Params p) {
     }
     if (!table) {  // once, behind the first loads
       table = true;
-      for (int i = threadIdx.x; i < tokens * half; i += THREADS) {
-        const int t = i / half, f = i - t * half;
+      auto angle = [&](int t, int f, uint64_t fraction) {
         const long long pos = p.pos64 ? static_cast<const int64_t*>(p.positions)[token0 + t]
                                       : static_cast<const int32_t*>(p.positions)[token0 + t];
-        const uint64_t phase = static_cast<uint64_t>(pos) * turn_fraction(p.freqs[f]);
+        const uint64_t phase = static_cast<uint64_t>(pos) * fraction;
         // half turns in [-1, 1)
         const float x = static_cast<float>(static_cast<int32_t>(phase >> 32)) * 4.656612873077393e-10f;
         float s, c;
         sincospif(x, &s, &c);
-        turn[i] = make_float2(c * p.scale, s * p.scale * p.sign);
+        turn[t * half + f] = make_float2(c * p.scale, s * p.scale * p.sign);
+      };
+      if (!SPREAD && p.half_log2 >= 0) {  // a thread keeps its pair
+        const int f = threadIdx.x & (half - 1);
+        const uint64_t fraction = turn_fraction(p.freqs[f]);
+        for (int t = threadIdx.x >> p.half_log2; t < tokens; t += THREADS >> p.half_log2) angle(t, f, fraction);
+      } else {
+        for (int i = threadIdx.x; i < tokens * half; i += THREADS) {
+          const int t = i / half, f = i - t * half;
+          angle(t, f, turn_fraction(p.freqs[f]));
+        }
       }
       __syncthreads();
     }
@@ -289,6 +301,10 @@ int go(Params& p, int64_t D, bool interleaved, cudaStream_t stream) {
     p.items = p.rot_items;
   }
   p.status = device_status_ptr();
+  p.half_log2 = -1;
+  for (int i = 0; 1 << i <= THREADS; ++i) {
+    if (p.rot == 2 << i) p.half_log2 = i;
+  }
   const long long per_token = static_cast<long long>(p.rows) * p.items;
   const int sms = current_sm_count();
   // One item to a thread while all of them are resident at once (2048 threads to an SM), if a token
@@ -299,9 +315,12 @@ int go(Params& p, int64_t D, bool interleaved, cudaStream_t stream) {
     const dim3 grid(p.tokens, static_cast<unsigned>((per_token + THREADS - 1) / THREADS));
     return start<T, CACHE, 1, true>(p, grid, interleaved, stream);
   }
-  // Tokens of a CTA: four items for a thread, but never fewer CTAs than fill the SMs.
+  // Tokens of a CTA: four items for a thread, but never fewer CTAs than fill the SMs, nor more than
+  // eight tokens where they give every thread an item (32768 tokens of one head: 10.3 us with 16
+  // tokens, 12.3 with 8; of four heads 15.8 with 8, 18.3 with 16).
   int per = 1;
-  while (per < MAX_TOKENS && per * per_token < 4 * THREADS && p.tokens / (2 * per) >= 8 * sms) per *= 2;
+  const int most = std::max(1, std::min(MAX_TOKENS, 4096 / p.rot));  // and 16 KB of cos and sin
+  while (per < most && per * per_token < (per < 8 ? 4 : 1) * THREADS && p.tokens / (2 * per) >= 8 * sms) per *= 2;
   p.per_cta = per;
   return start<T, CACHE, 2, false>(p, dim3((p.tokens + per - 1) / per), interleaved, stream);
 }

@@ -57,7 +57,8 @@ def test_forward_and_gradient(cuda_device, n, h, d, rot, interleaved, dtype):
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
-@pytest.mark.parametrize("n,h,d,rot", [(5000, 8, 128, 128), (20001, 2, 128, 96), (2400, 20, 256, 64)])
+@pytest.mark.parametrize("n,h,d,rot", [(5000, 8, 128, 128), (20001, 2, 128, 96), (2400, 20, 256, 64),
+                                       (40000, 1, 64, 64)])
 def test_more_than_a_wave(cuda_device, n, h, d, rot, interleaved):
     """Several items to a thread, and several tokens to a CTA; in place, what does not turn stays."""
     from kta_b200 import ops
