@@ -73,7 +73,8 @@ struct Layout {
   // pv_done[2], ml_full, ml_empty, o_done, o_free, turn[8]
   static constexpr int NUM_BARS = 4 * RING + 22;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
-  static constexpr int TOTAL = OFF_MISC + 16;  // tmem base, abort, non-finite drafts [2]
+  static constexpr int OFF_PLAN = OFF_MISC + 16;  // after tmem base, abort, non-finite drafts [2]
+  static constexpr int TOTAL = OFF_PLAN + PLAN_BYTES;
   static_assert(TOTAL <= 232448, "shared memory budget of one sm_100 CTA");
 };
 
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   pdl_wait();  // the previous grid's writes (this launch's inputs) are visible from here on
   // after the wait: the join kernel may be scheduled now, and waits for this grid itself
   pdl_launch_dependents();
-  Walk<false> w = plan<D, false>(p, smem + L::OFF_K);
+  Walk<false> w = plan<D, false>(p, smem + L::OFF_PLAN);
   // K and V that one row tile reads once leave L2 first (64 requests of 8 tokens, 8 heads to a KV head,
   // 1024 to 8192 keys: 197 us, 205 without); members of a share find them there.
   const uint64_t policy = p.row_tiles > 1 ? l2_policy_evict_normal() : l2_policy_evict_first();

@@ -161,14 +161,13 @@ struct Shares {
   }
 };
 
-// The tile that holds a position of the list.
-struct Place {
-  int b, kvh, tile, at;  // at: its own position
-  int unit, unit_end;    // of its (request, KV head)
-  int k;                 // row tiles of the request
+// The request that holds a position of the list.
+struct Holder {
+  int b, start;  // start: its own position
+  int unit;      // what one of its (request, KV head) takes of the list
   int row, tokens, ctx;
 };
-constexpr int PLAN_BYTES = 128 + 2 * static_cast<int>(sizeof(Place));  // shared memory of plan()
+constexpr int PLAN_BYTES = 128 + 2 * static_cast<int>(sizeof(Holder));  // shared memory of plan()
 
 // A CTA's walk over the segments of its share: runs of count() tiles from i0 on of one (request, KV
 // head). Every warp walks by itself, beside its work: what a request's tiles are is kept, no division
@@ -239,31 +238,31 @@ struct Walk {
 
 // The start of every CTA, after griddepcontrol.wait: places its share and returns the walk over it
 // (left is 0 where it has none); member 0 describes the unit that the share's end cuts. By all
-// threads, which it synchronises; `scratch` is PLAN_BYTES of shared memory. Rows of requests that
-// are out of range become zero.
+// threads; `scratch` is PLAN_BYTES of shared memory for this alone, so that each warp goes on by
+// itself from the last barrier. Rows of requests that are out of range become zero.
 template <int D, bool ONE>
 __device__ __forceinline__ Walk<ONE> plan(const Params& p, uint8_t* scratch) {
-  // The block tables into L2, a line for a thread: a producer that misses it waits behind the
-  // stream's own reads.
-  const int lines = (p.max_blocks * 4 + 127) / 128;
-  const long long line = static_cast<long long>(threadIdx.x) * gridDim.x + blockIdx.x;
-  if (line < static_cast<long long>(lines) * p.batch) {
-    const int b = static_cast<int>(line / lines);
-    const int32_t* at = p.tables + b * p.table_stride + (line - static_cast<long long>(b) * lines) * 32;
-    asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
-  }
   int2* warp_sum = reinterpret_cast<int2*>(scratch);
-  volatile Place* places = reinterpret_cast<volatile Place*>(scratch + 128);
+  volatile Holder* holders = reinterpret_cast<volatile Holder*>(scratch + 128);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = (p.batch + NUM_THREADS - 1) / NUM_THREADS;  // requests of a thread
   const int b0 = min(static_cast<int>(threadIdx.x) * per, p.batch), b1 = min(b0 + per, p.batch);
   // a thread's first request is kept: with up to 384 of them nothing is loaded twice
   Request kept = {};
+  if (b0 < b1) kept = request_of(p, b0);
+  // The block tables into L2, a line for a thread: a producer that misses it waits behind the
+  // stream's own reads.
+  const unsigned lines = (static_cast<unsigned>(p.max_blocks) + 31u) / 32u;  // of a request
+  const unsigned line = threadIdx.x * gridDim.x + blockIdx.x;
+  if (line < static_cast<unsigned long long>(lines) * p.batch) {
+    const unsigned b = line / lines;
+    const int32_t* at = p.tables + b * p.table_stride + (line - b * lines) * 32u;
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+  }
   int2 mine = make_int2(0, 0);  // tiles and units of the thread's requests, for each row tile
   bool bad = false;
   for (int b = b0; b < b1; ++b) {
-    const Request r = request_of(p, b);
-    if (b == b0) kept = r;
+    const Request r = b == b0 ? kept : request_of(p, b);
     const int k = p.hkv * (ONE ? 1 : row_tiles_of(p, r.tokens)), n = tiles_of(r);
     mine.x += n * k;
     mine.y += n > 0 ? k : 0;
@@ -285,37 +284,32 @@ __device__ __forceinline__ Walk<ONE> plan(const Params& p, uint8_t* scratch) {
     all = make_int2(all.x + v.x, all.y + v.y);
   }
   const Shares sh(p, all.x, all.y);
-  const int before = ahead.x + sh.extra * ahead.y, sum = mine.x + sh.extra * mine.y;
   const int share = ONE ? blockIdx.x : static_cast<int>(blockIdx.x) / p.row_tiles;
   const int member = ONE ? 0 : static_cast<int>(blockIdx.x) - share * p.row_tiles;
-  if (share < sh.n && sum > 0) {
-    // the starts of the share and of the next one, by the threads that hold them
-    for (int q = 0; q < 2; ++q) {
-      const int at = sh.start(share + q);
-      if (at < before || at >= before + sum) continue;
+  const int at0 = sh.start(share), at1 = sh.start(share + 1);
+  if (share < sh.n) {
+    // the requests with the starts of the share and of the next one, by the threads that have them
+    const int before = ahead.x + sh.extra * ahead.y, end = before + mine.x + sh.extra * mine.y;
+    const bool has0 = at0 >= before && at0 < end, has1 = at1 >= before && at1 < end;
+    if (has0 || has1) {
       int t = before;
       for (int b = b0; b < b1; ++b) {
         const Request r = b == b0 ? kept : request_of(p, b);
         const int k = ONE ? 1 : row_tiles_of(p, r.tokens);
-        const int pair = tiles_of(r) > 0 ? (tiles_of(r) + sh.extra) * k : 0;
-        if (at >= t + pair * p.hkv) {
-          t += pair * p.hkv;
-          continue;
+        const int unit = tiles_of(r) > 0 ? (tiles_of(r) + sh.extra) * k : 0;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int at = q == 0 ? at0 : at1;
+          if (at < t || at >= t + unit * p.hkv) continue;
+          volatile Holder* z = holders + q;
+          z->b = b;
+          z->start = t;
+          z->unit = unit;
+          z->row = r.row;
+          z->tokens = r.tokens;
+          z->ctx = r.ctx;
         }
-        volatile Place* z = places + q;
-        const int kvh = (at - t) / pair, unit = t + kvh * pair;
-        const int tile = max((at - unit) / k - sh.extra, 0);
-        z->b = b;
-        z->kvh = kvh;
-        z->tile = tile;
-        z->at = unit + (tile > 0 ? tile + sh.extra : 0) * k;
-        z->unit = unit;
-        z->unit_end = unit + pair;
-        z->k = k;
-        z->row = r.row;
-        z->tokens = r.tokens;
-        z->ctx = r.ctx;
-        break;
+        t += unit * p.hkv;
       }
     }
   }
@@ -335,36 +329,46 @@ __device__ __forceinline__ Walk<ONE> plan(const Params& p, uint8_t* scratch) {
   Walk<ONE> w = {};
   w.extra = sh.extra;
   w.member = member;
-  int cut = 0;  // shares that hold a part of the unit that starts in this one and ends later
+  Desc cut = {};  // of the unit that starts in this share and ends in a later one
   if (share < sh.n) {
+    // Of position `at` of the list: the tile that holds it, the tile's own position, its unit's.
+    struct Place {
+      int kvh, tile, at, unit, unit_end;
+    };
+    auto place = [&](volatile Holder& h, int at, int k) -> Place {
+      Place z;
+      const int length = h.unit;
+      z.kvh = (at - h.start) / length;
+      z.unit = h.start + z.kvh * length;
+      z.unit_end = z.unit + length;
+      const int in = at - z.unit;
+      z.tile = max((ONE || k == 1 ? in : in / k) - sh.extra, 0);
+      z.at = z.unit + (z.tile > 0 ? z.tile + sh.extra : 0) * k;
+      return z;
+    };
+    w.enter(p, holders[0].row, holders[0].tokens, holders[0].ctx);
+    const Place from = place(holders[0], at0, w.k);
     int end = sh.total;
     if (share + 1 < sh.n) {
-      end = places[1].at;
+      const int k = ONE ? 1 : row_tiles_of(p, holders[1].tokens);
+      const Place to = place(holders[1], at1, k);
+      end = to.at;
+      const int rt = threadIdx.x;
       // the next share starts inside a unit, and that unit starts in this one
-      if (end > places[1].unit && places[1].unit >= places[0].at) {
-        cut = sh.before(places[1].unit_end) - share + 1;
+      if (rt < p.row_tiles && rt < k && end > to.unit && to.unit >= from.at) {
+        cut.span = sh.before(to.unit_end) - share + 1;
+        cut.row = holders[1].row + rt * p.tok_tile;
+        cut.tokens = min(holders[1].tokens - rt * p.tok_tile, p.tok_tile);
+        cut.kvh = to.kvh;
       }
     }
-    w.b = places[0].b;
-    w.kvh = places[0].kvh;
-    w.i0 = places[0].tile;
-    w.left = end - places[0].at;
-    w.enter(p, places[0].row, places[0].tokens, places[0].ctx);
+    w.b = holders[0].b;
+    w.kvh = from.kvh;
+    w.i0 = from.tile;
+    w.left = end - from.at;
     w.settle(p);
   }
-  if (member == 0 && threadIdx.x < p.row_tiles) {
-    const int rt = threadIdx.x;
-    Desc d = {};
-    if (cut > 0 && rt < places[1].k) {
-      d.span = cut;
-      d.row = places[1].row + rt * p.tok_tile;
-      d.tokens = min(places[1].tokens - rt * p.tok_tile, p.tok_tile);
-      d.kvh = places[1].kvh;
-    }
-    p.desc[blockIdx.x + rt] = d;
-  }
-  fence_proxy_async_smem();  // the scratch's use comes before TMA writes to the same memory
-  __syncthreads();
+  if (member == 0 && threadIdx.x < p.row_tiles) p.desc[blockIdx.x + threadIdx.x] = cut;
   return w;
 }
 

@@ -69,7 +69,8 @@ struct Narrow {
   static constexpr int NUM_BARS = 4 * RING + 2 * Q_BUFS + 12;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
   // misc: tmem base, abort, non-finite drafts [2], correction requests [2][4]
-  static constexpr int TOTAL = OFF_MISC + 48;
+  static constexpr int OFF_PLAN = OFF_MISC + 48;
+  static constexpr int TOTAL = OFF_PLAN + PLAN_BYTES;
   static_assert(TOTAL <= 232448, "shared memory budget of one sm_100 CTA");
   // TMEM: S^T of buffer i at i N, O^T of warp w at (2 + w) N
   static constexpr uint32_t COL_O = 2 * N;
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   pdl_wait();  // the previous grid's writes (this launch's inputs) are visible from here on
   // after the wait: the join kernel may be scheduled now, and waits for this grid itself
   pdl_launch_dependents();
-  Walk<true> w = plan<D, true>(p, smem + L::OFF_K);
+  Walk<true> w = plan<D, true>(p, smem + L::OFF_PLAN);
 
   // K and V are read once: evict first, and the tables, partials and code stay in L2
   if (warp == K_WARP) {
