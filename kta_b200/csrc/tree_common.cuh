@@ -1,5 +1,5 @@
 // What the two tree-attention kernels (tree.cu: many query rows, tree_narrow.cu: up to 32) share:
-// the work list of a launch, the walk of a CTA over its range, the TMA producers, and the clean-up
+// the work list of a launch, the walk of a CTA over its share, the TMA producers, and the clean-up
 // of V tiles that end inside a page. The operator is described in tree.cu.
 #pragma once
 

@@ -15,7 +15,7 @@
 //
 // Measured: 4 x 131071 keys, 8 KV heads, one token of 4 heads: 330 us, 6500 GB/s (396 at 128 rows,
 // sustained). 64 requests of 8 tokens x 4 heads over 1k-8k keys, 8 KV heads: 197 us, 6180 GB/s. One
-// request of 8 tokens over 1000 keys: 11.3 us with its join, of which the launches and the plan are 5,
+// request of 8 tokens over 1000 keys: 11.2 us with its join, of which the launches and the plan are 5,
 // the loads' latency 2, one tile's chain of products and softmax 2, the join 2. 148 single tokens over
 // 100 keys: 25 us; a segment is a chain of ~3000 cycles there, a third of it walk and clean-up.
 //
