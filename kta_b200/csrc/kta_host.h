@@ -19,12 +19,14 @@ int current_sm_count();
 // Compute capability major of the current device; -1 on error.
 int current_cc_major();
 
-// Encodes a tiled tensor map (rank 2 or 3) through the driver's cuTensorMapEncodeTiled,
+// Encodes a tiled tensor map (rank 2 to 5) through the driver's cuTensorMapEncodeTiled,
 // resolved with cudaGetDriverEntryPoint (the library does not link libcuda).
 // dims/strides are innermost-first; strides_bytes holds rank-1 entries (dims 1..rank-1).
+// promotion: what L2 fetches from HBM at least, for a row of the box.
 int encode_tmap(CUtensorMap* map, CUtensorMapDataType dtype, int rank, const void* base,
                 const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
-                CUtensorMapSwizzle swizzle);
+                CUtensorMapSwizzle swizzle,
+                CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 
 // Maps the pending CUDA error of the last launch to a status code.
 int launch_status();
