@@ -304,12 +304,15 @@ def rope_freqs(rot: int, base: float = 10000.0, *, scaling: str | None = None, f
       and the highest kept;
     - "bands": frequencies that make fewer than ``low_turns`` turns in original_len tokens are
       divided by factor, those of more than ``high_turns`` kept, a linear ramp in between;
-    - "yarn": the same ramp over the pair index between the two bounds, and scale
-      1 + 0.1 ln(factor)."""
+    - "yarn": the same ramp over the pair index between the two bounds (rounded outward to whole
+      indices, in 0 .. rot - 1: the one for low_turns may lie behind the last pair), and scale
+      1 + 0.1 ln(factor). base > 1."""
     if rot < 2 or rot % 2:
         raise ValueError("rot must be even and positive")
     if not (base > 0 and factor >= 1 and original_len > 0 and 0 < low_turns < high_turns):
         raise ValueError("base > 0, factor >= 1, original_len > 0, 0 < low_turns < high_turns")
+    if scaling == "yarn" and base <= 1:
+        raise ValueError("yarn scaling needs base > 1: frequencies that fall with the pair index")
     if scaling == "ntk":
         if rot == 2:
             raise ValueError("ntk scaling needs more than one pair")
@@ -329,7 +332,8 @@ def rope_freqs(rot: int, base: float = 10000.0, *, scaling: str | None = None, f
                 return rot * math.log(original_len / (turns * 2 * math.pi)) / (2 * math.log(base))
 
             first = max(math.floor(index(high_turns)), 0)
-            last = max(min(math.ceil(index(low_turns)), rot // 2 - 1), first)
+            # rot - 1, not the last pair: a ramp that ends behind it does not divide it fully
+            last = max(min(math.ceil(index(low_turns)), rot - 1), first)
             keep = 1.0 - (pair - first) / max(last - first, 0.001)
             scale = 1.0 + 0.1 * math.log(factor)
         keep = keep.clamp(0.0, 1.0)

@@ -198,6 +198,45 @@ def test_rope_freqs():
             ops.rope_freqs(device="cpu", **bad)
 
 
+def _yarn(rot, base, factor, original_len, low_turns=1.0, high_turns=32.0):
+    """The ramp pair by pair: pair index x makes original_len base^(-2 x / rot) / (2 pi) turns, solved for
+    x at both bounds; whole indices outward, in 0 .. rot - 1 (the upper one may lie past the last pair)."""
+    def index(turns):
+        return rot / 2 * math.log(original_len / (2 * math.pi * turns), base)
+
+    low, high = max(math.floor(index(high_turns)), 0), min(math.ceil(index(low_turns)), rot - 1)
+    out = []
+    for i in range(rot // 2):
+        divided = min(max((i - low) / (high - low), 0.0), 1.0)
+        out.append(base ** (-2 * i / rot) * (1 - divided + divided / factor))
+    return out
+
+
+@pytest.mark.parametrize("rot,base,original_len,bounds,last", [
+    (64, 10000.0, 4096, (10, 23), 0.25),               # both bounds among the pairs
+    (64, 10000.0, 131072, (22, 35), 0.25 + 0.75 * 4 / 13),   # the upper one past the last pair, 31
+    (128, 10000.0, 131072, (45, 70), 0.25 + 0.75 * 7 / 25),  # ... 63
+    (16, 10000.0, 32768, (4, 8), 0.25 + 0.75 * 1 / 4),       # ... 7
+    (64, 100.0, 1 << 30, (107, 63), 1.0),              # even the lower one: every frequency is kept
+])
+def test_yarn_ramp_between_its_bounds(rot, base, original_len, bounds, last):
+    """The bounds by hand: rot / 2 * log_base(original_len / (2 pi turns))."""
+    freqs, _ = ops.rope_freqs(rot, base, scaling="yarn", factor=4.0, original_len=original_len, device="cpu")
+    plain = base ** (-2.0 * (rot // 2 - 1) / rot)
+    assert math.isclose(freqs[-1], plain * last, rel_tol=1e-12)
+    low, high = bounds
+    if low < high:
+        assert np.allclose(freqs.numpy(), _yarn(rot, base, 4.0, original_len), rtol=1e-12, atol=0)
+        if low + 1 < rot // 2:
+            assert freqs[low] == base ** (-2.0 * low / rot) and freqs[low + 1] < base ** (-2.0 * (low + 1) / rot)
+
+
+def test_yarn_needs_frequencies_that_fall():
+    for base in (1.0, 0.5):  # every pair turns as fast as the first, or faster: no index has the turns
+        with pytest.raises(ValueError):
+            ops.rope_freqs(64, base, scaling="yarn", factor=2.0, device="cpu")
+
+
 def test_float64_forms():
     """The oracle on cases that can be told by hand."""
     assert paged.tree_bits([-1, 0, 0, 1]) == [1, 3, 5, 11]
