@@ -32,16 +32,39 @@ def cache_slots(ctx, new, tables, free, block: int, rows: int):
     return tables, slots, positions, np.array(offsets), min(taken, len(free))
 
 
+_TURN_BITS = 320
+
+
+def _radian() -> int:
+    """1 / (2 pi) in units of 2^-_TURN_BITS of a turn, pi from Machin's 4 (4 acot 5 - acot 239) in integers."""
+    bits = _TURN_BITS + 32
+
+    def acot(n: int) -> int:
+        power = total = (1 << bits) // n
+        k = 1
+        while power:
+            power //= -n * n
+            k += 2
+            total += power // k
+        return total
+
+    return (1 << (bits + _TURN_BITS)) // (8 * (4 * acot(5) - acot(239)))
+
+
+_RADIAN = _radian()
+
+
 def rope(x, positions, freqs, interleaved: bool, inverse: bool = False, scale: float = 1.0):
-    """x [N, H, D] float64; whole turns are taken off in exact integers, so that positions of any
-    size keep their angle."""
+    """x [N, H, D] float64; the frequencies become turns and whole turns are taken off in integers of
+    320 bits, so that positions of any size keep their angle."""
     x = np.asarray(x, dtype=np.float64)
     y = x.copy()
     half = len(freqs)
     for i, f in enumerate(freqs):
         a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + half)
-        turn = round(float(f) / (2 * math.pi) * 2.0 ** 80)
-        t = np.array([(int(n) * turn % (1 << 80)) / 2.0 ** 80 for n in positions]) * 2 * math.pi
+        num, den = float(f).as_integer_ratio()
+        t = np.array([int(n) * num * _RADIAN // den % (1 << _TURN_BITS) / (1 << _TURN_BITS)
+                      for n in positions]) * 2 * math.pi
         t = (-t if inverse else t)[:, None]
         y[..., a] = scale * (x[..., a] * np.cos(t) - x[..., b] * np.sin(t))
         y[..., b] = scale * (x[..., b] * np.cos(t) + x[..., a] * np.sin(t))

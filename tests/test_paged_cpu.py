@@ -253,3 +253,11 @@ def test_float64_forms():
     q, k = np.zeros((1, 2)), np.ones((3, 2))
     out, lse, *_ = paged.attention(q, k, np.arange(6.0).reshape(3, 2), np.array([[True, True, False]]), 1.0)
     assert np.allclose(out, [[1, 2]]) and math.isclose(lse[0], math.log(2))
+
+
+def test_rope_oracle_at_far_positions():
+    """Against libm's sine and cosine, which reduce any argument; position * frequency is exact here."""
+    for f, n in ((1.0, 2**40 + 3), (1.0, -2**53 + 1), (0.75, 2**50 + 1), (1.0 + 2.0 ** -20, 2**31 - 1),
+                 (96.0, 2**46 + 5), (-3.0, 2**51 - 1)):
+        y = paged.rope(np.array([[[1.0, 0.0]]]), [n], [f], True)[0, 0]
+        assert np.allclose(y, [math.cos(n * f), math.sin(n * f)], rtol=0, atol=4e-16), (f, n)
