@@ -173,7 +173,8 @@ int kta_cache_slots(const void* context_lens, const void* new_lens, void* block_
  * `inverse` turns by -t: the gradient with respect to X of the same call. X, Y [tokens, heads, D]
  * with token and head strides in elements (X's may be 0: one row for all); positions int32 or
  * int64 (pos_bytes 4 or 8, any sign), freqs fp64 [rot / 2] finite radians per position. The angle
- * is reduced exactly for any position. X and Y may be the same tensor, and must not overlap
+ * is off by at most |position| 2^-64 turns and one fp32 rounding of what is left of it without whole
+ * turns: 1e-7 rad below position 2^38, 3e-3 rad at 2^53. X and Y may be the same tensor, and must not overlap
  * otherwise. D % 16 == 0, D <= 1024, rot % 16 == 0, strides multiples of 8, 16-byte aligned X, Y. */
 int kta_rope_f16(const void* X, const void* positions, int64_t pos_bytes, const void* freqs, void* Y,
                  int64_t tokens, int64_t heads, int64_t D, int64_t rot, int64_t x_token,

@@ -5,10 +5,11 @@
 //   (a, b) -> scale (a cos t - b sin t, b cos t + a sin t),   t = position * freq_i
 //   dimensions from rot on are copied; the gradient is the same map with -t (its transpose).
 //
-// The angle is kept in turns as a 64-bit fraction: f = frac(freq / 2 pi) 2^64 is an integer, and
-// position * f mod 2^64 drops whole turns exactly, so a position of a million loses nothing (a
-// 32-bit product would be off by 0.06 rad there) and the only 32-bit rounding is that of the
-// reduced angle (2^-25 of a half turn). Rotation in fp32, one rounding to the storage type.
+// The angle is kept in turns as a 64-bit fraction: f = frac(freq / 2 pi) 2^64 is an integer, off by
+// at most one, and position * f mod 2^64 drops whole turns exactly. So an angle is off by |position|
+// 2^-64 turns (4e-7 rad at 2^40; a 32-bit product would be off by 0.06 rad at a million) and by the
+// one 32-bit rounding, that of the reduced angle (2^-25 of a half turn). Rotation in fp32, one
+// rounding to the storage type.
 //
 // HBM-bound: 4 bytes per element (read once, written once). A CTA takes a few tokens: its threads
 // first put their loads in flight, then compute the tokens' cos and sin once into shared memory
@@ -78,10 +79,17 @@ __device__ __forceinline__ uint32_t pack<__half>(float a, float b) { return pack
 template <>
 __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
 
-// frac(freq / 2 pi) as a 64-bit fraction of a turn.
+// frac(freq / 2 pi) as a 64-bit fraction of a turn, within 2^-64 for |freq| < 2^40. 1 / (2 pi) in two
+// parts, and the first product's rounding error by fma (Dekker's exact product): one product in 64
+// bits would be off by 2^-53 of the frequency, which a position of 2^40 makes 7e-5 rad. The rest is
+// small enough to become an integer by an addition.
 __device__ __forceinline__ uint64_t turn_fraction(double freq) {
-  const double turns = freq * 0.15915494309189535;  // 1 / (2 pi)
-  return static_cast<uint64_t>((turns - floor(turns)) * 18446744073709551616.0);
+  constexpr double HI = 0x1.45f306dc9c883p-3, LO = -0x1.6b01ec5417056p-57;
+  constexpr double ONES = 0x1.8p52;  // doubles around it are the whole numbers
+  const double turns = freq * HI, rest = fma(freq, LO, fma(freq, HI, -turns));
+  const long long whole = __double2ll_rn((turns - rint(turns)) * 0x1p64);  // of [-1/2, 1/2] turns
+  const long long more = __double_as_longlong(fma(rest, 0x1p64, ONES)) - __double_as_longlong(ONES);
+  return static_cast<uint64_t>(whole + (fabs(freq) < 0x1p40 ? more : 0));
 }
 
 // An item's place: source, destination and first vector's two element offsets, its token in the
@@ -130,9 +138,11 @@ __device__ __forceinline__ Item<T> item_at(const Params& p, int token0, int toke
 }
 
 // UNROLL: items of a thread whose loads are in flight together. SPREAD: a token's items over
-// gridDim.y CTAs, one for a thread.
+// gridDim.y CTAs, one for a thread; twelve of them to an SM (with 48 registers, and so ten, 64 tokens of
+// 32 heads take 2.8 us, not 2.4). Nine otherwise (with 64 registers, and so eight, 32768 tokens of 32
+// heads take 95 us, not 92).
 template <typename T, bool INTER, bool CACHE, int UNROLL, bool SPREAD>
-__global__ void __launch_bounds__(THREADS) rope_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, SPREAD ? 12 : 9) rope_kernel(const Params p) {
   extern __shared__ float2 turn[];  // [tokens of the CTA][rot / 2] scale * (cos, sin)
   __shared__ long long slot[MAX_TOKENS];
   pdl_launch_dependents();

@@ -191,3 +191,34 @@ def test_rope_cache(cuda_device, n, hq, hkv, d, rot, bs, interleaved, dtype):
     want_k.fill_(3.0).flatten(0, 1)[slots[on]] = turned[on]
     assert torch.equal(kc2, want_k)
     assert lib.device_status(clear=True)[0] == 9
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("freqs", ["model", "turning"])
+def test_positions_past_32_bits(cuda_device, freqs, interleaved):
+    """A frequency's fraction of a turn is off by 2^-64, so an angle by |position| 2^-64 turns and the
+    reduced angle's rounding to fp32 (the 1e-7 rad in _close's 6e-7): tight at 2^40, 3e-3 rad at 2^53. In
+    both forms of the kernel (a token's heads over several CTAs, and several tokens to a CTA)."""
+    from kta_b200 import ops
+
+    dev = cuda_device
+    if freqs == "model":
+        f, _ = ops.rope_freqs(64, 500000.0, device="cpu")
+    else:  # more than a turn to a position, and negative ones
+        f = torch.linspace(-40.0, 90.0, 32, dtype=torch.float64)
+    far = [2**31 - 1, -2**31, 2**32 + 1, 2**40 + 3, -2**40 - 77, 2**47 + 12345, 2**53 - 1, -2**53]
+    for n, h in ((len(far), 32), (5000, 1)):
+        pos = (far * n)[:n]
+        x = _x((n, h, 64), torch.float16, 11)
+        got = ops.rope(x.to(dev), torch.tensor(pos, dtype=torch.int64).to(dev), f.to(dev),
+                       interleaved=interleaved).double().cpu().numpy()
+        x = x.double().numpy()
+        want = paged.rope(x, pos, f.tolist(), interleaved)
+        turned = paged.rope(np.abs(x), [0] * n, f.tolist(), interleaved)  # |x|, and its pair's other one
+        other = (turned.reshape(n, h, 32, 2)[..., ::-1].reshape(n, h, 64) if interleaved
+                 else np.roll(turned, 32, -1))
+        angle = 6e-7 + 2 * np.pi * 2.0 ** -64 * np.abs(np.array(pos, dtype=np.float64))[:, None, None]
+        fp32 = angle * (turned + other)
+        half = torch.finfo(torch.float16).eps / 2
+        tiny = torch.finfo(torch.float16).smallest_normal * half
+        assert (np.abs(got - want) <= fp32 + half * (np.abs(want) + fp32) + tiny).all()
