@@ -12,6 +12,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -28,6 +29,7 @@ struct Refused {  // becomes a ValueError
 [[noreturn]] void refuse(const std::string& why) { throw Refused{why}; }
 
 PyObject* g_check = nullptr;  // kta_b200.lib.check, set by the module's user
+PyObject* g_rope = nullptr;   // rope() as a node of autograd's graph, set by kta_b200.ops
 
 // Raises KtaError for a status code.
 bool passed(const char* entry, int status) {
@@ -251,6 +253,13 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
       rows_like(out, x, "out");
       if (out.size(1) != x.size(1)) refuse("out must have X's heads");
     }
+    if (c10::GradMode::is_enabled() &&
+        (x.requires_grad() || freqs.requires_grad() || (a.given(6) && a.tensor(6, "out").requires_grad()))) {
+      if (freqs.requires_grad()) refuse("there is no gradient of freqs: detach them");
+      if (a.given(6)) refuse("out cannot carry a gradient: leave it out, or use torch.no_grad()");
+      if (g_rope == nullptr) refuse("kta_b200.ops is not loaded");
+      return PyObject_Vectorcall(g_rope, a.at, 6, nullptr);  // which comes back with gradients off
+    }
     On dev(x);
     dev.also(positions);
     dev.also(freqs);
@@ -380,10 +389,12 @@ PyObject* tree_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-PyObject* set_check(PyObject*, PyObject* f) {
+// What the functions above call.
+template <PyObject*& F>
+PyObject* set_call(PyObject*, PyObject* f) {
   Py_INCREF(f);
-  Py_XDECREF(g_check);
-  g_check = f;
+  Py_XDECREF(F);
+  F = f;
   Py_RETURN_NONE;
 }
 
@@ -392,7 +403,9 @@ PyObject* set_check(PyObject*, PyObject* f) {
 PyMethodDef g_methods[] = {
     {"cache_slots", FAST(cache_slots), nullptr}, {"rope", FAST(rope), nullptr},
     {"rope_cache", FAST(rope_cache), nullptr},   {"tree_attn", FAST(tree_attn), nullptr},
-    {"set_check", set_check, METH_O, nullptr},   {nullptr, nullptr, 0, nullptr},
+    {"set_check", set_call<g_check>, METH_O, nullptr},
+    {"set_rope", set_call<g_rope>, METH_O, nullptr},
+    {nullptr, nullptr, 0, nullptr},
 };
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, g_methods,

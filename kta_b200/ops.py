@@ -260,7 +260,8 @@ def decode_gqa(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
 
 
 # ---- paged KV cache -------------------------------------------------------------------------
-# Short calls: tensor checks, allocation and launch are native code (csrc/binding.cpp).
+# Short calls: tensor checks, allocation and launch are native code (csrc/binding.cpp). rope() is
+# differentiable; the others, like the rest of the library, record no gradient.
 
 _native: ModuleType | None = None
 
@@ -268,7 +269,29 @@ _native: ModuleType | None = None
 def _bind() -> ModuleType:
     global _native
     _native = lib.native()
+    _native.set_rope(_Rope.apply)
     return _native
+
+
+class _Rope(torch.autograd.Function):
+    """``rope`` of a tensor that requires a gradient: the binding comes here where gradients are recorded.
+    The map is linear, so the gradient is its transpose, the same call with the other ``inverse``."""
+
+    @staticmethod
+    def forward(ctx, x, positions, freqs, interleaved, inverse, scale):  # noqa: ANN001, ANN205
+        ctx.save_for_backward(positions, freqs)
+        ctx.turn = (interleaved, inverse, scale)
+        return (_native or _bind()).rope(x, positions, freqs, interleaved, inverse, scale, None)
+
+    @staticmethod
+    def backward(ctx, g):  # noqa: ANN001, ANN205
+        positions, freqs = ctx.saved_tensors
+        interleaved, inverse, scale = ctx.turn
+        # autograd hands over any strides; what the kernel does not read in place is copied
+        if g.stride(2) != 1 or g.stride(0) % 8 or g.stride(1) % 8 or g.data_ptr() % 16:
+            g = g.clone(memory_format=torch.contiguous_format)
+        return rope(g, positions, freqs, interleaved=interleaved, inverse=not inverse,
+                    scale=scale), None, None, None, None, None
 
 
 def cache_slots(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor,
@@ -349,8 +372,8 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *, inter
     multiples of 8): the first 2 len(freqs) dimensions turn in pairs by positions[n] * freqs[i]
     and are scaled, the others are copied. Pairs are (i, i + rot / 2), or neighbours where
     ``interleaved``. ``inverse`` turns back: given the gradient of the output of a call, it is the
-    gradient of its input. positions int32 or int64 [tokens]; freqs fp64 (``rope_freqs``). ``out``
-    may be X itself."""
+    gradient of its input. Where X requires a gradient, autograd has it so; ``out`` is refused there.
+    positions int32 or int64 [tokens]; freqs fp64 (``rope_freqs``). ``out`` may be X itself."""
     return (_native or _bind()).rope(x, positions, freqs, interleaved, inverse, scale, out)
 
 

@@ -261,3 +261,13 @@ def test_rope_oracle_at_far_positions():
                  (96.0, 2**46 + 5), (-3.0, 2**51 - 1)):
         y = paged.rope(np.array([[[1.0, 0.0]]]), [n], [f], True)[0, 0]
         assert np.allclose(y, [math.cos(n * f), math.sin(n * f)], rtol=0, atol=4e-16), (f, n)
+
+
+def test_rope_of_a_tensor_that_needs_a_gradient_refuses_out():
+    """An output given by the caller has no history: the gradient would be lost without a word."""
+    x = torch.zeros(4, 2, 64, dtype=torch.bfloat16, requires_grad=True)
+    pos, freqs = torch.zeros(4, dtype=torch.int32), torch.zeros(16, dtype=torch.float64)
+    for args, out in (((x, pos, freqs), torch.zeros(4, 2, 64, dtype=torch.bfloat16)), ((x, pos, freqs), x),
+                      ((x.detach(), pos, freqs.clone().requires_grad_()), None)):
+        with pytest.raises(ValueError, match="gradient"):
+            ops.rope(*args, out=out)

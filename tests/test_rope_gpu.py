@@ -222,3 +222,71 @@ def test_positions_past_32_bits(cuda_device, freqs, interleaved):
         half = torch.finfo(torch.float16).eps / 2
         tiny = torch.finfo(torch.float16).smallest_normal * half
         assert (np.abs(got - want) <= fp32 + half * (np.abs(want) + fp32) + tiny).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved,inverse", [(False, False), (True, True)])
+def test_autograd(cuda_device, interleaved, inverse, dtype):
+    """The gradient of a loss over the output reaches the input: the formula's (the transpose, in float64),
+    for dense, broadcast and strided gradients, through views, and twice."""
+    from kta_b200 import ops
+
+    dev = cuda_device
+    freqs, _ = ops.rope_freqs(96, device=dev)
+    pos = torch.arange(7, 7 + 33, device=dev)
+    turn = dict(interleaved=interleaved, inverse=inverse, scale=1.25)
+
+    def want(g):
+        return paged.rope(g.double().cpu().numpy(), pos.tolist(), freqs.tolist(), interleaved, not inverse, 1.25)
+
+    fused = _x((33, 5, 128), dtype, 20).to(dev).requires_grad_()
+    x = fused[:, 1:4]
+    y = ops.rope(x, pos, freqs, **turn)
+    assert y.requires_grad and torch.equal(y, ops.rope(x.detach(), pos, freqs, **turn))
+    wide = _x((33, 3, 256), dtype, 21).to(dev)
+    for g in (wide[..., :128].contiguous(), wide[..., :128], wide[..., 4:132], wide[:, :, ::2],
+              wide[:1, :1, :1].expand(33, 3, 128)):
+        got, = torch.autograd.grad(y, fused, g, retain_graph=True)
+        _close(got[:, 1:4], g.double().cpu().numpy(), want(g), 1.25, 96, interleaved, dtype)
+        assert (got[:, 0] == 0).all() and (got[:, 4] == 0).all()
+    # linear: the gradient's own gradient, with respect to g, is the output of that direction
+    g = wide[..., :128].clone().requires_grad_()
+    first, = torch.autograd.grad(y, fused, g, create_graph=True)
+    h = _x((33, 5, 128), dtype, 22).to(dev)
+    second, = torch.autograd.grad(first, g, h)
+    assert torch.equal(second, ops.rope(h[:, 1:4], pos, freqs, **turn))
+    # one row for all heads: the heads' gradients are added up by autograd
+    one = _x((33, 1, 128), dtype, 23).to(dev).requires_grad_()
+    g = wide[:, :, :128].contiguous()
+    got, = torch.autograd.grad(ops.rope(one.expand(33, 3, 128), pos, freqs, **turn), one, g)
+    each = ops.rope(g, pos, freqs, interleaved=interleaved, inverse=not inverse, scale=1.25)
+    assert torch.equal(got, each.sum(1, keepdim=True))
+    with torch.no_grad():
+        assert not ops.rope(fused, pos, freqs, **turn).requires_grad
+        ops.rope(fused, pos, freqs, out=torch.empty_like(fused), **turn)
+
+
+def test_autograd_on_another_stream_and_captured(cuda_device):
+    from kta_b200 import ops
+
+    dev = cuda_device
+    freqs, _ = ops.rope_freqs(64, device=dev)
+    pos = torch.arange(40, device=dev)
+    x = _x((40, 4, 64), torch.bfloat16, 30).to(dev)
+    g = _x((40, 4, 64), torch.bfloat16, 31).to(dev)
+    want = ops.rope(g, pos, freqs, inverse=True)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    leaf = x.clone().requires_grad_()
+    with torch.cuda.stream(stream):
+        for _ in range(2):  # as torch asks for before a capture
+            got, = torch.autograd.grad(ops.rope(leaf, pos, freqs), leaf, g)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(ops.rope(leaf, pos, freqs), leaf, g)
+    got.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
