@@ -7,7 +7,9 @@ libcuda, cuBLAS or torch library is linked (the anti-cheat rule of
 src/kta/checks/anticheat.py:38-58 in the reference).
 
 Beside it, ``kta_b200/_binding.so`` (csrc/binding.cpp, g++): the Python binding of the entries
-whose calls are short, which uses torch's headers and links the library.
+whose calls are short, which uses torch's headers and links the library. It is left out, with a
+message, where g++, Python's headers or a CUDA build of torch are missing: the C library needs none
+of them.
 """
 
 from __future__ import annotations
@@ -88,33 +90,51 @@ def _run(cmd: list[str], what: str, verbose: bool) -> None:
         raise RuntimeError(f"{what} failed:\n{res.stdout}\n{res.stderr}")
 
 
-def _build_binding(verbose: bool) -> None:
-    """Compiles csrc/binding.cpp against the torch of this interpreter and the built library."""
+def _binding_command() -> tuple[list[str], bytes]:
+    """The binding's compiler command, against the torch of this interpreter and the built library,
+    and torch's version; raises LookupError for what is missing."""
     spec = importlib.util.find_spec("torch")
     if spec is None or not spec.submodule_search_locations:
-        raise RuntimeError("torch not found: the binding is built against its headers")
+        raise LookupError("torch not found")
     torch_dir = Path(spec.submodule_search_locations[0])
-    src = CSRC / "binding.cpp"
+    if not (torch_dir / "lib" / "libc10_cuda.so").exists():
+        raise LookupError("torch's CUDA libraries not found")
+    gxx = shutil.which("g++")
+    if gxx is None:
+        raise LookupError("g++ not found")
+    python = Path(sysconfig.get_paths()["include"])
+    if not (python / "Python.h").exists():
+        raise LookupError("Python.h not found")
     cuda = Path(nvcc()).resolve().parent.parent
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{INCLUDE}", f"-I{torch_dir}/include",
-           f"-I{torch_dir}/include/torch/csrc/api/include", f"-I{cuda}/include",
-           f"-I{sysconfig.get_paths()['include']}", str(src), "-o", str(BINDING),
+    cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{INCLUDE}", f"-I{torch_dir}/include",
+           f"-I{torch_dir}/include/torch/csrc/api/include", f"-I{cuda}/include", f"-I{python}",
+           str(CSRC / "binding.cpp"), "-o", str(BINDING),
            f"-L{torch_dir}/lib", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
            f"-L{PKG}", "-l:libkta_b200.so", "-Wl,-rpath,$ORIGIN"]
-    version = (torch_dir / "version.py").read_bytes()
-    h = hashlib.sha256(" ".join(cmd).encode() + src.read_bytes() + version)
+    return cmd, (torch_dir / "version.py").read_bytes()
+
+
+def _build_binding(verbose: bool) -> None:
+    stamp = BUILD / "binding.hash"
+    try:
+        cmd, version = _binding_command()
+    except LookupError as exc:
+        # one of an earlier build may not fit the library's entries
+        BINDING.unlink(missing_ok=True)
+        stamp.unlink(missing_ok=True)
+        print(f"binding not built: {exc} (the paged-cache functions of kta_b200.ops need it; the C "
+              "library does not)", file=sys.stderr)
+        return
+    h = hashlib.sha256(" ".join(cmd).encode() + (CSRC / "binding.cpp").read_bytes() + version)
     for hdr in sorted(INCLUDE.glob("*.h")):
         h.update(hdr.read_bytes())
-    stamp = BUILD / "binding.hash"
     if BINDING.exists() and stamp.exists() and stamp.read_text() == h.hexdigest():
         return
     _run(cmd, "building the binding", verbose)
     stamp.write_text(h.hexdigest())
 
 
-def build(verbose: bool = False, ptxas: bool = False) -> Path:
-    """Compiles and links the library and its binding; returns the library's path. Raises on any
-    compiler error."""
+def _build_library(verbose: bool, ptxas: bool) -> Path:
     BUILD.mkdir(exist_ok=True)
     extra = ["-Xptxas", "-v"] if ptxas else []
     srcs = sources()
@@ -127,8 +147,15 @@ def build(verbose: bool = False, ptxas: bool = False) -> Path:
     newest = max(Path(o).stat().st_mtime for o in objs)
     if not LIB.exists() or LIB.stat().st_mtime < newest:
         _run([nvcc(), *ARCH, "-shared", "-o", str(LIB), *objs], "link", verbose)
-    _build_binding(verbose)
     return LIB
+
+
+def build(verbose: bool = False, ptxas: bool = False) -> Path:
+    """Compiles and links the library and, where its needs are met, the binding; returns the library's
+    path. Raises on any compiler error."""
+    path = _build_library(verbose, ptxas)
+    _build_binding(verbose)
+    return path
 
 
 def main(argv: list[str]) -> int:
