@@ -154,13 +154,15 @@ void caches(const at::Tensor& k, const at::Tensor& v, const at::Tensor& q) {
   if (!k.is_contiguous() || !v.is_contiguous()) refuse("K and V caches must be contiguous");
 }
 
+// The lock is taken again on the way out of an exception too: a tensor without memory (a sparse one, one
+// that a tracer made) throws from data_ptr().
 template <typename F>
 int without_gil(F&& call) {
-  int status;
-  Py_BEGIN_ALLOW_THREADS;
-  status = call();
-  Py_END_ALLOW_THREADS;
-  return status;
+  struct Released {
+    PyThreadState* state = PyEval_SaveThread();
+    ~Released() { PyEval_RestoreThread(state); }
+  } released;
+  return call();
 }
 
 // Runs `body` with `n` arguments; a refusal becomes a ValueError, any other C++ exception the
