@@ -646,7 +646,8 @@ int launch(const void* Q, const void* Kc, const void* Vc, const void* tables, co
       max_blocks <= 0 || max_new <= 0) {
     return KTA_ERR_INVALID_ARG;
   }
-  if (!(scale > 0.f) || !std::isfinite(scale)) return KTA_ERR_INVALID_ARG;
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!(scale > 0.f) || !std::isfinite(scale_log2)) return KTA_ERR_INVALID_ARG;
   if (B > 1 && table_stride < max_blocks) return KTA_ERR_INVALID_ARG;
   if (!sizes_ok(max_new, Hq, Hkv, D) || B > MAX_BATCH) return KTA_ERR_UNSUPPORTED;
   if (block < 8 || block > 256 || (block & (block - 1)) != 0) return KTA_ERR_UNSUPPORTED;
@@ -705,7 +706,7 @@ int launch(const void* Q, const void* Kc, const void* Vc, const void* tables, co
   p.box_tokens = std::min(p.tok_tile, p.max_new);
   p.row_tiles = static_cast<int>(row_tiles);
   p.row_cap = ws.row_cap;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.scale_log2 = scale_log2;
   p.status = device_status_ptr();
   if (D == 64) return go<BF16, 64>(p, Q, Kc, Vc, q_token, stream);
   return go<BF16, 128>(p, Q, Kc, Vc, q_token, stream);

@@ -271,3 +271,21 @@ def test_rope_of_a_tensor_that_needs_a_gradient_refuses_out():
                       ((x.detach(), pos, freqs.clone().requires_grad_()), None)):
         with pytest.raises(ValueError, match="gradient"):
             ops.rope(*args, out=out)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_tree_attn_scale_in_its_own_units(dt):
+    """The kernel's scores are in powers of two: a scale whose scale * log2(e) is infinite makes NaN of
+    every masked key (-inf + inf), so it is refused like an infinite one."""
+    L = lib.load()
+    need = L.kta_tree_attn_workspace_bytes(1, 8, 2, 64)
+    largest = 3.4028235e38
+
+    def call(scale):
+        return getattr(L, f"kta_tree_attn_{dt}")(A, A, A, A, A, A, None, A + (1 << 20), A, 1, 1, 8, 2, 64, 512,
+                                                 4, 16, 2, 2, 1, scale, A, need, None)
+
+    for scale in (largest, largest / 1.4, math.inf, math.nan, 0.0, -0.0):
+        assert call(scale) == INVALID, scale
+    if NO_GPU:
+        assert call(largest / 1.5) == call(1e-30) == NO_DEVICE
