@@ -358,3 +358,43 @@ def test_offsets_past_32_bits(cuda_device):
     ops.rope_cache(q[:5], k, -k, pos, slots, freqs, big_k, big_v)
     assert torch.equal(big_k[-1, :5], k) and torch.equal(big_v[-1, :5], -k)
     assert _status() == 0
+
+
+@pytest.mark.parametrize("value", [-1, "past", 2**31 - 1, -2**31])
+@pytest.mark.parametrize("block,which", [(16, 3), (16, -1), (128, 1), (256, 0), (256, -1)])
+@pytest.mark.parametrize("max_new", [4, 64])  # one kernel and the other
+def test_a_block_out_of_range_reads_as_zeros(cuda_device, max_new, block, which, value):
+    """Of the context and of the drafted tokens, and one that is two boxes: the formula with zeros for its
+    K and V, in every row; stale tiles or another block's values would show."""
+    from kta_b200 import ops
+
+    c = Case([40, 900, 7], [4, 4, 4], 8, 2, 128, block, BF16, wide=1, seed=12)
+    c.run(cuda_device, max_new=max_new)
+    assert _status() == 0
+    q, kc, vc, tables, ctx, offsets = c.dev
+    last = -(-904 // block) - 1
+    at = last if which < 0 else which
+    moved = tables.clone()
+    moved[1, at] = c.blocks if value == "past" else value
+    c.kc[c.tables[1, at]] = 0
+    c.vc[c.tables[1, at]] = 0
+    out, lse = ops.tree_attn(q, kc, vc, moved, ctx, offsets, max_new, torch.from_numpy(c.bits).to(cuda_device))
+    c.check(out, lse)
+    assert _status() == 9
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("max_new", [6, 32])
+def test_large_scores_in_a_known_order(cuda_device, max_new, dtype):
+    """Blocks whose scores grow up to some hundreds, in rising, falling and mixed order."""
+    for order in ("up", "down", "mixed"):
+        c = Case([900, 600], [6, 6], 8, 2, 128, 16, dtype, seed=4)
+        c.q *= 8
+        grow = torch.linspace(0.1, 3.0, 57)
+        grow = {"up": grow, "down": grow.flip(0),
+                "mixed": grow[torch.randperm(57, generator=torch.Generator().manual_seed(5))]}[order].to(dtype)
+        for row in c.tables:
+            held = torch.from_numpy(row[row >= 0]).long()
+            c.kc[held] *= grow[:len(held), None, None, None]
+        c.check(*c.run(cuda_device, max_new=max_new))
+        assert _status() == 0
