@@ -618,7 +618,7 @@ int go(Params& p, const void* Q, const void* Kc, const void* Vc, int64_t q_token
   if (sms < p.row_tiles) return KTA_ERR_UNSUPPORTED;
   p.groups = sms / p.row_tiles;
   const int grid = p.groups * p.row_tiles;
-  // One tcgen05 tile has 128 rows in wide_kernel however few are real, and up to 64 in the other.
+  // One tcgen05 tile has 128 rows in wide_kernel however few are real, and 16 or 32 in the other.
   const bool narrow = p.box_tokens * p.group <= NARROW_ROWS;
   if (narrow) {
     s = launch_narrow<BF16, D>(p, tq, tk, tv, grid, stream);

@@ -138,13 +138,12 @@ __device__ __forceinline__ int row_tiles_of(const Params& p, int tokens) {
 // three rounds from a counter) measured 218 to 246 us where these take 202: what a cut unit costs is
 // more than the even end gives.
 constexpr int SWITCH = 3;
-constexpr int SWITCH_FROM = 1;  // tiles of a share from which on they are counted
 
 struct Shares {
   int total, n, extra;  // extra: what a unit counts beyond its tiles
   int length, longer;   // of a share, before it is rounded down to tiles; the first `longer` have one more
   __device__ __forceinline__ Shares(const Params& p, int tiles, int units) {
-    extra = tiles >= SWITCH_FROM * p.row_tiles * p.groups ? SWITCH : 0;
+    extra = tiles >= p.row_tiles * p.groups ? SWITCH : 0;  // a tile to a share, and more
     total = tiles + extra * units;
     // a share is at least (1 + extra) row_tiles long, so that it has a tile wherever it starts
     const int least = (1 + extra) * p.row_tiles;

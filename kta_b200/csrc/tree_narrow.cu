@@ -86,24 +86,14 @@ __device__ __forceinline__ void tmem_ld_16x256b(uint32_t taddr, uint32_t* r) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
                    "=r"(r[7])
                  : "r"(taddr));
-  } else if constexpr (N == 32) {
+  } else {
+    static_assert(N == 32);
     asm volatile(
         "tcgen05.ld.sync.aligned.16x256b.x4.b32"
         " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
           "=r"(r[15])
-        : "r"(taddr));
-  } else {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x8.b32"
-        " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
-        " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-          "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
-          "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
-          "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
   }
 }
@@ -640,6 +630,7 @@ int launch_narrow(const Params& p, const CUtensorMap& tq, const CUtensorMap& tk,
     return launch_ex(kernel, dim3(grid), dim3(NUM_THREADS), smem, stream, 1, tq, tk, tv, p);
   };
   const int rows = p.box_tokens * p.group;
+  static_assert(NARROW_ROWS == 32, "the most query rows of a kernel below");
   return rows <= 16 ? go(narrow_kernel<BF16, D, 16>, Narrow<D, 16>::TOTAL)
                     : go(narrow_kernel<BF16, D, 32>, Narrow<D, 32>::TOTAL);
 }
