@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             f2_split(shifted(c, i), x0, x1);
             const float e0 = ex2(x0), e1 = ex2(x1);
             sum[c] = add2(sum[c], f2(e0, e1));
-            pk[i] = pack2<BF16>(e0, e1);
+            pk[i] = pack2<BF16>(e0, e1);  // rounded as tree.cu explains; the sum is of e
           }
           stmatrix_x4_trans(p_row + buf * L::P_BUF + c * 1024, pk[0], pk[1], pk[2], pk[3]);
         }

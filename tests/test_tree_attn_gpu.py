@@ -398,3 +398,31 @@ def test_large_scores_in_a_known_order(cuda_device, max_new, dtype):
             c.kc[held] *= grow[:len(held), None, None, None]
         c.check(*c.run(cuda_device, max_new=max_new))
         assert _status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("max_new", [2, 6, 64])  # 8, 24 and 128 query rows
+@pytest.mark.parametrize("at", [3, 250, 399])
+def test_infinite_values_in_the_context(cuda_device, at, max_new, dtype):
+    """Every row sees them: one gives its infinity, two of different signs NaN, NaN itself; the other
+    dimensions are as they were, in requests that one CTA has and in ones that several share."""
+    for ctx in ([400, 30], [400, 60000]):
+        c = Case(ctx, [2, 2], 8, 2, 128, 16, dtype, seed=15)
+        c.q *= 0.25  # no weight is lost below the smallest number
+        want, want_lse = c.run(cuda_device, max_new=max_new)
+        c.check(want, want_lse)
+        block, place = c.tables[0, at // 16], at % 16
+        c.vc[block, place, 1, 5] = float("inf")
+        c.vc[block, place, 1, 6] = -float("inf")
+        c.vc[block, place, 1, 7] = float("nan")
+        c.vc[block, place, 1, 8] = float("inf")
+        c.vc[c.tables[0, 1], 1, 1, 8] = -float("inf")
+        out, lse = c.run(cuda_device, max_new=max_new)
+        o = out[:2, 4:].cpu()
+        assert (o[..., 5] == float("inf")).all() and (o[..., 6] == -float("inf")).all()
+        assert torch.isnan(o[..., 7:9]).all()
+        keep = [i for i in range(128) if not 5 <= i < 9]
+        assert torch.equal(o[..., keep], want[:2, 4:].cpu()[..., keep])
+        assert torch.equal(out[:2, :4], want[:2, :4]) and torch.equal(out[2:], want[2:])
+        assert torch.equal(lse, want_lse)
+        assert _status() == 0
