@@ -156,12 +156,16 @@ int kta_decode_gqa_bf16_noalloc(const void* Q, const void* Kc, const void* Vc,
  * table_stride elements; other entries are not touched), and lists the new tokens request after
  * request: slots (int64 [max_tokens]), positions (int32 [max_tokens]), offsets (int32 [B + 1],
  * request b's rows are offsets[b] .. offsets[b + 1]) and used (int32 [1], blocks taken). Rows past
- * the last token get slot -1 and position 0. Checked on the device, each recorded as
- * KTA_ERR_DEVICE_BOUNDS: a request with a negative length or more tokens than its table's row
- * holds is listed without new tokens; blocks past num_free are entered as -1, and their tokens'
- * slots are -1; tokens past max_tokens are cut off (offsets end at max_tokens). B <= 2048,
- * max_blocks * block_size < 2^31, max_tokens <= 2^30. No output overlaps an input or another
- * output. */
+ * the last token get slot -1 and position 0. free_blocks is read only and only context_lens says
+ * what a request holds, so before the next step the caller takes the first `used` ids off the
+ * list and, where context_lens ends up below context + new (drafts that were rejected), returns
+ * the entries of the table from ceil(context / block_size) on to it; with the same list twice,
+ * two requests share a block. A negative id in the list is no block: its tokens' slots are -1.
+ * Checked on the device, each recorded as KTA_ERR_DEVICE_BOUNDS: a request with a negative length
+ * or more tokens than its table's row holds is listed without new tokens; blocks past num_free
+ * are entered as -1, and their tokens' slots are -1; tokens past max_tokens are cut off (offsets
+ * end at max_tokens), but their blocks are taken. B <= 2048, max_blocks * block_size < 2^31,
+ * max_tokens <= 2^30. No output overlaps an input or another output. */
 int kta_cache_slots(const void* context_lens, const void* new_lens, void* block_tables,
                     const void* free_blocks, void* slots, void* positions, void* offsets, void* used,
                     int64_t B, int64_t max_blocks, int64_t table_stride, int64_t num_free,
@@ -173,9 +177,10 @@ int kta_cache_slots(const void* context_lens, const void* new_lens, void* block_
  * `inverse` turns by -t: the gradient with respect to X of the same call. X, Y [tokens, heads, D]
  * with token and head strides in elements (X's may be 0: one row for all); positions int32 or
  * int64 (pos_bytes 4 or 8, any sign), freqs fp64 [rot / 2] finite radians per position. The angle
- * is off by at most |position| 2^-64 turns and one fp32 rounding of what is left of it without whole
- * turns: 1e-7 rad below position 2^38, 3e-3 rad at 2^53. X and Y may be the same tensor, and must not overlap
- * otherwise. D % 16 == 0, D <= 1024, rot % 16 == 0, strides multiples of 8, 16-byte aligned X, Y. */
+ * is off by at most |position| 2^-64 turns (|freqs| < 2^40) and one fp32 rounding of what is left
+ * of it without whole turns: 1e-7 rad below position 2^38, 3e-3 rad at 2^53. X and Y may be the
+ * same tensor, and must not overlap otherwise. D % 16 == 0, D <= 1024, rot % 16 == 0, strides
+ * multiples of 8, 16-byte aligned X, Y. */
 int kta_rope_f16(const void* X, const void* positions, int64_t pos_bytes, const void* freqs, void* Y,
                  int64_t tokens, int64_t heads, int64_t D, int64_t rot, int64_t x_token,
                  int64_t x_head, int64_t y_token, int64_t y_head, int interleaved, int inverse,
@@ -188,10 +193,10 @@ int kta_rope_bf16(const void* X, const void* positions, int64_t pos_bytes, const
 /* The same for a step's Q [tokens, Hq, D] and K [tokens, Hkv, D] at once: Qo = rotated Q, and the
  * rotated K and the V go to slots[n] (int64 [tokens]) of the caches Kc, Vc (num_slots =
  * num_blocks * block_size rows of [Hkv, D]). A negative slot leaves the caches alone; one past
- * num_slots does too and is recorded as KTA_ERR_DEVICE_BOUNDS; two tokens with one slot leave
- * either's values there. `strides` points to eight host int64 values, token and head stride of Q,
- * K, V and Qo in elements (slices of one fused tensor will do). Qo may be Q; the caches overlap
- * no input. */
+ * num_slots does too and is recorded as KTA_ERR_DEVICE_BOUNDS; of two tokens with one slot, every
+ * 16 bytes there are one or the other's. `strides` points to eight host int64 values, token and
+ * head stride of Q, K, V and Qo in elements (slices of one fused tensor will do). Qo may be Q;
+ * the caches overlap no input. */
 int kta_rope_cache_f16(const void* Q, const void* K, const void* V, const void* positions,
                        int64_t pos_bytes, const void* slots, const void* freqs, void* Qo, void* Kc,
                        void* Vc, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t D, int64_t rot,
@@ -209,7 +214,8 @@ int kta_rope_cache_bf16(const void* Q, const void* K, const void* V, const void*
  * are offsets[b] .. offsets[b + 1] (int32 [B + 1]). Row i sees every cached token, and drafted
  * token j iff bit j of tree[i] (int64 [tokens]) is set; without a tree (NULL) the drafted tokens
  * are a chain, and one drafted token is a decode step. O = softmax(scale Q K^T) V over what a row
- * sees, LSE = natural log of the sum; a row that sees nothing has O = 0 and LSE = -inf; values of
+ * sees, LSE = natural log of the sum (weights are rounded to the storage type for the product with V;
+ * sums, O until its end and LSE are fp32); a row that sees nothing has O = 0 and LSE = -inf; values of
  * tokens that a row does not see do not reach it, infinities and NaN included. Rows that belong to
  * no request are left as they were. Q's token stride is q_token elements, its heads are D apart.
  * block_tables int32 [B, max_blocks], row stride table_stride. Checked on the device, recorded as

@@ -310,7 +310,12 @@ def cache_slots(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tables
     tokens, -1 and 0 behind the last one; ``offsets`` (int32 [B + 1], first row of each
     request); ``used`` (int32 [1], blocks taken). What of them is not given shares one allocation.
     What does not fit (a table's row, the free list, max_tokens) is cut off and recorded in the
-    device status block."""
+    device status block; blocks are taken for tokens past max_tokens too.
+
+    The free list is not changed. Before the next step the caller takes its first ``used`` ids off,
+    or other tokens get the same blocks; and where a request keeps fewer tokens than it had new ones
+    (rejected drafts), the ids of its table from ceil(context_lens / block_size) on go back to the
+    list, or nobody has them any more. A negative id in the list is no block (slots -1)."""
     return (_native or _bind()).cache_slots(context_lens, new_lens, block_tables, free_blocks,
                                             block_size, max_tokens, slots, positions, offsets, used)
 
@@ -384,8 +389,8 @@ def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: tor
     """Rotary positions of a step's Q [tokens, Hq, D] and K [tokens, Hkv, D] (``rope``), with the
     rotated K and the V written to ``slots`` (int64 [tokens], ``cache_slots``) of the paged caches
     [num_blocks, block_size, Hkv, D]; a negative slot writes nothing, and one that occurs twice
-    holds either token's values. Returns the rotated Q (``out`` may be Q itself). Q, K and V may be
-    slices of one fused tensor."""
+    holds a mixture of both tokens' values. Returns the rotated Q (``out`` may be Q itself). Q, K
+    and V may be slices of one fused tensor."""
     return (_native or _bind()).rope_cache(q, k, v, positions, slots, freqs, k_cache, v_cache,
                                            interleaved, scale, out)
 
@@ -407,7 +412,7 @@ def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     and max_new = 1 is a decode step. Caches [num_blocks, block_size, Hkv, D], block_tables int32
     [B, max_blocks]. Returns O [tokens, Hq, D] and LSE fp32 [tokens, Hq] (natural log, to merge
     with attention over other keys); a row that sees nothing has O = 0 and LSE = -inf, rows of no
-    request are left as they were.
+    request are left as they were. Softmax weights are rounded to Q's type for the product with V.
 
     Q's heads are contiguous, its tokens at any stride (a slice of a fused tensor will do); ``out``
     and ``lse`` are contiguous and overlap no input. ``workspace`` (uint8,

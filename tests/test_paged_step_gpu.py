@@ -167,3 +167,75 @@ def test_two_streams_at_once(cuda_device):
     for one, two in zip(*made):
         for a, b in zip(one, two):
             assert torch.equal(a, b)
+
+
+def _after(free, used, tables, ctx, new, kept):
+    """What a server does between steps, on the device: ids that were taken leave the free list, those of
+    blocks behind the tokens it keeps return to it, and no list or length passes through the host."""
+    column = torch.arange(tables.shape[1], device=tables.device)
+    back = (column >= -(-kept // BLOCK)[:, None]) & (column < -(-(ctx + new) // BLOCK)[:, None])
+    rest = (torch.arange(len(free), device=free.device) >= used) & (free >= 0)
+    live, ids = torch.cat([rest, back.flatten()]), torch.cat([free, tables.flatten()])
+    order = torch.argsort(live.logical_not().byte(), stable=True)[:len(free)]  # the live ones first
+    free.copy_(torch.where(live, ids, -1)[order])
+    ctx.copy_(kept)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_pool_that_only_the_device_knows(cuda_device, captured):
+    """Steps with rejected drafts, the free list kept on the device and the whole of it replayed as one
+    graph: no block has two owners, none is lost, and every kept token's V is where the table says."""
+    from kta_b200 import lib, ops
+
+    dev, batch, blocks, heads, d = cuda_device, 6, 40, 2, 64
+    g = np.random.default_rng(3)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    free = i32(g.permutation(blocks).tolist())
+    tables = torch.full((batch, 12), -1, dtype=torch.int32, device=dev)
+    ctx, new, kept = (torch.zeros(batch, dtype=torch.int32, device=dev) for _ in range(3))
+    kc = torch.zeros((blocks, BLOCK, heads, d), dtype=torch.bfloat16, device=dev)
+    vc = torch.zeros_like(kc)
+    freqs, _ = ops.rope_freqs(d, device=dev)
+    x = torch.zeros((ROWS, 3 * heads, d), dtype=torch.bfloat16, device=dev)
+
+    def step():
+        slots, pos, offsets, used = ops.cache_slots(ctx, new, tables, free, BLOCK, ROWS)
+        q, k, v = x.split(heads, 1)
+        q = ops.rope_cache(q, k, v, pos, slots, freqs, kc, vc)
+        out, _ = ops.tree_attn(q, kc, vc, tables, ctx, offsets, MOST)
+        _after(free, used, tables, ctx, new, kept)
+        return offsets, out
+
+    if captured:
+        for _ in range(2):
+            step()  # no new tokens: nothing moves
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            result = step()
+    held = [np.zeros((0, heads, d)) for _ in range(batch)]
+    for i in range(12):
+        n = g.integers(0, 17, batch) if i else np.array([16, 1, 15, 17, 0, 24])
+        keep = np.array([int(g.integers(0, m + 1)) for m in n])
+        if i % 4 == 3:  # a request ends: all of its blocks return
+            keep[i % batch] = -len(held[i % batch])
+        x.copy_(torch.from_numpy(g.standard_normal(x.shape)).to(torch.bfloat16))
+        new.copy_(i32(n.tolist()))
+        kept.copy_(i32([len(h) + int(m) for h, m in zip(held, keep)]))
+        if captured:
+            graph.replay()
+        else:
+            result = step()
+        torch.cuda.synchronize()
+        v, offsets = x[:, 2 * heads:].double().cpu().numpy(), result[0].tolist()
+        assert offsets == [0, *np.cumsum(n).tolist()]
+        table, pool, cache = tables.tolist(), free.tolist(), vc.double().cpu().numpy()
+        owned = []
+        for b in range(batch):
+            held[b] = np.concatenate([held[b], v[offsets[b]:offsets[b + 1]]])[:len(held[b]) + keep[b]]
+            ids = table[b][:-(-len(held[b]) // BLOCK)]
+            assert np.array_equal(cache[ids].reshape(-1, heads, d)[:len(held[b])], held[b])
+            owned += ids
+        assert sorted(owned + [f for f in pool if f >= 0]) == list(range(blocks))
+        assert pool[len(pool) - len(owned):] == [-1] * len(owned)
+    assert lib.device_status(clear=True)[0] == 0
