@@ -17,14 +17,15 @@
 // vectors half a region apart (rotated region or rest), which is the pair of the half layout and
 // in every layout keeps a warp's loads and stores contiguous.
 //
-// Small CTAs with two items to a thread in flight, and streaming loads and stores: 32768 x 32 heads
-// take 89.3 us (6010 GB/s; a plain copy of as many bytes 82.5) against 97.6 with 256 threads and
-// four items, 101 to 127 with 512 threads or without the streaming hints. Few tokens are latency:
-// there a thread has one item, and a token's heads are spread over several CTAs (512 tokens of 48
-// heads: 4.3 us with one item to a thread, 5.6 with 256 threads and four; 64 tokens 1.85 us). With few
-// heads the angles are the work: a thread keeps its pair where it can, and its frequency's fraction
-// (32768 tokens of one head 13.6 us without, 9.8 so with more tokens to a CTA). With the
-// cache write, 16384 tokens of 48 heads: 64.3 us, 6260 GB/s.
+// Figures of replayed graphs. Small CTAs with two items to a thread in flight, and streaming loads and
+// stores: 32768 x 32 heads take 89.3 us (6010 GB/s; a plain copy of as many bytes 82.5) against 97.6
+// with 256 threads and four items, 101 to 127 with 512 threads or without the streaming hints. Few
+// tokens are latency: there a thread has one item, and a token's heads are spread over several CTAs
+// (512 tokens of 48 heads: 4.3 us with one item to a thread, 5.6 with 256 threads and four; 64 tokens
+// 1.8 us). With few heads the angles are the work: a thread keeps its pair where it can, and its
+// frequency's fraction (32768 tokens of one head 13.6 us without, 10.1 so with more tokens to a CTA).
+// With the cache write, 16384 tokens of 48 heads: 64.3 us, 6260 GB/s. Single calls on changing inputs,
+// one after the other: 96.1 us (5590 GB/s) and 66.9 (6020).
 #include <algorithm>
 #include <cmath>
 
@@ -317,9 +318,10 @@ int go(Params& p, int64_t D, bool interleaved, cudaStream_t stream) {
   }
   const long long per_token = static_cast<long long>(p.rows) * p.items;
   const int sms = current_sm_count();
-  // One item to a thread while all of them are resident at once (2048 threads to an SM), if a token
-  // fills a CTA: 1024 tokens of 32 heads take 5.4 us so and 5.7 the other way, 2400 tokens 9.6 and
-  // 9.4; 9400 tokens of 4 heads 11.2 and 6.5.
+  // One item to a thread while all of them are resident at once (2048 threads to an SM; 1184 tokens of
+  // 32 heads of 128 at 148 SMs), if a token fills a CTA. 1024 tokens of 32 heads take 5.4 us so and 5.7
+  // the other way; 2400, past the limit, would take 9.6 us so and take 9.4 the other way. 9400 tokens of
+  // 4 heads, which do not fill a CTA, 11.2 and 6.5.
   if (per_token >= THREADS && p.tokens * per_token <= 2048LL * sms) {
     p.per_cta = 1;
     const dim3 grid(p.tokens, static_cast<unsigned>((per_token + THREADS - 1) / THREADS));

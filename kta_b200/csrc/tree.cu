@@ -37,8 +37,9 @@
 //     request's rows are zero (LSE -inf), such a block reads as zeros. Every wait is bounded.
 //
 // wide_kernel, tensor- and power-bound. 32 trees of 33 to 64 tokens with 8 heads to a KV head, over
-// 2048 to 8192 keys: 350 to 400 us (800 to 700 TFLOP/s of the rows that exist, 14 % more with their
-// padding), the SMs at 1.54 to 1.6 GHz under the 1000 W cap and ~1930 cycles to a 128 x 128 tile.
+// 2048 to 8192 keys: 404 us in a long run of calls (690 TFLOP/s of the rows that exist, 14 % more with
+// their padding), 344 to 375 in short ones, the SMs at 1.54 to 1.6 GHz under the 1000 W cap and ~1930
+// cycles to a 128 x 128 tile.
 //
 //   * Warps 0-3 and 4-7 are two softmax warpgroups: each takes 64 keys of every tile (thread = query
 //     row = TMEM lane) and has its own O, maximum and sum, so that neither waits for the other before
@@ -615,7 +616,10 @@ int go(Params& p, const void* Q, const void* Kc, const void* Vc, int64_t q_token
   const uint64_t strides[4] = {token, 128, 8 * token, D * 2};
   const uint32_t box[5] = {64, 8, L::HALVES, (1u << p.box_log2) / 8, 1};
   // A token's row of a head is 128 or 256 bytes: promoted to more, L2 would fetch the next head's too
-  // (64 x 8000 keys, 8 KV heads of 64: 185 us, 237 with 256 bytes; rings of six tiles there 190).
+  // (64 x 8000 keys, 8 KV heads of 64: 185 us, 237 with 256 bytes; rings of six tiles there 190; 2 KV
+  // heads of 64 over 30000 keys 168 and 217). With one KV head the next row is the next token's: 167 us
+  // either way for 64 x 60000 keys. Heads of 128: 325 either way, 64 requests of 8 tokens 196.7 with 256
+  // bytes and 197.4 with 128.
   const auto promotion = D == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
   int s = encode_tmap(&tk, type, 5, Kc, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, promotion);
   if (s != KTA_OK) return s;

@@ -130,9 +130,11 @@ __device__ __forceinline__ int row_tiles_of(const Params& p, int tokens) {
 // row tile of its request, in equal shares for `row_tiles` CTAs each (a share's members). A segment's
 // start and end cost a CTA about as much as SWITCH tiles (with equal numbers of tiles, shares of 3
 // segments had their keys at 183 us and shares of 10 at 215), so every unit counts so many more, ahead
-// of its first tile: 64 single tokens of 8 KV heads over 64 to 512 keys 36.6 us, 42.0 with equal
-// numbers of tiles; 32 over 256 to 1024 keys 29.9 and 32.2. Not where a share has less than a tile
-// (one request of 4 tokens over 1024 keys 15.0 us, 16.3 with them counted).
+// of its first tile: 64 requests of 8 tokens, 8 KV heads, over 1024 to 8192 keys 196.4 us, 198.4 with
+// equal numbers of tiles; 64 single tokens over 64 to 512 keys 25.6 and 26.6; 16 trees of 33 to 64 tokens
+// of 8 heads over 500 to 2000 keys 66 and 74; but 32 single tokens over 256 to 1024 keys 24.3 and 23.3.
+// Not where a share has less than a tile (one request of 4 tokens over 1024 keys 15.0 us, 16.3 with
+// them counted, when a segment's start cost more than it does now).
 //
 // Shares that are taken as they are finished (the first 78 to 88 % to each CTA, the rest in one to
 // three rounds from a counter) measured 218 to 246 us where these take 202: what a cut unit costs is
