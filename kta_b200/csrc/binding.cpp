@@ -100,6 +100,11 @@ class On {
   c10::cuda::OptionalCUDAGuard guard_;
 };
 
+// Counts a call's write to a tensor of the caller: autograd compares versions before it uses what it kept.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // A contiguous 1-D tensor of `type`, of n elements where n >= 0.
 void vector(const at::Tensor& t, at::ScalarType type, int64_t n, const char* name) {
   if (t.scalar_type() != type || t.dim() != 1 || !t.is_contiguous() || (n >= 0 && t.size(0) != n)) {
@@ -231,6 +236,7 @@ PyObject* cache_slots(PyObject*, PyObject* const* args, Py_ssize_t n) {
                              dev.stream());
     });
     if (!passed("kta_cache_slots", status)) return nullptr;
+    for (const at::Tensor* t : {&tables, &slots, &positions, &offsets, &used}) written(*t);
     PyObject* r = PyTuple_New(4);
     if (r == nullptr) return nullptr;
     PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(slots));
@@ -276,6 +282,7 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
                    row_stride(out, 0), row_stride(out, 1), inter, inverse, scale, dev.stream());
     });
     if (!passed(bf16 ? "kta_rope_bf16" : "kta_rope_f16", status)) return nullptr;
+    written(out);
     return THPVariable_Wrap(out);
   });
 }
@@ -321,6 +328,7 @@ PyObject* rope_cache(PyObject*, PyObject* const* args, Py_ssize_t n) {
                    dev.stream());
     });
     if (!passed(bf16 ? "kta_rope_cache_bf16" : "kta_rope_cache_f16", status)) return nullptr;
+    for (const at::Tensor* t : {&kc, &vc, &out}) written(*t);
     return THPVariable_Wrap(out);
   });
 }
@@ -383,6 +391,7 @@ PyObject* tree_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
                    ws.data_ptr(), ws.nbytes(), dev.stream());
     });
     if (!passed(bf16 ? "kta_tree_attn_bf16" : "kta_tree_attn_f16", status)) return nullptr;
+    for (const at::Tensor* t : {&out, &lse}) written(*t);
     PyObject* r = PyTuple_New(2);
     if (r == nullptr) return nullptr;
     PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(out));

@@ -390,7 +390,7 @@ def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: tor
     rotated K and the V written to ``slots`` (int64 [tokens], ``cache_slots``) of the paged caches
     [num_blocks, block_size, Hkv, D]; a negative slot writes nothing, and one that occurs twice
     holds a mixture of both tokens' values. Returns the rotated Q (``out`` may be Q itself). Q, K
-    and V may be slices of one fused tensor."""
+    and V may be slices of one fused tensor. For serving: no gradient is recorded."""
     return (_native or _bind()).rope_cache(q, k, v, positions, slots, freqs, k_cache, v_cache,
                                            interleaved, scale, out)
 
