@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               uint32_t pk[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
-                pk[e] = pack2<BF16>(__uint_as_float(o[16 * i + 2 * e]), __uint_as_float(o[16 * i + 2 * e + 1]));
+                pk[e] = pack_o<BF16>(__uint_as_float(o[16 * i + 2 * e]), __uint_as_float(o[16 * i + 2 * e + 1]));
               }
               st_global_v8(dst + 16 * i, pk);
             }
@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Params p) {
     const long long at =
         static_cast<long long>(d.row + tok) * p.hq + d.kvh * p.group + (row - tok * p.group);
     uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at * D + d4 * 4);
-    *dst = make_uint2(pack2<BF16>(o.x * inv, o.y * inv), pack2<BF16>(o.z * inv, o.w * inv));
+    *dst = make_uint2(pack_o<BF16>(o.x * inv, o.y * inv), pack_o<BF16>(o.z * inv, o.w * inv));
     if (d4 == 0) p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
   }
 }

@@ -432,6 +432,21 @@ __device__ __forceinline__ float load16(const void* base, long long i) {
   }
 }
 
+// Two elements of O. A weighted mean is never beyond its values, but the rounding of the weights (up to
+// 2^-11) can carry a mean of f16's largest numbers past 65520, which would become infinite: what is
+// finite stays so. (A bf16 mean would be infinite in fp32 already.)
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_o(float a, float b) {
+  if constexpr (!BF16) {
+    const auto within = [](float x) {
+      return fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
+    };
+    a = within(a);
+    b = within(b);
+  }
+  return pack2<BF16>(a, b);
+}
+
 // The bits of drafted token t (in its request of `tokens`): the drafted tokens that it sees.
 __device__ __forceinline__ uint64_t bits_of(const Params& p, int row, int t, int tokens) {
   const uint64_t bits = p.tree != nullptr ? static_cast<uint64_t>(p.tree[row + t])

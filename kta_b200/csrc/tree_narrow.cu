@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           v = fmaf(__uint_as_float(o[3][i]), wt.w, v);
           if (c + i < rows && d < D) {
             if (whole) {
-              out[at] = static_cast<uint16_t>(pack2<BF16>(v, 0.f) & 0xffffu);
+              out[at] = static_cast<uint16_t>(pack_o<BF16>(v, 0.f) & 0xffffu);
             } else {
               part[(c + i) * D] = v;
             }

@@ -426,3 +426,31 @@ def test_infinite_values_in_the_context(cuda_device, at, max_new, dtype):
         assert torch.equal(out[:2, :4], want[:2, :4]) and torch.equal(out[2:], want[2:])
         assert torch.equal(lse, want_lse)
         assert _status() == 0
+
+
+@pytest.mark.parametrize("max_new", [2, 7, 64])  # 8, 28 and 128 query rows
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_mean_of_the_largest_numbers_is_finite(cuda_device, d, max_new):
+    """A weighted mean is never beyond its values: where every V is f16's largest number (clipped
+    activations), O is that, and not infinite because the weights were rounded. Here all but one of a
+    row's weights are 0.5003 of the first one's: f16 has 0.50049, 4e-4 more, and 65504 (1 + 2^-12) is
+    rounded to infinity."""
+    scale = -np.log(0.5003)
+    c = Case([31, 0, 40, 3000], [2, 2, 1, 2], 8, 2, d, 16, F16, seed=16)
+    c.q.zero_()
+    c.q[..., 0] = 1
+    top = torch.finfo(F16).max
+    sign = 1 - 2.0 * (torch.arange(d) % 3 == 0)
+    for b, (n, m) in enumerate(zip(c.ctx, c.new)):
+        for p in range(n + m):
+            c.kc[c.tables[b, p // 16], p % 16] = 0
+            c.kc[c.tables[b, p // 16], p % 16, :, 0] = -1.0 if p else 0.0
+            c.vc[c.tables[b, p // 16], p % 16] = (top * sign).to(F16)
+    out, lse = c.run(cuda_device, max_new=max_new, scale=scale)
+    assert torch.isfinite(out).all()
+    c.check(out, lse, scale=scale)
+    # what is infinite stays so
+    c.vc[c.tables[3, 2], 5, 1, 7] = float("inf")
+    out, _ = c.run(cuda_device, max_new=max_new, scale=scale)
+    assert (out[5:, 4:, 7] == float("inf")).all() and torch.isfinite(out[5:, :4]).all()
+    assert _status() == 0
