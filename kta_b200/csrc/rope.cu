@@ -318,8 +318,8 @@ int go(Params& p, int64_t D, bool interleaved, cudaStream_t stream) {
   }
   const long long per_token = static_cast<long long>(p.rows) * p.items;
   const int sms = current_sm_count();
-  // One item to a thread while all of them are resident at once (2048 threads to an SM; 1184 tokens of
-  // 32 heads of 128 at 148 SMs), if a token fills a CTA. 1024 tokens of 32 heads take 5.4 us so and 5.7
+  // One item to a thread while they are little more than the SMs hold at once (1536 threads each; the
+  // limit of 2048 is 1184 tokens of 32 heads of 128 at 148 SMs), if a token fills a CTA. 1024 tokens of 32 heads take 5.4 us so and 5.7
   // the other way; 2400, past the limit, would take 9.6 us so and take 9.4 the other way. 9400 tokens of
   // 4 heads, which do not fill a CTA, 11.2 and 6.5.
   if (per_token >= THREADS && p.tokens * per_token <= 2048LL * sms) {
